@@ -12,7 +12,13 @@ LIB_PATH = os.environ.get("DM_SAMPLER_LIB", os.path.join(_HERE, "libdm_sampler.s
 
 _lib = None
 
-_vp, _sz, _i, _f = C.c_void_p, C.c_size_t, C.c_int, C.c_float
+_vp, _sz, _i, _f, _l = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_int64
+
+
+class RotaryTensor(C.Structure):
+    """dm_rotary_tensor"""
+    _fields_ = [("in_", _vp), ("out", _vp), ("in_stride", _l * 3), ("out_stride", _l * 3), ("heads", _i)]
+
 
 _SIGS = {
     "dm_last_error": (C.c_char_p, []),
@@ -54,9 +60,19 @@ _SIGS = {
     "dm_groupnorm_silu": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp]),
     "dm_conv2d": (_i, [_i, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _f, _vp, _vp, _vp, _i, _vp, _vp,
                        _i, _i, _i, _vp]),
+    "dm_layer_norm": (_i, [_vp, _l, _vp, _vp, _i, _vp, _vp, _vp, _l, _i, _f, _i, _vp]),
+    "dm_layer_norm_backward_workspace_bytes": (_sz, [_l, _i]),
+    "dm_layer_norm_backward": (_i, [_vp, _l, _vp, _l, _vp, _i, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _vp, _sz, _vp]),
+    "dm_rotary": (_i, [C.POINTER(RotaryTensor), C.POINTER(RotaryTensor), _vp, C.POINTER(_l), _i, _vp, _l, _l, _i, _i, _i, _f, _i, _i, _vp]),
+    "dm_gated_ffn_saved_bytes": (_sz, [_l, _i, _i]),
+    "dm_gated_ffn_workspace_bytes": (_sz, [_l, _i, _i, _i, _i]),
+    "dm_gated_ffn": (_i, [_vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "dm_gated_ffn_backward_workspace_bytes": (_sz, [_l, _i, _i, _i, _i]),
+    "dm_gated_ffn_backward": (_i, [_vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp,
+                                   _sz, _vp]),
 }
 EXPORTS = tuple(_SIGS)
-ABI_VERSION = 4  # include/dm_sampler.h: DM_ABI_VERSION
+ABI_VERSION = 5  # include/dm_sampler.h: DM_ABI_VERSION
 CHUNK_FN = C.CFUNCTYPE(_vp, _vp, _i, _i)  # dm_chunk_fn
 
 

@@ -37,6 +37,13 @@ int fail(const char* fmt, ...) {
   return 1;
 }
 
+}  // namespace
+__attribute__((visibility("hidden"))) int dm_set_error(const char* msg) {  // for the other translation units of the library
+  g_err = msg;
+  return 1;
+}
+namespace {
+
 #define HIP_TRY(expr)                                                                   \
   do {                                                                                  \
     hipError_t e_ = (expr);                                                             \

@@ -1,0 +1,556 @@
+// dm_block_ffn.hip — the gated feed-forward block and its gradients.
+//   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) u, y = h Wd^T + bd
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h, biases: column sums.
+// Both projections, the activation and the product are one kernel; so are dh, dg, du and the h that dWd needs (recomputed from g and u,
+// which the forward pass keeps for training).  Two paths: up to SKINNY_ROWS rows (decode) the weights' bandwidth bounds the block and
+// every wave streams weight rows straight into matrix instructions; above that the tiled products of dm_block_gemm.hip.
+// Rounding: g, u, dg, du and h are kept in the tensors' type between the products (16-bit: the matrix pipe takes nothing wider), every
+// sum is fp32.  fp32 tensors are split into three bf16 terms and multiplied as six products (a1b1 a1b2 a2b1 a2b2 a1b3 a3b1; what is left
+// out is below 2^-25 of |a||b|).
+#include <type_traits>
+
+#include "dm_block_gemm.hip"
+
+namespace dmb {
+
+constexpr int SKINNY_ROWS = 64;
+
+// ---- operands that the products cannot read as they are: fp32 (three bf16 planes) and rows of no whole number of 16-byte pieces
+template <typename S, typename D, bool PLANES>
+__global__ void __launch_bounds__(256)
+pack_rows_kernel(const S* __restrict__ src, int64_t ld, D* __restrict__ dst, int64_t plane, int64_t rows, int cols, int pitch) {
+  const int pieces = pitch / 8;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < rows * pieces; id += (int64_t)gridDim.x * 256) {
+    const int64_t r = id / pieces;
+    const int c = (int)(id % pieces) * 8;
+    const S* s = src + r * ld + c;
+    S v[8];
+    if (sizeof(S) == 4 && c + 8 <= cols && ((uintptr_t)s & 15) == 0) {
+      const Vec<S, 4> a = *reinterpret_cast<const Vec<S, 4>*>(s), b = *reinterpret_cast<const Vec<S, 4>*>(s + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { v[i] = a.v[i]; v[4 + i] = b.v[i]; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? s[i] : (S)0.f;
+    }
+    if constexpr (PLANES) {
+      Vec<bf16, 8> o[3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { bf16 t[3]; split3((float)v[i], t); o[0].v[i] = t[0]; o[1].v[i] = t[1]; o[2].v[i] = t[2]; }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<bf16, 8>*>(dst + k * plane + r * pitch + c) = o[k];
+    } else {
+      Vec<D, 8> o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o.v[i] = (D)v[i];
+      *reinterpret_cast<Vec<D, 8>*>(dst + r * pitch + c) = o;
+    }
+  }
+}
+
+// ---- column sums of one or two [M][C] arrays of PL planes: part[block row][2][C], joined by partial_rows_kernel
+template <typename T, int PL>
+__global__ void __launch_bounds__(64)
+column_sums_kernel(const T* __restrict__ p0, const T* __restrict__ p1, int64_t plane, int64_t ld, int64_t M, int C, float* __restrict__ part) {
+  const int c = (blockIdx.x * 64 + threadIdx.x) * 4;
+  if (c >= C) return;
+  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool vec = ld % 4 == 0 && c + 4 <= C && ((uintptr_t)p0 & (4 * sizeof(T) - 1)) == 0;
+  auto add = [&](const T* p, int64_t m, float (&s)[4]) {
+#pragma unroll
+    for (int k = 0; k < PL; ++k) {
+      const T* r = p + k * plane + m * ld + c;
+      if (vec) {
+        float v[4];
+        load_vec<T, 4>(r, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < C) s[e] += (float)r[e];
+      }
+    }
+  };
+#pragma unroll 4
+  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+    add(p0, m, s0);
+    if (p1) add(p1, m, s1);
+  }
+  float* o = part + (int64_t)blockIdx.y * 2 * C + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < C) { o[e] = s0[e]; o[C + e] = s1[e]; }
+}
+inline int column_sums_rows(int64_t M, int C) {
+  const int64_t want = 4096 / ((C + 255) / 256);
+  const int64_t r = want < 1 ? 1 : want > 512 ? 512 : want;
+  return (int)(r < M ? r : M);
+}
+
+// ---- up to SKINNY_ROWS rows
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Skinny;
+template <> struct Skinny<bf16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ f32x4 mul(const Vec<bf16, 8>& a, const Vec<bf16, 8>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Skinny<f16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ f32x4 mul(const Vec<f16, 8>& a, const Vec<f16, 8>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Skinny<float> {  // four instructions of four k each: instruction i takes element i of every lane's piece, on both sides
+  static constexpr int V = 4;
+  static __device__ __forceinline__ f32x4 mul(const Vec<float, 4>& a, const Vec<float, 4>& b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_piece(const T* row, int k, int K, bool vec) {
+  Vec<T, V> r;
+  if (vec) {
+    if (k < K) return *reinterpret_cast<const Vec<T, V>*>(row + k);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = (T)0.f;
+    return r;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = k + i < K ? row[k + i] : (T)0.f;
+  return r;
+}
+
+constexpr int SKINNY_WAVES = 8;
+
+// out[m, n] for 16 n per block: the waves deal the k range among themselves in pieces, and their sums meet in LDS.
+template <typename T, int MT, bool GATE, bool VEC>
+__global__ void __launch_bounds__(SKINNY_WAVES * 64)
+skinny_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ w, const T* __restrict__ w2, int64_t ldw, const T* __restrict__ bias,
+              const T* __restrict__ bias2, T* __restrict__ out, int64_t ldo, T* __restrict__ g_out, T* __restrict__ u_out, int M, int N, int K, int act) {
+  constexpr int V = Skinny<T>::V, STEP = 4 * V, P = GATE ? 2 : 1;
+  __shared__ f32x4 red[SKINNY_WAVES][P][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = blockIdx.x * 16 + (lane & 15);
+  const int nc = n < N ? n : N - 1;
+  const T* w1r = w + nc * ldw;
+  const T* w2r = GATE ? w2 + nc * ldw : nullptr;
+  const T* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int m = t * 16 + (lane & 15);
+    xr[t] = x + (m < M ? m : M - 1) * xs;
+  }
+  f32x4 acc[P][MT] = {};
+  constexpr int U = 4;  // pieces in flight
+  for (int k0 = wave * STEP; k0 < K; k0 += SKINNY_WAVES * STEP * U) {
+    Vec<T, V> a[U], a2[U], b[U][MT];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = k0 + i * SKINNY_WAVES * STEP + (lane >> 4) * V;
+      a[i] = load_piece<T, V>(w1r, k, K, VEC);
+      if (GATE) a2[i] = load_piece<T, V>(w2r, k, K, VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = k0 + i * SKINNY_WAVES * STEP + (lane >> 4) * V;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) b[i][t] = load_piece<T, V>(xr[t], k, K, VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        acc[0][t] = Skinny<T>::mul(a[i], b[i][t], acc[0][t]);
+        if constexpr (GATE) acc[1][t] = Skinny<T>::mul(a2[i], b[i][t], acc[1][t]);
+      }
+  }
+#pragma unroll
+  for (int q = 0; q < P; ++q)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[wave][q][t][lane] = acc[q][t];
+  __syncthreads();
+  if (wave >= MT) return;
+  f32x4 s[P];
+#pragma unroll
+  for (int q = 0; q < P; ++q) {
+    s[q] = red[0][q][wave][lane];
+#pragma unroll
+    for (int v = 1; v < SKINNY_WAVES; ++v) s[q] += red[v][q][wave][lane];
+  }
+  const int m = wave * 16 + (lane & 15);
+  if (m >= M) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = blockIdx.x * 16 + (lane >> 4) * 4 + e;
+    if constexpr (GATE) {
+      if (c >= ((N + 7) & ~7)) continue;
+      float g = 0.f, u = 0.f;  // the padding of a row holds zeros
+      if (c < N) {
+        g = s[0][e] + (bias ? (float)bias[c] : 0.f);
+        u = s[P - 1][e] + (bias2 ? (float)bias2[c] : 0.f);
+      }
+      const int64_t at = (int64_t)m * ldo + c;
+      out[at] = (T)(c < N ? act_value(act, g) * u : 0.f);
+      if (g_out) { g_out[at] = (T)g; u_out[at] = (T)u; }
+    } else {
+      if (c >= N) continue;
+      out[(int64_t)m * ldo + c] = (T)(s[0][e] + (bias ? (float)bias[c] : 0.f));
+    }
+  }
+}
+
+template <typename T, bool GATE, bool VEC>
+int skinny_launch(const T* x, int64_t xs, const T* w, const T* w2, int64_t ldw, const T* bias, const T* bias2, T* out, int64_t ldo, T* g, T* u,
+                  int M, int N, int K, int act, hipStream_t st) {
+  const dim3 grid((N + 15) / 16), block(SKINNY_WAVES * 64);
+  switch ((M + 15) / 16) {
+    case 1: skinny_kernel<T, 1, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, g, u, M, N, K, act); break;
+    case 2: skinny_kernel<T, 2, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, g, u, M, N, K, act); break;
+    default: skinny_kernel<T, 4, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, g, u, M, N, K, act);
+  }
+  return launched("dm_gated_ffn");
+}
+
+// ---- workspace
+struct Carver {
+  char* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+// A matrix as the products read it: rows of `ld` 16-bit elements; fp32 matrices as three planes.
+struct Operand { const void* p; int64_t ld, plane; };
+
+struct FfnSizes { int64_t M; int D, F, N, dtype; };
+
+template <typename T>
+int pack_launch(const void* src, int64_t ld, void* dst, int64_t plane, int64_t rows, int cols, hipStream_t st) {
+  const int pitch = (int)round_up(cols, 8);
+  const int64_t blocks = (rows * (pitch / 8) + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
+  if constexpr (std::is_same<T, float>::value)
+    pack_rows_kernel<float, bf16, true><<<grid, dim3(256), 0, st>>>((const float*)src, ld, (bf16*)dst, plane, rows, cols, pitch);
+  else
+    pack_rows_kernel<T, T, false><<<grid, dim3(256), 0, st>>>((const T*)src, ld, (T*)dst, plane, rows, cols, pitch);
+  return launched("gated feed-forward block");
+}
+
+// Takes room for the packed form of a [rows][cols] matrix where the products cannot read it as it lies, and (launch) fills it.
+template <typename T>
+int prepare_operand(Operand& o, const void* src, int64_t ld, int64_t rows, int cols, Carver& ws, bool launch, hipStream_t st) {
+  constexpr bool F32 = std::is_same<T, float>::value;
+  if (!F32 && cols % 8 == 0) {
+    o = {src, ld, 0};
+    return 0;
+  }
+  const int64_t pitch = round_up(cols, 8);
+  o.ld = pitch;
+  o.plane = rows * pitch;
+  void* p = ws.take((size_t)(F32 ? 3 : 1) * rows * pitch * 2);
+  o.p = p;
+  return launch ? pack_launch<T>(src, ld, p, o.plane, rows, cols, st) : 0;
+}
+template <typename T>
+Operand take_operand(int64_t rows, int cols, Carver& ws) {
+  const int64_t pitch = round_up(cols, 8);
+  Operand o = {nullptr, pitch, rows * pitch};
+  o.p = ws.take((size_t)(std::is_same<T, float>::value ? 3 : 1) * rows * pitch * 2);
+  return o;
+}
+
+// The product terms of two operands: one, or the six of split fp32.
+template <typename T>
+void add_segments(GemmArgs& g, const Operand& a, const Operand& b, const Operand* b2 = nullptr) {
+  auto add = [&](int i, int j) {
+    g.a[g.segments] = (const bf16*)a.p + i * a.plane;
+    g.b[g.segments] = (const bf16*)b.p + j * b.plane;
+    g.b2[g.segments] = b2 ? (const bf16*)b2->p + j * b2->plane : nullptr;
+    ++g.segments;
+  };
+  if (std::is_same<T, float>::value) { add(0, 2); add(2, 0); add(1, 1); add(0, 1); add(1, 0); }  // small terms first
+  add(0, 0);
+  g.lda = a.ld;
+  g.ldb = b.ld;
+}
+
+template <typename T> using Mat = typename std::conditional<std::is_same<T, float>::value, bf16, T>::type;  // what the matrix pipe sees
+
+template <typename T>
+Out result(void* p, int64_t ld, int N) {  // a tensor of the caller's
+  constexpr bool F32 = std::is_same<T, float>::value;
+  return {p, ld, 0, F32 ? OUT_F32 : OUT_16, ld % 4 == 0 && aligned(p, 4 * sizeof(T))};
+}
+template <typename T>
+Out between(const Operand& o) {  // an operand of a later product
+  return {const_cast<void*>(o.p), o.ld, o.plane, std::is_same<T, float>::value ? OUT_PLANES : OUT_16, 1};
+}
+
+// out[M][N] = A B (+ bias), the k range split where that pays.
+template <typename T, bool AKS, bool BKS>
+int product(GemmArgs g, const Out& out, const void* bias, void* part, hipStream_t st) {
+  const GemmPlan plan = gemm_plan(g.M, g.N, g.iters * g.segments, part != nullptr);
+  g.splits = plan.splits;
+  g.bias_f32 = std::is_same<T, float>::value;
+  if (plan.splits == 1) {
+    g.out = out;
+    g.bias = bias;
+    return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.big, st);
+  }
+  const int ldp = (int)round_up(g.N, 4);
+  g.split_stride = g.M * ldp;
+  g.out = {part, ldp, 0, OUT_F32, 1};
+  if (const int rc = gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.big, st)) return rc;
+  const int64_t blocks = (g.M * (ldp / 4) + 255) / 256;
+  gemm_join_kernel<Mat<T>><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>((const float*)part, plan.splits, g.split_stride,
+                                                                                                    bias, g.bias_f32, out, g.M, g.N, ldp);
+  return launched("gated feed-forward block");
+}
+
+inline int iters_of(int64_t K) { return (int)((K + 63) / 64); }
+inline int64_t pad8(int64_t v) { return round_up(v, 8); }
+
+struct FfnIn { const void *x, *wg, *wu, *wd, *bg, *bu, *bd; int64_t xs; };
+
+// run: launch; otherwise only count the workspace.
+template <typename T>
+int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int act, Carver& ws, bool run, hipStream_t st) {
+  const int64_t Fp = pad8(z.F);
+  T* gs = (T*)saved;
+  T* us = saved ? gs + z.M * Fp : nullptr;
+  if (z.M <= SKINNY_ROWS) {
+    T* h = (T*)ws.take((size_t)z.M * Fp * sizeof(T));
+    if (!run) return 0;
+    constexpr int V = Skinny<T>::V;
+    const int M = (int)z.M;
+    const bool vg = z.D % V == 0;  // (rows are 16-byte aligned then: ffn_check)
+    auto gate = vg ? skinny_launch<T, true, true> : skinny_launch<T, true, false>;
+    if (const int rc = gate((const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp, gs, us, M, z.F, z.D,
+                            act, st))
+      return rc;
+    auto down = z.F % V == 0 ? skinny_launch<T, false, true> : skinny_launch<T, false, false>;
+    return down(h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, M, z.N, z.F, act, st);
+  }
+  Operand x, wg, wu, wd, h;
+  int rc = prepare_operand<T>(x, in.x, in.xs, z.M, z.D, ws, run, st);
+  if (!rc) rc = prepare_operand<T>(wg, in.wg, z.D, z.F, z.D, ws, run, st);
+  if (!rc) rc = prepare_operand<T>(wu, in.wu, z.D, z.F, z.D, ws, run, st);
+  if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
+  if (rc) return rc;
+  h = take_operand<T>(z.M, z.F, ws);
+  const int segs = std::is_same<T, float>::value ? 6 : 1;
+  const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F) * segs, true).part_bytes;
+  void* part = ws.take(part_bytes);
+  if (!run) return 0;
+
+  GemmArgs g = {};
+  add_segments<T>(g, x, wg, &wu);
+  g.M = z.M; g.N = z.F; g.K = z.D; g.iters = iters_of(g.K); g.splits = 1;
+  g.out = between<T>(h);
+  g.out2 = result<T>(gs, Fp, z.F);
+  g.out3 = result<T>(us, Fp, z.F);
+  g.bias = in.bg; g.bias2 = in.bu; g.bias_f32 = std::is_same<T, float>::value; g.act = act;
+  const bool big = gemm_plan(z.M, 2 * z.F, g.iters * g.segments, false).big;
+  if ((rc = gemm_launch<Mat<T>, false, false, EPI_GATE>(g, big, st))) return rc;
+
+  GemmArgs d = {};
+  add_segments<T>(d, h, wd);
+  d.M = z.M; d.N = z.N; d.K = z.F; d.iters = iters_of(z.F);
+  return product<T, false, false>(d, result<T>(y, z.N, z.N), in.bd, part, st);
+}
+
+struct FfnGrads { void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd; };
+
+template <typename T>
+int column_sums(const Operand& a, const Operand* b, int64_t M, int C, void* out0, void* out1, float* part, hipStream_t st) {
+  constexpr int PL = std::is_same<T, float>::value ? 3 : 1;
+  const int rows = column_sums_rows(M, C);
+  column_sums_kernel<Mat<T>, PL><<<dim3((C + 255) / 256, rows), dim3(64), 0, st>>>((const Mat<T>*)a.p, b ? (const Mat<T>*)b->p : nullptr, a.plane, a.ld, M,
+                                                                                    C, part);
+  if (const int rc = launched("dm_gated_ffn_backward")) return rc;
+  partial_rows_kernel<T><<<dim3((unsigned)((2 * (int64_t)C + 15) / 16)), dim3(256), 0, st>>>(part, rows, C, (T*)out0, (T*)out1);
+  return launched("dm_gated_ffn_backward");
+}
+
+template <typename T>
+int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys, const void* saved, const FfnGrads& gr, int act, Carver& ws, bool run,
+                 hipStream_t st) {
+  const int64_t Fp = pad8(z.F);
+  const int segs = std::is_same<T, float>::value ? 6 : 1;
+  Operand x, wg, wu, wd, y;
+  int rc = prepare_operand<T>(y, dy, dys, z.M, z.N, ws, run, st);
+  if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
+  if (!rc) rc = prepare_operand<T>(x, in.x, in.xs, z.M, z.D, ws, run && (gr.dwg || gr.dwu), st);
+  if (!rc) rc = prepare_operand<T>(wg, in.wg, z.D, z.F, z.D, ws, run && gr.dx, st);
+  if (!rc) rc = prepare_operand<T>(wu, in.wu, z.D, z.F, z.D, ws, run && gr.dx, st);
+  if (rc) return rc;
+  const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws), h = take_operand<T>(z.M, z.F, ws);
+  const int rows_it = iters_of(z.M) * segs;
+  size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F) * segs * 2, true).part_bytes;
+  const size_t more[] = {gemm_plan(z.F, z.D, rows_it, true).part_bytes, gemm_plan(z.N, z.F, rows_it, true).part_bytes,
+                         (size_t)column_sums_rows(z.M, z.F) * 2 * z.F * 4, (size_t)column_sums_rows(z.M, z.N) * 2 * z.N * 4};
+  for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
+  void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
+  if (!run) return 0;
+
+  GemmArgs a = {};  // dh, and from it dg, du and h
+  add_segments<T>(a, y, wd);
+  a.M = z.M; a.N = z.F; a.K = z.N; a.iters = iters_of(a.K); a.splits = 1;
+  a.out = between<T>(dg); a.out2 = between<T>(du); a.out3 = between<T>(h);
+  a.g = saved; a.u = (const T*)saved + z.M * Fp; a.ldg = Fp; a.gu_f32 = std::is_same<T, float>::value; a.act = act;
+  if ((rc = gemm_launch<Mat<T>, false, true, EPI_DACT>(a, gemm_plan(z.M, z.F, a.iters * a.segments, false).big, st))) return rc;
+
+  if (gr.dx) {
+    GemmArgs g = {};
+    add_segments<T>(g, dg, wg);
+    add_segments<T>(g, du, wu);
+    g.M = z.M; g.N = z.D; g.K = z.F; g.iters = iters_of(z.F);
+    if ((rc = product<T, false, true>(g, result<T>(gr.dx, z.D, z.D), nullptr, part, st))) return rc;
+  }
+  auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out) {
+    GemmArgs g = {};
+    add_segments<T>(g, l, r);
+    g.M = rows; g.N = cols; g.K = (int)z.M; g.iters = iters_of(z.M);
+    return product<T, true, true>(g, result<T>(out, cols, cols), nullptr, part, st);
+  };
+  if (gr.dwg && (rc = weight(dg, x, z.F, z.D, gr.dwg))) return rc;
+  if (gr.dwu && (rc = weight(du, x, z.F, z.D, gr.dwu))) return rc;
+  if (gr.dwd && (rc = weight(y, h, z.N, z.F, gr.dwd))) return rc;
+  if ((gr.dbg || gr.dbu) && (rc = column_sums<T>(dg, &du, z.M, z.F, gr.dbg, gr.dbu, (float*)part, st))) return rc;
+  if (gr.dbd && (rc = column_sums<T>(y, nullptr, z.M, z.N, gr.dbd, nullptr, (float*)part, st))) return rc;
+  return 0;
+}
+
+inline int ffn_check(const char* who, const FfnSizes& z, int act) {
+  if (!dtype_ok(z.dtype)) return fail("%s: unknown dtype %d", who, z.dtype);
+  if (act < DM_ACT_SILU || act > DM_ACT_SIGMOID) return fail("%s: unknown activation %d", who, act);
+  const int most = 1 << 20;
+  if (z.D < 1 || z.F < 1 || z.N < 1 || z.D > most || z.F > most || z.N > most)
+    return fail("%s: widths %d, %d, %d (1 to 2^20)", who, z.D, z.F, z.N);
+  if (z.M < 0 || z.M > (1 << 28)) return fail("%s: %lld rows (up to 2^28)", who, (long long)z.M);
+  return 0;
+}
+// Rows that the kernels read as 16-byte pieces start at multiples of 16 bytes; rows of no whole number of pieces are read element by element.
+inline int ffn_check_matrix(const char* who, const char* what, const void* p, int64_t ld, int64_t rows, int cols, int dtype) {
+  if (!p) return fail("%s: null argument (%s)", who, what);
+  if (ld < cols && rows > 1) return fail("%s: %s: row stride %lld below the width %d", who, what, (long long)ld, cols);
+  if (ld > (1 << 21)) return fail("%s: %s: row stride %lld above 2^21", who, what, (long long)ld);
+  const int es = dtype_size(dtype);
+  if (cols % (16 / es) == 0 && (!aligned(p, 16) || (rows > 1 && ld % (16 / es))))
+    return fail("%s: %s: rows must start at multiples of 16 bytes", who, what);
+  if (!aligned(p, es)) return fail("%s: %s: not aligned to its elements", who, what);
+  return 0;
+}
+
+template <typename F>
+int ffn_types(int dtype, F&& f) {
+  switch (dtype) {
+    case DM_F32: return f(float());
+    case DM_BF16: return f(bf16());
+    default: return f(f16());
+  }
+}
+
+__global__ void fill_zero_bytes_kernel(uint32_t* p, int64_t words, uint16_t* tail) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) p[i] = 0;
+  if (tail && blockIdx.x == 0 && threadIdx.x == 0) *tail = 0;
+}
+
+}  // namespace dmb
+
+extern "C" {
+
+size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype) {
+  using namespace dmb;
+  if (M <= 0 || F < 1 || !dtype_ok(dtype)) return 0;
+  return (size_t)2 * M * pad8(F) * dtype_size(dtype);
+}
+
+size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype) {
+  using namespace dmb;
+  const FfnSizes z = {M, D, F, N, dtype};
+  if (M <= 0 || ffn_check("dm_gated_ffn_workspace_bytes", z, DM_ACT_SILU)) return 0;
+  Carver ws = {nullptr};
+  ffn_types(dtype, [&](auto t) { return ffn_forward<decltype(t)>(z, FfnIn{}, nullptr, nullptr, 0, ws, false, nullptr); });
+  return ws.used;
+}
+
+size_t dm_gated_ffn_backward_workspace_bytes(int64_t M, int D, int F, int N, int dtype) {
+  using namespace dmb;
+  const FfnSizes z = {M, D, F, N, dtype};
+  if (M <= 0 || ffn_check("dm_gated_ffn_backward_workspace_bytes", z, DM_ACT_SILU)) return 0;
+  Carver ws = {nullptr};
+  ffn_types(dtype, [&](auto t) {
+    return ffn_backward<decltype(t)>(z, FfnIn{}, nullptr, 0, nullptr, FfnGrads{}, 0, ws, false, nullptr);
+  });
+  return ws.used;
+}
+
+int dm_gated_ffn(const void* x_dev, int64_t x_stride, const void* w_gate_dev, const void* w_up_dev, const void* w_down_dev, const void* b_gate_dev,
+                 const void* b_up_dev, const void* b_down_dev, void* y_dev, void* saved_dev, int64_t M, int D, int F, int N, int activation, int dtype,
+                 void* workspace_dev, size_t workspace_bytes, void* stream) {
+  using namespace dmb;
+  const char* who = "dm_gated_ffn";
+  const FfnSizes z = {M, D, F, N, dtype};
+  if (const int rc = ffn_check(who, z, activation)) return rc;
+  if (M == 0) return 0;
+  if (ffn_check_matrix(who, "x", x_dev, x_stride, M, D, dtype) || ffn_check_matrix(who, "w_gate", w_gate_dev, D, F, D, dtype) ||
+      ffn_check_matrix(who, "w_up", w_up_dev, D, F, D, dtype) || ffn_check_matrix(who, "w_down", w_down_dev, F, N, F, dtype))
+    return 1;
+  if (!y_dev) return fail("%s: null argument (y)", who);
+  if (saved_dev && !aligned(saved_dev, 16)) return fail("%s: saved must be aligned to 16 bytes", who);
+  const size_t need = dm_gated_ffn_workspace_bytes(M, D, F, N, dtype);
+  if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16))
+    return fail("%s: workspace of %zu bytes, %zu needed (aligned to 16)", who, workspace_dev ? workspace_bytes : (size_t)0, need);
+  const FfnIn in = {x_dev, w_gate_dev, w_up_dev, w_down_dev, b_gate_dev, b_up_dev, b_down_dev, x_stride};
+  Carver ws = {(char*)workspace_dev};
+  return ffn_types(dtype, [&](auto t) { return ffn_forward<decltype(t)>(z, in, y_dev, saved_dev, activation, ws, true, (hipStream_t)stream); });
+}
+
+int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_dev, int64_t x_stride, const void* w_gate_dev, const void* w_up_dev,
+                          const void* w_down_dev, const void* saved_dev, void* dx_dev, void* dw_gate_dev, void* dw_up_dev, void* dw_down_dev,
+                          void* db_gate_dev, void* db_up_dev, void* db_down_dev, int64_t M, int D, int F, int N, int activation, int dtype,
+                          void* workspace_dev, size_t workspace_bytes, void* stream) {
+  using namespace dmb;
+  const char* who = "dm_gated_ffn_backward";
+  const FfnSizes z = {M, D, F, N, dtype};
+  if (const int rc = ffn_check(who, z, activation)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (M == 0) {  // no rows: the parameters' gradients are zero
+    void* const p[] = {dw_gate_dev, dw_up_dev, dw_down_dev, db_gate_dev, db_up_dev, db_down_dev};
+    const int64_t n[] = {(int64_t)F * D, (int64_t)F * D, (int64_t)N * F, F, F, N};
+    for (int i = 0; i < 6; ++i) {
+      if (!p[i]) continue;
+      const int64_t bytes = n[i] * dtype_size(dtype), words = bytes / 4;
+      fill_zero_bytes_kernel<<<dim3((unsigned)(words / 256 + 1 < 65536 ? words / 256 + 1 : 65536)), dim3(256), 0, st>>>(
+          (uint32_t*)p[i], words, bytes % 4 ? (uint16_t*)((char*)p[i] + words * 4) : nullptr);
+      if (const int rc = launched(who)) return rc;
+    }
+    return 0;
+  }
+  if (ffn_check_matrix(who, "dy", dy_dev, dy_stride, M, N, dtype) || ffn_check_matrix(who, "x", x_dev, x_stride, M, D, dtype) ||
+      ffn_check_matrix(who, "w_gate", w_gate_dev, D, F, D, dtype) || ffn_check_matrix(who, "w_up", w_up_dev, D, F, D, dtype) ||
+      ffn_check_matrix(who, "w_down", w_down_dev, F, N, F, dtype))
+    return 1;
+  if (!saved_dev || !aligned(saved_dev, 16)) return fail("%s: saved must be what dm_gated_ffn wrote, aligned to 16 bytes", who);
+  const size_t need = dm_gated_ffn_backward_workspace_bytes(M, D, F, N, dtype);
+  if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16))
+    return fail("%s: workspace of %zu bytes, %zu needed (aligned to 16)", who, workspace_dev ? workspace_bytes : (size_t)0, need);
+  const FfnIn in = {x_dev, w_gate_dev, w_up_dev, w_down_dev, nullptr, nullptr, nullptr, x_stride};
+  const FfnGrads gr = {dx_dev, dw_gate_dev, dw_up_dev, dw_down_dev, db_gate_dev, db_up_dev, db_down_dev};
+  Carver ws = {(char*)workspace_dev};
+  return ffn_types(dtype,
+                   [&](auto t) { return ffn_backward<decltype(t)>(z, in, dy_dev, dy_stride, saved_dev, gr, activation, ws, true, st); });
+}
+
+}  // extern "C"

@@ -1,0 +1,293 @@
+"""Operators of a transformer block over tokens (no counterpart in the reference's models): layer norm, rotary positions and
+the gated feed-forward block, each with its backward pass, on the HIP kernels of libdm_sampler.so (include/dm_sampler.h).
+
+They work on fp32, bfloat16 and half tensors of one GPU and run on that GPU's current stream; every sum is fp32.  Like
+the rest of the package they carry no autograd: a training step calls the backward functions itself.  Inputs may be views:
+what the kernels cannot read as it lies (a last dimension with a stride, rows off 16-byte boundaries) is copied first.
+Outputs and workspaces come from torch's allocator, so the calls may be captured into a graph.  There is no CPU path."""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
+
+
+def _dtype(t, name):
+    if not torch.is_tensor(t):
+        raise RuntimeError(f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} must be on the GPU (it is on {t.device}). There is no CPU path.")
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be fp32, bfloat16 or half (got {t.dtype})")
+    return _DTYPES[t.dtype]
+
+
+def _like(t, x, name, dtypes=None):
+    _dtype(t, name)
+    if t.device != x.device:
+        raise RuntimeError(f"{name} must be on {x.device} (got {t.device})")
+    if t.dtype not in (dtypes or (x.dtype,)):
+        raise RuntimeError(f"{name} must be of type {' or '.join(str(d) for d in dtypes or (x.dtype,))} (got {t.dtype})")
+    return t
+
+
+def _vector(t, n, x, name, dtypes=None):
+    if t is None:
+        return None
+    _like(t, x, name, dtypes)
+    if t.shape != (n,):
+        raise RuntimeError(f"{name} must be [{n}] (got {tuple(t.shape)})")
+    return t.contiguous()
+
+
+def _rows(t):
+    """[..., C] as rows the kernels can read: (tensor [M, C], row stride in elements)."""
+    c = t.shape[-1]
+    r = t.reshape(-1, c)
+    whole = 16 // t.element_size()
+    if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and (r.stride(0) < c or r.stride(0) > 1 << 21)):
+        r = r.contiguous()
+    if c % whole == 0 and (r.data_ptr() % 16 or (r.shape[0] > 1 and r.stride(0) % whole)):
+        r = r.clone(memory_format=torch.contiguous_format)
+    return r, (r.stride(0) if r.shape[0] > 1 else c)
+
+
+def _matrix(t, rows, cols, x, name):
+    _like(t, x, name)
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or t.shape[1] != cols:
+        raise RuntimeError(f"{name} must be [{rows if rows is not None else 'any'}, {cols}] (got {tuple(t.shape)})")
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _workspace(t, nbytes):
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=t.device)
+
+
+# ------------------------------------------------------------------ layer norm
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension.  ``weight`` and ``bias`` ([C], either may be
+    missing) are of x's type or fp32.  ``return_stats``: (y, mean, rstd), fp32, for the backward pass."""
+    dt = _dtype(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"layer_norm needs a last dimension to normalise (got {tuple(x.shape)})")
+    c = x.shape[-1]
+    w = _vector(weight, c, x, "weight", (x.dtype, torch.float32))
+    b = _vector(bias, c, x, "bias", (x.dtype, torch.float32) if w is None else (w.dtype,))
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    p = w if w is not None else b
+    with torch.cuda.device(x.device):
+        r, stride = _rows(x)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = rstd = None
+        if return_stats:
+            mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+        _lib.check(_lib.lib().dm_layer_norm(
+            _lib.ptr(r), stride, _lib.ptr(w), _lib.ptr(b), dt if p is None else _DTYPES[p.dtype], _lib.ptr(y), _lib.ptr(mean),
+            _lib.ptr(rstd), r.shape[0], c, eps, dt, _stream(x)))
+    return (y, mean, rstd) if return_stats else y
+
+
+def layer_norm_backward(grad, x, weight, mean, rstd):
+    """(dx, dweight, dbias) from the output's gradient and what ``layer_norm(..., return_stats=True)`` returned.  The parameters'
+    gradients are None where ``weight`` is None, otherwise of its type, summed over all rows in a fixed order."""
+    dt = _dtype(x, "x")
+    _like(grad, x, "grad")
+    if x.dim() < 1 or x.shape[-1] < 1 or grad.shape != x.shape:
+        raise RuntimeError(f"grad must have x's shape {tuple(x.shape)} (got {tuple(grad.shape)})")
+    c = x.shape[-1]
+    w = _vector(weight, c, x, "weight", (x.dtype, torch.float32))
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _like(t, x, name, (torch.float32,))
+        if t.shape != x.shape[:-1]:
+            raise RuntimeError(f"{name} must be {tuple(x.shape[:-1])} (got {tuple(t.shape)})")
+    with torch.cuda.device(x.device):
+        L = _lib.lib()
+        r, stride = _rows(x)
+        g, gstride = _rows(grad)
+        mean, rstd = mean.contiguous(), rstd.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = db = ws = None
+        if w is not None:
+            dw, db = torch.empty_like(w), torch.empty_like(w)
+            ws = _workspace(x, L.dm_layer_norm_backward_workspace_bytes(r.shape[0], c))
+        _lib.check(L.dm_layer_norm_backward(
+            _lib.ptr(g), gstride, _lib.ptr(r), stride, _lib.ptr(w), dt if w is None else _DTYPES[w.dtype], _lib.ptr(mean), _lib.ptr(rstd),
+            _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), r.shape[0], c, dt, _lib.ptr(ws), 0 if ws is None else ws.numel(), _stream(x)))
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------ rotary positions
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_length=None, axes=1, device=None):
+    """(inv_freq, scale) for ``apply_rotary``: inv_freq[i] = base^(-2i / d), float64, with d = rotary_dim / axes (each axis has
+    the whole range).  To stretch positions trained up to ``original_length`` by ``factor``: "linear" divides all frequencies;
+    "ntk" raises the base so that the slowest pair is divided by ``factor``; "yarn" divides the pairs that turn less than once over
+    the trained length, keeps those that turn more than 32 times, blends between, and scales by 0.1 ln(factor) + 1."""
+    if axes < 1 or rotary_dim < 0 or rotary_dim % (2 * axes):
+        raise ValueError(f"rotary_dim {rotary_dim} must be a multiple of {2 * axes} (pairs on {axes} axes)")
+    if base <= 0 or factor <= 0:
+        raise ValueError("base and factor must be positive")
+    pairs = rotary_dim // 2 // axes
+    i = torch.arange(pairs, dtype=torch.float64)
+    span, scale = max(pairs, 1), 1.0
+    if scaling == "ntk" and pairs > 1:
+        base = base * factor ** (pairs / (pairs - 1))
+    inv = float(base) ** (-i / span)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        if not original_length or original_length <= 0:
+            raise ValueError("yarn scaling needs the trained length (original_length)")
+        if base <= 1:
+            raise ValueError("yarn scaling needs a base above 1")
+
+        def pair_that_turns(n):
+            return span * math.log(original_length / (n * 2 * math.pi)) / math.log(base)
+        low = max(math.floor(pair_that_turns(32)), 0)
+        high = min(math.ceil(pair_that_turns(1)), span - 1)
+        ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+        inv = inv / factor * ramp + inv * (1 - ramp)
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"Unknown rotary scaling: {scaling}")
+    return inv.repeat(axes).to(device if device is not None else "cpu"), scale
+
+
+def _rotary_tensor(t, out):
+    r = _lib.RotaryTensor()
+    r.in_, r.out, r.heads = t.data_ptr(), out.data_ptr(), t.shape[2]
+    for i in range(3):
+        r.in_stride[i], r.out_stride[i] = t.stride(i), out.stride(i)
+    return r
+
+
+def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inverse=False, inplace=False):
+    """Turns the pairs of every head of ``q`` [B, T, heads, head_dim] and ``k`` (the same with its own heads, or None) by
+    position * inv_freq; returns (q, k).  ``inv_freq`` (float64 [rotary_dim / 2], on the GPU) says how much of the head turns;
+    the rest is copied.  ``positions``: integers [T], [B, T], or [axes, B, T] (pair i takes axis i // (pairs / axes)), None for
+    0..T-1; angles are formed in 64 bits.  ``layout``: "half" pairs element i with i + rotary_dim/2, "interleaved" 2i with 2i + 1.
+    ``inverse`` turns back: applied to gradients it is the backward pass.  ``inplace`` writes into q and k themselves."""
+    dt = _dtype(q, "q")
+    if q.dim() != 4 or q.shape[3] < 1:
+        raise RuntimeError(f"q must be [B, T, heads, head_dim] (got {tuple(q.shape)})")
+    b, t, _, d = q.shape
+    if k is not None:
+        _like(k, q, "k")
+        if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != d:
+            raise RuntimeError(f"k must be [{b}, {t}, heads, {d}] (got {tuple(k.shape)})")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"Unknown rotary layout: {layout}")
+    if not torch.is_tensor(inv_freq) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device:
+        raise RuntimeError(f"inv_freq must be a float64 vector on {q.device} (rotary_frequencies makes one)")
+    rotary_dim = 2 * inv_freq.numel()
+    if rotary_dim > d:
+        raise RuntimeError(f"{inv_freq.numel()} pairs do not fit a head of {d} elements")
+    axes, strides = 1, None
+    if positions is not None:
+        if positions.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8) or positions.device != q.device:
+            raise RuntimeError(f"positions must be integers on {q.device}")
+        axes = positions.shape[0] if positions.dim() == 3 else 1
+        if positions.dim() not in (1, 2, 3) or axes < 1:
+            raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] (got {tuple(positions.shape)})")
+        if any(have not in (1, want) for have, want in zip(positions.shape[::-1], (t, b))):
+            raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] with B = {b}, T = {t} (got {tuple(positions.shape)})")
+        positions = positions.to(torch.int64).expand(axes, b, t)
+        strides = (C.c_int64 * 3)(*positions.stride())
+    if inv_freq.numel() % axes:
+        raise RuntimeError(f"{inv_freq.numel()} pairs do not divide into {axes} axes")
+    with torch.cuda.device(q.device):
+        ins, outs = [], []
+        for x in (q, k):
+            if x is None:
+                outs.append(None)
+                continue
+            if inplace:
+                if (d > 1 and x.stride(3) != 1) or any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+                    raise RuntimeError("in place needs contiguous head elements and no expanded dimension")
+                out = x
+            else:
+                x = x if d == 1 or x.stride(3) == 1 else x.contiguous()
+                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            ins.append(x)
+            outs.append(out)
+        args = [_rotary_tensor(x, o) for x, o in zip(ins, [o for o in outs if o is not None])]
+        inv_freq = inv_freq.contiguous()
+        _lib.check(_lib.lib().dm_rotary(
+            C.byref(args[0]), C.byref(args[1]) if len(args) > 1 else None, _lib.ptr(positions), strides, axes, _lib.ptr(inv_freq), b, t, d,
+            rotary_dim, int(layout == "interleaved"), scale, int(inverse), dt, _stream(q)))
+    return tuple(outs)
+
+
+# ------------------------------------------------------------------ gated feed-forward block
+
+def _ffn_check(x, w_gate, w_up, w_down, activation):
+    dt = _dtype(x, "x")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"Unknown activation: {activation}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"x must be [..., width] (got {tuple(x.shape)})")
+    d = x.shape[-1]
+    with torch.cuda.device(x.device):
+        w_gate = _matrix(w_gate, None, d, x, "w_gate")
+        f = w_gate.shape[0]
+        w_up = _matrix(w_up, f, d, x, "w_up")
+        w_down = _matrix(w_down, None, f, x, "w_down")
+    if f < 1 or w_down.shape[0] < 1:
+        raise RuntimeError("the weights must not be empty")
+    return dt, d, f, w_down.shape[0], w_gate, w_up, w_down
+
+
+def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation="silu", save=False):
+    """(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down, with weights as nn.Linear holds them: w_gate and w_up
+    [hidden, width], w_down [out, hidden].  All tensors are of one type.  ``activation``: silu, gelu (erf), gelu_tanh, relu, sigmoid.
+    ``save``: (y, saved), with ``saved`` (opaque) for ``gated_ffn_backward``.  16-bit types round the projections and their product to
+    that type between the matrix products; fp32 keeps fp32 accuracy."""
+    dt, d, f, n, w_gate, w_up, w_down = _ffn_check(x, w_gate, w_up, w_down, activation)
+    b_gate, b_up, b_down = _vector(b_gate, f, x, "b_gate"), _vector(b_up, f, x, "b_up"), _vector(b_down, n, x, "b_down")
+    with torch.cuda.device(x.device):
+        L = _lib.lib()
+        r, stride = _rows(x)
+        m = r.shape[0]
+        y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+        saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt), dtype=torch.uint8, device=x.device) if save else None
+        ws = _workspace(x, L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt))
+        _lib.check(L.dm_gated_ffn(
+            _lib.ptr(r), stride, _lib.ptr(w_gate), _lib.ptr(w_up), _lib.ptr(w_down), _lib.ptr(b_gate), _lib.ptr(b_up), _lib.ptr(b_down),
+            _lib.ptr(y), _lib.ptr(saved), m, d, f, n, _ACTIVATIONS[activation], dt, _lib.ptr(ws), ws.numel(), _stream(x)))
+    return (y, saved) if save else y
+
+
+def gated_ffn_backward(grad, x, w_gate, w_up, w_down, saved, activation="silu", bias=False):
+    """(dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) from the output's gradient and the ``saved`` of the forward call; the
+    biases' gradients are None unless ``bias``.  Sums run in a fixed order: the same inputs give the same bits."""
+    dt, d, f, n, w_gate, w_up, w_down = _ffn_check(x, w_gate, w_up, w_down, activation)
+    _like(grad, x, "grad")
+    if grad.shape != x.shape[:-1] + (n,):
+        raise RuntimeError(f"grad must be {tuple(x.shape[:-1]) + (n,)} (got {tuple(grad.shape)})")
+    with torch.cuda.device(x.device):
+        L = _lib.lib()
+        r, stride = _rows(x)
+        g, gstride = _rows(grad)
+        m = r.shape[0]
+        if not torch.is_tensor(saved) or saved.device != x.device or saved.dtype != torch.uint8 or not saved.is_contiguous() or \
+                saved.numel() != L.dm_gated_ffn_saved_bytes(m, f, dt):
+            raise RuntimeError("saved must be what gated_ffn(..., save=True) returned for this input")
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dws = [torch.empty_like(w) for w in (w_gate, w_up, w_down)]
+        dbs = [torch.empty(size, dtype=x.dtype, device=x.device) if bias else None for size in (f, f, n)]
+        ws = _workspace(x, L.dm_gated_ffn_backward_workspace_bytes(m, d, f, n, dt))
+        _lib.check(L.dm_gated_ffn_backward(
+            _lib.ptr(g), gstride, _lib.ptr(r), stride, _lib.ptr(w_gate), _lib.ptr(w_up), _lib.ptr(w_down), _lib.ptr(saved), _lib.ptr(dx),
+            *(_lib.ptr(t) for t in dws + dbs), m, d, f, n, _ACTIVATIONS[activation], dt, _lib.ptr(ws), ws.numel(), _stream(x)))
+    return (dx, *dws, *dbs)

@@ -41,8 +41,9 @@ const char* dm_last_error(void);
  * DM_K_COUNT grew, dm_sample accepts host pointers and sizes its workspace with dm_sample_workspace_bytes;
  * 3: dm_sample_chunked, the fused low-resolution kernel class, the any-geometry kernel classes;
  * 4: dm_sample's workspace holds one carve per parallel sub-batch chain (dm_sample_workspace_bytes grew for large batches),
- *    dm_sample_branches, dm_stream_create / dm_stream_destroy). */
-#define DM_ABI_VERSION 4
+ *    dm_sample_branches, dm_stream_create / dm_stream_destroy;
+ * 5: the transformer-block operators dm_layer_norm*, dm_rotary, dm_gated_ffn*; nothing of version 4 changed). */
+#define DM_ABI_VERSION 5
 int dm_version(void);
 /* sha256 over the compiler flags and sources this library was built from (__graft_entry__.build_key); "unkeyed" for a
  * hand build.  build() compares it with the tree it runs in, so a library built with other flags is not reused. */
@@ -300,6 +301,62 @@ int dm_conv2d(int kind, const float* x1_dev, int c1, const float* x2_dev, int c2
               const float* stats_in_dev, int pin, float cnt_in, const float* gamma_dev,
               const float* beta_dev, const float* temb_dev, int temb_stride, float* y_dev,
               float* stats_out_dev, int B, int H, int W, void* stream);
+
+/* ---- transformer-block operators (no counterpart in the reference's models): what stands around dm_attention in a
+ * transformer over image tokens - layer norm, rotary positions, gated feed-forward block - with their backward passes.
+ * Element types: DM_F32, DM_BF16, DM_F16; every sum, statistic and activation is fp32.  Nothing allocates or
+ * synchronises: workspaces are the caller's (their contents do not matter, calls in one stream may share one, calls that
+ * may overlap may not).  A call launches on the current device, in `stream`; it may be captured into a graph.  Outputs are
+ * contiguous and overlap no input unless said otherwise.  The same call gives the same bits every time. */
+enum { DM_F32 = 0, DM_BF16 = 1, DM_F16 = 2 };
+enum { DM_ACT_SILU = 0, DM_ACT_GELU = 1 /* erf */, DM_ACT_GELU_TANH = 2, DM_ACT_RELU = 3, DM_ACT_SIGMOID = 4 };
+
+/* y[m,:] = (x[m,:] - mean) rstd weight + bias over rows of C elements, rstd = 1/sqrt(var + eps), var the biased variance.
+ * x rows are x_stride elements apart.  weight, bias: [C] of x's type or fp32 (param_dtype), either may be NULL.
+ * mean_dev, rstd_dev: [M] fp32 for the backward pass, or NULL.  M == 0 does nothing. */
+int dm_layer_norm(const void* x_dev, int64_t x_stride, const void* weight_dev, const void* bias_dev, int param_dtype,
+                  void* y_dev, float* mean_dev, float* rstd_dev, int64_t M, int C, float eps, int dtype, void* stream);
+/* dx, and the parameters' gradients summed over the rows (either may be NULL; both of param_dtype).  The workspace is needed
+ * only for the parameters' gradients.  M == 0 clears them. */
+size_t dm_layer_norm_backward_workspace_bytes(int64_t M, int C);
+int dm_layer_norm_backward(const void* dy_dev, int64_t dy_stride, const void* x_dev, int64_t x_stride, const void* weight_dev,
+                           int param_dtype, const float* mean_dev, const float* rstd_dev, void* dx_dev, void* dweight_dev,
+                           void* dbias_dev, int64_t M, int C, int dtype, void* workspace_dev, size_t workspace_bytes,
+                           void* stream);
+
+/* Rotary positions on [B][T][heads][head_dim] tensors (query, and key or NULL) with any strides, head elements contiguous.
+ * Pair i of rotary_dim / 2 turns by position * inv_freq[i] (64-bit angles; exact for positions below 2^53), its two values
+ * scaled by `scale`: elements (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`.  Elements from rotary_dim on are
+ * copied.  positions int64 with strides (axis, image, token) in elements, or NULL for 0 .. T-1; with `axes` > 1 pair i takes
+ * the axis i / (pairs / axes).  `inverse` turns back: the gradient of the forward call.  out == in (same strides) works in
+ * place; otherwise the two may not overlap. */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t in_stride[3], out_stride[3]; /* image, token, head, in elements */
+  int heads;
+} dm_rotary_tensor;
+int dm_rotary(const dm_rotary_tensor* q, const dm_rotary_tensor* k, const int64_t* positions_dev,
+              const int64_t* position_strides, int axes, const double* inv_freq_dev, int64_t B, int64_t T, int head_dim,
+              int rotary_dim, int interleaved, float scale, int inverse, int dtype, void* stream);
+
+/* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down: x [M][D] rows x_stride apart, w_gate and w_up [F][D],
+ * w_down [N][F], y [M][N], biases [F], [F], [N] or NULL, all of one type.  saved_dev: NULL, or dm_gated_ffn_saved_bytes for the
+ * backward pass.  Between its products the block keeps the tensors' type: 16-bit types round g, u and h there.  fp32 operands
+ * are multiplied as three bf16 terms each above 64 rows (an infinite operand gives NaN there, where fp32 would give an infinity).
+ * Rows of whole 16-byte pieces must start at multiples of 16 bytes. */
+size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype);
+size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype);
+int dm_gated_ffn(const void* x_dev, int64_t x_stride, const void* w_gate_dev, const void* w_up_dev, const void* w_down_dev,
+                 const void* b_gate_dev, const void* b_up_dev, const void* b_down_dev, void* y_dev, void* saved_dev, int64_t M,
+                 int D, int F, int N, int activation, int dtype, void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Gradients from dy [M][N] (rows dy_stride apart); any of the seven may be NULL.  M == 0 clears the parameters' gradients. */
+size_t dm_gated_ffn_backward_workspace_bytes(int64_t M, int D, int F, int N, int dtype);
+int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_dev, int64_t x_stride, const void* w_gate_dev,
+                          const void* w_up_dev, const void* w_down_dev, const void* saved_dev, void* dx_dev, void* dw_gate_dev,
+                          void* dw_up_dev, void* dw_down_dev, void* db_gate_dev, void* db_up_dev, void* db_down_dev, int64_t M,
+                          int D, int F, int N, int activation, int dtype, void* workspace_dev, size_t workspace_bytes,
+                          void* stream);
 
 #ifdef __cplusplus
 }
