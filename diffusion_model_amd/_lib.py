@@ -65,7 +65,7 @@ _SIGS = {
     "dm_layer_norm_backward": (_i, [_vp, _l, _vp, _l, _vp, _i, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _vp, _sz, _vp]),
     "dm_rotary": (_i, [C.POINTER(RotaryTensor), C.POINTER(RotaryTensor), _vp, C.POINTER(_l), _i, _vp, _l, _l, _i, _i, _i, _f, _i, _i, _vp]),
     "dm_gated_ffn_saved_bytes": (_sz, [_l, _i, _i]),
-    "dm_gated_ffn_workspace_bytes": (_sz, [_l, _i, _i, _i, _i]),
+    "dm_gated_ffn_workspace_bytes": (_sz, [_l, _i, _i, _i, _i, _i]),
     "dm_gated_ffn": (_i, [_vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "dm_gated_ffn_backward_workspace_bytes": (_sz, [_l, _i, _i, _i, _i]),
     "dm_gated_ffn_backward": (_i, [_vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp,

@@ -1,10 +1,10 @@
 // dm_block_ffn.hip — the gated feed-forward block and its gradients.
 //   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) u, y = h Wd^T + bd
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h, biases: column sums.
-// Both projections, the activation and the product are one kernel; so are dh, dg, du and the h that dWd needs (recomputed from g and u,
-// which the forward pass keeps for training).  Two paths: up to SKINNY_ROWS rows (decode) the weights' bandwidth bounds the block and
+// Both projections, the activation and the product are one kernel; so are dh, dg and du: for training the forward pass keeps u act'(g),
+// act(g) and h, three values where g and u would be two, so that none is rounded twice and nothing is computed again.  Two paths: up to SKINNY_ROWS rows (decode) the weights' bandwidth bounds the block and
 // every wave streams weight rows straight into matrix instructions; above that the tiled products of dm_block_gemm.hip.
-// Rounding: g, u, dg, du and h are kept in the tensors' type between the products (16-bit: the matrix pipe takes nothing wider), every
+// Rounding: h, u act'(g), act(g), dg and du are kept in the tensors' type between the products (16-bit: the matrix pipe takes nothing wider), every
 // sum is fp32.  fp32 tensors are split into three bf16 terms and multiplied as six products (a1b1 a1b2 a2b1 a2b2 a1b3 a3b1; what is left
 // out is below 2^-25 of |a||b|).
 #include <type_traits>
@@ -46,46 +46,6 @@ pack_rows_kernel(const S* __restrict__ src, int64_t ld, D* __restrict__ dst, int
       *reinterpret_cast<Vec<D, 8>*>(dst + r * pitch + c) = o;
     }
   }
-}
-
-// ---- column sums of one or two [M][C] arrays of PL planes: part[block row][2][C], joined by partial_rows_kernel
-template <typename T, int PL>
-__global__ void __launch_bounds__(64)
-column_sums_kernel(const T* __restrict__ p0, const T* __restrict__ p1, int64_t plane, int64_t ld, int64_t M, int C, float* __restrict__ part) {
-  const int c = (blockIdx.x * 64 + threadIdx.x) * 4;
-  if (c >= C) return;
-  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-  const bool vec = ld % 4 == 0 && c + 4 <= C && ((uintptr_t)p0 & (4 * sizeof(T) - 1)) == 0;
-  auto add = [&](const T* p, int64_t m, float (&s)[4]) {
-#pragma unroll
-    for (int k = 0; k < PL; ++k) {
-      const T* r = p + k * plane + m * ld + c;
-      if (vec) {
-        float v[4];
-        load_vec<T, 4>(r, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < C) s[e] += (float)r[e];
-      }
-    }
-  };
-#pragma unroll 4
-  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-    add(p0, m, s0);
-    if (p1) add(p1, m, s1);
-  }
-  float* o = part + (int64_t)blockIdx.y * 2 * C + c;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (c + e < C) { o[e] = s0[e]; o[C + e] = s1[e]; }
-}
-inline int column_sums_rows(int64_t M, int C) {
-  const int64_t want = 4096 / ((C + 255) / 256);
-  const int64_t r = want < 1 ? 1 : want > 512 ? 512 : want;
-  return (int)(r < M ? r : M);
 }
 
 // ---- up to SKINNY_ROWS rows
@@ -133,7 +93,7 @@ constexpr int SKINNY_WAVES = 8;
 template <typename T, int MT, bool GATE, bool VEC>
 __global__ void __launch_bounds__(SKINNY_WAVES * 64)
 skinny_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ w, const T* __restrict__ w2, int64_t ldw, const T* __restrict__ bias,
-              const T* __restrict__ bias2, T* __restrict__ out, int64_t ldo, T* __restrict__ g_out, T* __restrict__ u_out, int M, int N, int K, int act) {
+              const T* __restrict__ bias2, T* __restrict__ out, int64_t ldo, T* __restrict__ ug_out, T* __restrict__ ag_out, bf16* __restrict__ planes, int M, int N, int K, int act) {
   constexpr int V = Skinny<T>::V, STEP = 4 * V, P = GATE ? 2 : 1;
   __shared__ f32x4 red[SKINNY_WAVES][P][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -186,34 +146,46 @@ skinny_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ w, cons
   }
   const int m = wave * 16 + (lane & 15);
   if (m >= M) return;
+  const int c0 = blockIdx.x * 16 + (lane >> 4) * 4;
+  if constexpr (GATE) {
+    with_activation(act, [&](auto a) __attribute__((always_inline)) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int c = blockIdx.x * 16 + (lane >> 4) * 4 + e;
-    if constexpr (GATE) {
-      if (c >= ((N + 7) & ~7)) continue;
-      float g = 0.f, u = 0.f;  // the padding of a row holds zeros
-      if (c < N) {
-        g = s[0][e] + (bias ? (float)bias[c] : 0.f);
-        u = s[P - 1][e] + (bias2 ? (float)bias2[c] : 0.f);
+      for (int e = 0; e < 4; ++e) {
+        const int c = c0 + e;
+        if (c >= ((N + 7) & ~7)) continue;
+        float h = 0.f, ug = 0.f, ag = 0.f;  // the padding of a row holds zeros
+        if (c < N) {
+          const float g = s[0][e] + (bias ? (float)bias[c] : 0.f), u = s[P - 1][e] + (bias2 ? (float)bias2[c] : 0.f);
+          float slope;
+          activation<decltype(a)::value, sizeof(T) == 2>(g, ag, slope);
+          h = ag * u;
+          ug = u * slope;
+        }
+        const int64_t at = (int64_t)m * ldo + c;
+        out[at] = (T)h;
+        if (ug_out) { ug_out[at] = (T)ug; ag_out[at] = (T)ag; }
+        if (planes) {
+          bf16 t[3];
+          split3(h, t);
+          for (int k = 0; k < 3; ++k) planes[k * M * ldo + at] = t[k];
+        }
       }
-      const int64_t at = (int64_t)m * ldo + c;
-      out[at] = (T)(c < N ? act_value(act, g) * u : 0.f);
-      if (g_out) { g_out[at] = (T)g; u_out[at] = (T)u; }
-    } else {
-      if (c >= N) continue;
-      out[(int64_t)m * ldo + c] = (T)(s[0][e] + (bias ? (float)bias[c] : 0.f));
-    }
+    });
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c0 + e < N) out[(int64_t)m * ldo + c0 + e] = (T)(s[0][e] + (bias ? (float)bias[c0 + e] : 0.f));
   }
 }
 
 template <typename T, bool GATE, bool VEC>
-int skinny_launch(const T* x, int64_t xs, const T* w, const T* w2, int64_t ldw, const T* bias, const T* bias2, T* out, int64_t ldo, T* g, T* u,
-                  int M, int N, int K, int act, hipStream_t st) {
+int skinny_launch(const T* x, int64_t xs, const T* w, const T* w2, int64_t ldw, const T* bias, const T* bias2, T* out, int64_t ldo, T* ug, T* ag,
+                  bf16* planes, int M, int N, int K, int act, hipStream_t st) {
   const dim3 grid((N + 15) / 16), block(SKINNY_WAVES * 64);
   switch ((M + 15) / 16) {
-    case 1: skinny_kernel<T, 1, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, g, u, M, N, K, act); break;
-    case 2: skinny_kernel<T, 2, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, g, u, M, N, K, act); break;
-    default: skinny_kernel<T, 4, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, g, u, M, N, K, act);
+    case 1: skinny_kernel<T, 1, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, ug, ag, planes, M, N, K, act); break;
+    case 2: skinny_kernel<T, 2, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, ug, ag, planes, M, N, K, act); break;
+    default: skinny_kernel<T, 4, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, ug, ag, planes, M, N, K, act);
   }
   return launched("dm_gated_ffn");
 }
@@ -287,33 +259,37 @@ void add_segments(GemmArgs& g, const Operand& a, const Operand& b, const Operand
 template <typename T> using Mat = typename std::conditional<std::is_same<T, float>::value, bf16, T>::type;  // what the matrix pipe sees
 
 template <typename T>
-Out result(void* p, int64_t ld, int N) {  // a tensor of the caller's
-  constexpr bool F32 = std::is_same<T, float>::value;
-  return {p, ld, 0, F32 ? OUT_F32 : OUT_16, ld % 4 == 0 && aligned(p, 4 * sizeof(T))};
+Out result(void* p, int64_t ld) {  // a tensor of the caller's
+  return {p, ld, 0, std::is_same<T, float>::value, ld % (16 / sizeof(T)) == 0 && aligned(p, 16)};
 }
 template <typename T>
 Out between(const Operand& o) {  // an operand of a later product
-  return {const_cast<void*>(o.p), o.ld, o.plane, std::is_same<T, float>::value ? OUT_PLANES : OUT_16, 1};
+  return {const_cast<void*>(o.p), o.ld, o.plane, 0, 1};
 }
 
-// out[M][N] = A B (+ bias), the k range split where that pays.
+// out[M][N] = A B (+ bias), the k range split where that pays; sums: the sum of A over k (both operands KS).
 template <typename T, bool AKS, bool BKS>
-int product(GemmArgs g, const Out& out, const void* bias, void* part, hipStream_t st) {
+int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part, hipStream_t st) {
+  constexpr bool F32 = std::is_same<T, float>::value;
   const GemmPlan plan = gemm_plan(g.M, g.N, g.iters * g.segments, part != nullptr);
   g.splits = plan.splits;
-  g.bias_f32 = std::is_same<T, float>::value;
+  g.sums_f32 = F32;
+  g.sum_segments = F32 ? 1 << 1 | 1 << 4 | 1 << 5 : 1;  // add_segments: each plane of A once
   if (plan.splits == 1) {
     g.out = out;
     g.bias = bias;
+    g.sums = sums;
     return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.big, st);
   }
-  const int ldp = (int)round_up(g.N, 4);
+  const int ldp = (int)round_up(g.N, 8);
   g.split_stride = g.M * ldp;
-  g.out = {part, ldp, 0, OUT_F32, 1};
+  g.out = {part, ldp, 0, 1, 1};
+  float* sum_part = (float*)part + plan.splits * g.split_stride;
+  g.sums = sums ? sum_part : nullptr;
   if (const int rc = gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.big, st)) return rc;
-  const int64_t blocks = (g.M * (ldp / 4) + 255) / 256;
-  gemm_join_kernel<Mat<T>><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>((const float*)part, plan.splits, g.split_stride,
-                                                                                                    bias, g.bias_f32, out, g.M, g.N, ldp);
+  const int64_t blocks = (g.M * (ldp / 8) + 255) / 256;
+  gemm_join_kernel<Mat<T>><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(
+      (const float*)part, plan.splits, g.split_stride, bias, out, g.M, g.N, ldp, sum_part, sums);
   return launched("gated feed-forward block");
 }
 
@@ -322,24 +298,38 @@ inline int64_t pad8(int64_t v) { return round_up(v, 8); }
 
 struct FfnIn { const void *x, *wg, *wu, *wd, *bg, *bu, *bd; int64_t xs; };
 
+// What the forward pass keeps for the backward pass: u act'(g), act(g), and h as an operand of dWd = dy^T h.
+template <typename T>
+struct Saved {
+  T *ug = nullptr, *ag = nullptr;
+  Operand h = {nullptr, 0, 0};
+  Saved(void* p, int64_t M, int F) {
+    if (!p) return;
+    const int64_t Fp = pad8(F);
+    ug = (T*)p;
+    ag = ug + M * Fp;
+    h = {ag + M * Fp, Fp, M * Fp};
+  }
+};
+
 // run: launch; otherwise only count the workspace.
 template <typename T>
 int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int act, Carver& ws, bool run, hipStream_t st) {
+  constexpr bool F32 = std::is_same<T, float>::value;
   const int64_t Fp = pad8(z.F);
-  T* gs = (T*)saved;
-  T* us = saved ? gs + z.M * Fp : nullptr;
+  const Saved<T> kept(saved, z.M, z.F);
   if (z.M <= SKINNY_ROWS) {
-    T* h = (T*)ws.take((size_t)z.M * Fp * sizeof(T));
+    T* h = saved && !F32 ? (T*)kept.h.p : (T*)ws.take((size_t)z.M * Fp * sizeof(T));
     if (!run) return 0;
     constexpr int V = Skinny<T>::V;
     const int M = (int)z.M;
     const bool vg = z.D % V == 0;  // (rows are 16-byte aligned then: ffn_check)
     auto gate = vg ? skinny_launch<T, true, true> : skinny_launch<T, true, false>;
-    if (const int rc = gate((const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp, gs, us, M, z.F, z.D,
-                            act, st))
+    if (const int rc = gate((const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp, kept.ug, kept.ag,
+                            saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act, st))
       return rc;
     auto down = z.F % V == 0 ? skinny_launch<T, false, true> : skinny_launch<T, false, false>;
-    return down(h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, M, z.N, z.F, act, st);
+    return down(h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, M, z.N, z.F, act, st);
   }
   Operand x, wg, wu, wd, h;
   int rc = prepare_operand<T>(x, in.x, in.xs, z.M, z.D, ws, run, st);
@@ -347,8 +337,8 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   if (!rc) rc = prepare_operand<T>(wu, in.wu, z.D, z.F, z.D, ws, run, st);
   if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
   if (rc) return rc;
-  h = take_operand<T>(z.M, z.F, ws);
-  const int segs = std::is_same<T, float>::value ? 6 : 1;
+  h = saved ? kept.h : take_operand<T>(z.M, z.F, ws);
+  const int segs = F32 ? 6 : 1;
   const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F) * segs, true).part_bytes;
   void* part = ws.take(part_bytes);
   if (!run) return 0;
@@ -357,33 +347,22 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   add_segments<T>(g, x, wg, &wu);
   g.M = z.M; g.N = z.F; g.K = z.D; g.iters = iters_of(g.K); g.splits = 1;
   g.out = between<T>(h);
-  g.out2 = result<T>(gs, Fp, z.F);
-  g.out3 = result<T>(us, Fp, z.F);
-  g.bias = in.bg; g.bias2 = in.bu; g.bias_f32 = std::is_same<T, float>::value; g.act = act;
+  g.out2 = result<T>(kept.ug, Fp);
+  g.out3 = result<T>(kept.ag, Fp);
+  g.bias = in.bg; g.bias2 = in.bu; g.act = act;
   const bool big = gemm_plan(z.M, 2 * z.F, g.iters * g.segments, false).big;
-  if ((rc = gemm_launch<Mat<T>, false, false, EPI_GATE>(g, big, st))) return rc;
+  if ((rc = gemm_launch<Mat<T>, false, false, F32 ? EPI_GATE_F32 : EPI_GATE>(g, big, st))) return rc;
 
   GemmArgs d = {};
   add_segments<T>(d, h, wd);
   d.M = z.M; d.N = z.N; d.K = z.F; d.iters = iters_of(z.F);
-  return product<T, false, false>(d, result<T>(y, z.N, z.N), in.bd, part, st);
+  return product<T, false, false>(d, result<T>(y, z.N), in.bd, nullptr, part, st);
 }
 
 struct FfnGrads { void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd; };
 
 template <typename T>
-int column_sums(const Operand& a, const Operand* b, int64_t M, int C, void* out0, void* out1, float* part, hipStream_t st) {
-  constexpr int PL = std::is_same<T, float>::value ? 3 : 1;
-  const int rows = column_sums_rows(M, C);
-  column_sums_kernel<Mat<T>, PL><<<dim3((C + 255) / 256, rows), dim3(64), 0, st>>>((const Mat<T>*)a.p, b ? (const Mat<T>*)b->p : nullptr, a.plane, a.ld, M,
-                                                                                    C, part);
-  if (const int rc = launched("dm_gated_ffn_backward")) return rc;
-  partial_rows_kernel<T><<<dim3((unsigned)((2 * (int64_t)C + 15) / 16)), dim3(256), 0, st>>>(part, rows, C, (T*)out0, (T*)out1);
-  return launched("dm_gated_ffn_backward");
-}
-
-template <typename T>
-int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys, const void* saved, const FfnGrads& gr, int act, Carver& ws, bool run,
+int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys, const void* saved, const FfnGrads& gr, Carver& ws, bool run,
                  hipStream_t st) {
   const int64_t Fp = pad8(z.F);
   const int segs = std::is_same<T, float>::value ? 6 : 1;
@@ -394,40 +373,39 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   if (!rc) rc = prepare_operand<T>(wg, in.wg, z.D, z.F, z.D, ws, run && gr.dx, st);
   if (!rc) rc = prepare_operand<T>(wu, in.wu, z.D, z.F, z.D, ws, run && gr.dx, st);
   if (rc) return rc;
-  const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws), h = take_operand<T>(z.M, z.F, ws);
+  const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws);
+  const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
   const int rows_it = iters_of(z.M) * segs;
   size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F) * segs * 2, true).part_bytes;
-  const size_t more[] = {gemm_plan(z.F, z.D, rows_it, true).part_bytes, gemm_plan(z.N, z.F, rows_it, true).part_bytes,
-                         (size_t)column_sums_rows(z.M, z.F) * 2 * z.F * 4, (size_t)column_sums_rows(z.M, z.N) * 2 * z.N * 4};
+  const size_t more[] = {gemm_plan(z.F, z.D, rows_it, true).part_bytes, gemm_plan(z.N, z.F, rows_it, true).part_bytes};
   for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
   void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
   if (!run) return 0;
 
-  GemmArgs a = {};  // dh, and from it dg, du and h
+  GemmArgs a = {};  // dh, and from it dg and du
   add_segments<T>(a, y, wd);
   a.M = z.M; a.N = z.F; a.K = z.N; a.iters = iters_of(a.K); a.splits = 1;
-  a.out = between<T>(dg); a.out2 = between<T>(du); a.out3 = between<T>(h);
-  a.g = saved; a.u = (const T*)saved + z.M * Fp; a.ldg = Fp; a.gu_f32 = std::is_same<T, float>::value; a.act = act;
-  if ((rc = gemm_launch<Mat<T>, false, true, EPI_DACT>(a, gemm_plan(z.M, z.F, a.iters * a.segments, false).big, st))) return rc;
+  a.out = between<T>(dg); a.out2 = between<T>(du);
+  a.ug = kept.ug; a.ag = kept.ag; a.ldg = Fp;
+  if ((rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, gemm_plan(z.M, z.F, a.iters * a.segments, false).big, st))) return rc;
 
   if (gr.dx) {
     GemmArgs g = {};
     add_segments<T>(g, dg, wg);
     add_segments<T>(g, du, wu);
     g.M = z.M; g.N = z.D; g.K = z.F; g.iters = iters_of(z.F);
-    if ((rc = product<T, false, true>(g, result<T>(gr.dx, z.D, z.D), nullptr, part, st))) return rc;
+    if ((rc = product<T, false, true>(g, result<T>(gr.dx, z.D), nullptr, nullptr, part, st))) return rc;
   }
-  auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out) {
+  // (the sum of dg^T, du^T, dy^T over the rows of the batch is the bias' gradient)
+  auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out, void* bias) {
     GemmArgs g = {};
     add_segments<T>(g, l, r);
     g.M = rows; g.N = cols; g.K = (int)z.M; g.iters = iters_of(z.M);
-    return product<T, true, true>(g, result<T>(out, cols, cols), nullptr, part, st);
+    return product<T, true, true>(g, result<T>(out, cols), nullptr, bias, part, st);
   };
-  if (gr.dwg && (rc = weight(dg, x, z.F, z.D, gr.dwg))) return rc;
-  if (gr.dwu && (rc = weight(du, x, z.F, z.D, gr.dwu))) return rc;
-  if (gr.dwd && (rc = weight(y, h, z.N, z.F, gr.dwd))) return rc;
-  if ((gr.dbg || gr.dbu) && (rc = column_sums<T>(dg, &du, z.M, z.F, gr.dbg, gr.dbu, (float*)part, st))) return rc;
-  if (gr.dbd && (rc = column_sums<T>(y, nullptr, z.M, z.N, gr.dbd, nullptr, (float*)part, st))) return rc;
+  if (gr.dwg && (rc = weight(dg, x, z.F, z.D, gr.dwg, gr.dbg))) return rc;
+  if (gr.dwu && (rc = weight(du, x, z.F, z.D, gr.dwu, gr.dbu))) return rc;
+  if (gr.dwd && (rc = weight(y, kept.h, z.N, z.F, gr.dwd, gr.dbd))) return rc;
   return 0;
 }
 
@@ -473,15 +451,15 @@ extern "C" {
 size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype) {
   using namespace dmb;
   if (M <= 0 || F < 1 || !dtype_ok(dtype)) return 0;
-  return (size_t)2 * M * pad8(F) * dtype_size(dtype);
+  return (size_t)M * pad8(F) * (dtype == DM_F32 ? 2 * 4 + 3 * 2 : 3 * 2);
 }
 
-size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype) {
+size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype, int save) {
   using namespace dmb;
   const FfnSizes z = {M, D, F, N, dtype};
   if (M <= 0 || ffn_check("dm_gated_ffn_workspace_bytes", z, DM_ACT_SILU)) return 0;
   Carver ws = {nullptr};
-  ffn_types(dtype, [&](auto t) { return ffn_forward<decltype(t)>(z, FfnIn{}, nullptr, nullptr, 0, ws, false, nullptr); });
+  ffn_types(dtype, [&](auto t) { return ffn_forward<decltype(t)>(z, FfnIn{}, nullptr, save ? &ws : nullptr, 0, ws, false, nullptr); });
   return ws.used;
 }
 
@@ -491,7 +469,7 @@ size_t dm_gated_ffn_backward_workspace_bytes(int64_t M, int D, int F, int N, int
   if (M <= 0 || ffn_check("dm_gated_ffn_backward_workspace_bytes", z, DM_ACT_SILU)) return 0;
   Carver ws = {nullptr};
   ffn_types(dtype, [&](auto t) {
-    return ffn_backward<decltype(t)>(z, FfnIn{}, nullptr, 0, nullptr, FfnGrads{}, 0, ws, false, nullptr);
+    return ffn_backward<decltype(t)>(z, FfnIn{}, nullptr, 0, nullptr, FfnGrads{}, ws, false, nullptr);
   });
   return ws.used;
 }
@@ -509,7 +487,7 @@ int dm_gated_ffn(const void* x_dev, int64_t x_stride, const void* w_gate_dev, co
     return 1;
   if (!y_dev) return fail("%s: null argument (y)", who);
   if (saved_dev && !aligned(saved_dev, 16)) return fail("%s: saved must be aligned to 16 bytes", who);
-  const size_t need = dm_gated_ffn_workspace_bytes(M, D, F, N, dtype);
+  const size_t need = dm_gated_ffn_workspace_bytes(M, D, F, N, dtype, saved_dev != nullptr);
   if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16))
     return fail("%s: workspace of %zu bytes, %zu needed (aligned to 16)", who, workspace_dev ? workspace_bytes : (size_t)0, need);
   const FfnIn in = {x_dev, w_gate_dev, w_up_dev, w_down_dev, b_gate_dev, b_up_dev, b_down_dev, x_stride};
@@ -542,6 +520,8 @@ int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_d
       ffn_check_matrix(who, "w_gate", w_gate_dev, D, F, D, dtype) || ffn_check_matrix(who, "w_up", w_up_dev, D, F, D, dtype) ||
       ffn_check_matrix(who, "w_down", w_down_dev, F, N, F, dtype))
     return 1;
+  if ((db_gate_dev && !dw_gate_dev) || (db_up_dev && !dw_up_dev) || (db_down_dev && !dw_down_dev))
+    return fail("%s: a bias' gradient comes with its weight's", who);
   if (!saved_dev || !aligned(saved_dev, 16)) return fail("%s: saved must be what dm_gated_ffn wrote, aligned to 16 bytes", who);
   const size_t need = dm_gated_ffn_backward_workspace_bytes(M, D, F, N, dtype);
   if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16))
@@ -550,7 +530,7 @@ int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_d
   const FfnGrads gr = {dx_dev, dw_gate_dev, dw_up_dev, dw_down_dev, db_gate_dev, db_up_dev, db_down_dev};
   Carver ws = {(char*)workspace_dev};
   return ffn_types(dtype,
-                   [&](auto t) { return ffn_backward<decltype(t)>(z, in, dy_dev, dy_stride, saved_dev, gr, activation, ws, true, st); });
+                   [&](auto t) { return ffn_backward<decltype(t)>(z, in, dy_dev, dy_stride, saved_dev, gr, ws, true, st); });
 }
 
 }  // extern "C"

@@ -8,9 +8,12 @@
 // A workgroup owns a BM x BN tile and walks k in steps of 64: two LDS stages, filled by buffer loads that write LDS directly (16 bytes
 // per lane, rows and columns out of range are bounds-checked to zero by the buffer resource), one barrier per step.  The LDS image
 // is swizzled in 16-byte pieces so that fragment reads touch all 64 banks once.  Fragments feed v_mfma_f32_32x32x16 with the n side as
-// the first operand: a lane then holds four consecutive n of one m, which the epilogue stores as one vector.
+// the first operand, its rows permuted: a lane then holds sixteen consecutive n of one m, which the epilogue stores as whole vectors.
+// A bias' gradient, the sum of A over k, is one more product with ones from the same fragments.
 #ifndef DM_BLOCK_GEMM_HIP
 #define DM_BLOCK_GEMM_HIP
+#include <type_traits>
+
 #include "dm_block_common.h"
 
 namespace dmb {
@@ -44,70 +47,93 @@ __device__ __forceinline__ void split3(float v, bf16 (&t)[3]) {
 }
 
 enum { OUT_16 = 0, OUT_F32 = 1, OUT_PLANES = 2 };
-// Where a result goes: rows of `ld` elements; OUT_PLANES: three bf16 planes, `plane` elements apart.  `vec`: rows take 4-element stores.
-struct Out { void* p; int64_t ld, plane; int mode, vec; };
+// Where a result goes: rows of `ld` elements; OUT_PLANES: three bf16 planes, `plane` elements apart.  `vec`: rows take 16-byte stores.
+struct Out { void* p; int64_t ld, plane; int f32, vec; };
 
-template <typename T>
-__device__ __forceinline__ void store4(const Out& o, int64_t m, int n, int N, const float (&v)[4]) {
+template <typename T, int MODE>
+__device__ __forceinline__ void store8(const Out& o, int64_t m, int n, int N, const float (&v)[8]) {
   const int64_t at = m * o.ld + n;
-  if (o.vec && n + 4 <= N) {
-    if (o.mode == OUT_F32) {
-      store_vec<float, 4>((float*)o.p + at, v);
-    } else if (o.mode == OUT_16) {
-      store_vec<T, 4>((T*)o.p + at, v);
+  if (o.vec && n + 8 <= N) {
+    if constexpr (MODE == OUT_16) {
+      store_vec<T, 8>((T*)o.p + at, v);
+    } else if constexpr (MODE == OUT_F32) {
+      const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+      store_vec<float, 4>((float*)o.p + at, a);
+      store_vec<float, 4>((float*)o.p + at + 4, b);
     } else {
-      Vec<bf16, 4> r[3];
+      Vec<bf16, 8> r[3];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { bf16 t[3]; split3(v[i], t); r[0].v[i] = t[0]; r[1].v[i] = t[1]; r[2].v[i] = t[2]; }
+      for (int i = 0; i < 8; ++i) { bf16 t[3]; split3(v[i], t); r[0].v[i] = t[0]; r[1].v[i] = t[1]; r[2].v[i] = t[2]; }
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<bf16, 4>*>((bf16*)o.p + k * o.plane + at) = r[k];
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<bf16, 8>*>((bf16*)o.p + k * o.plane + at) = r[k];
     }
     return;
   }
+  if constexpr (MODE != OUT_PLANES) {  // (planes are the block's own and take whole pieces)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (n + i >= N) break;
-    if (o.mode == OUT_F32) ((float*)o.p)[at + i] = v[i];
-    else if (o.mode == OUT_16) ((T*)o.p)[at + i] = (T)v[i];
-    else { bf16 t[3]; split3(v[i], t); for (int k = 0; k < 3; ++k) ((bf16*)o.p)[k * o.plane + at + i] = t[k]; }
+    for (int i = 0; i < 8; ++i) {
+      if (n + i >= N) break;
+      if constexpr (MODE == OUT_16) ((T*)o.p)[at + i] = (T)v[i];
+      else ((float*)o.p)[at + i] = v[i];
+    }
   }
 }
 
-// ---- activations: value and slope, fp32
-__device__ __forceinline__ float act_value(int act, float v) {
-  switch (act) {
-    case DM_ACT_RELU: return v > 0.f ? v : (v != v ? v : 0.f);
-    case DM_ACT_GELU: return v * (0.5f * (1.f + erff(v * 0.70710678f)));
-    case DM_ACT_GELU_TANH: return 0.5f * v * (1.f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
-    case DM_ACT_SIGMOID: return 1.f / (1.f + expf(-v));
-    default: return v / (1.f + expf(-v));
+// ---- activations: value and slope in fp32, all but the erf form by way of s(z) = 1 / (1 + exp(-z)); tanh's by 1 + tanh(y) = 2 s(2 y).
+// Results that are rounded to 16 bits take the hardware's exp2 and reciprocal (relative error below 2^-20 for |z| < 16).
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float z) {
+  if (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+  return 1.f / (1.f + expf(-z));
+}
+template <int ACT, bool FAST>
+__device__ __forceinline__ void activation(float v, float& value, float& slope) {
+  if constexpr (ACT == DM_ACT_RELU) {
+    value = v > 0.f ? v : (v != v ? v : 0.f);
+    slope = v > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == DM_ACT_GELU) {
+    const float cdf = 0.5f * erfcf(v * -0.70710678f);
+    value = v * cdf;
+    slope = cdf + v * expf(-0.5f * v * v) * 0.39894228f;
+  } else if constexpr (ACT == DM_ACT_GELU_TANH) {
+    const float s = sigmoid<FAST>(1.5957691f * (v + 0.044715f * v * v * v));
+    value = v * s;
+    slope = s + v * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * v * v);
+  } else {
+    const float s = sigmoid<FAST>(v);
+    value = ACT == DM_ACT_SIGMOID ? s : v * s;
+    slope = ACT == DM_ACT_SIGMOID ? s * (1.f - s) : s * (1.f + v * (1.f - s));
   }
 }
-__device__ __forceinline__ void act_slope(int act, float v, float& value, float& slope) {
+// f(constant) for the activation at run time
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
   switch (act) {
-    case DM_ACT_RELU: value = v > 0.f ? v : (v != v ? v : 0.f); slope = v > 0.f ? 1.f : 0.f; break;
-    case DM_ACT_GELU: {
-      const float cdf = 0.5f * (1.f + erff(v * 0.70710678f));
-      value = v * cdf;
-      slope = cdf + v * expf(-0.5f * v * v) * 0.39894228f;
-      break;
-    }
-    case DM_ACT_GELU_TANH: {
-      const float t = tanhf(0.79788456f * (v + 0.044715f * v * v * v));
-      value = 0.5f * v * (1.f + t);
-      slope = 0.5f * (1.f + t) + 0.5f * v * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * v * v);
-      break;
-    }
-    case DM_ACT_SIGMOID: { const float s = 1.f / (1.f + expf(-v)); value = s; slope = s * (1.f - s); break; }
-    default: { const float s = 1.f / (1.f + expf(-v)); value = v * s; slope = s * (1.f + v * (1.f - s)); }
+    case DM_ACT_RELU: return f(std::integral_constant<int, DM_ACT_RELU>{});
+    case DM_ACT_GELU: return f(std::integral_constant<int, DM_ACT_GELU>{});
+    case DM_ACT_GELU_TANH: return f(std::integral_constant<int, DM_ACT_GELU_TANH>{});
+    case DM_ACT_SIGMOID: return f(std::integral_constant<int, DM_ACT_SIGMOID>{});
+    default: return f(std::integral_constant<int, DM_ACT_SILU>{});
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) { load_vec<T, 4>(p, v); }
+template <typename S>
+__device__ __forceinline__ float bias_at(const void* b, int n, int N) { return b && n < N ? (float)((const S*)b)[n] : 0.f; }
+template <typename S>
+__device__ __forceinline__ void load8(const S* p, float (&v)[8]) {
+  if constexpr (sizeof(S) == 4) {
+    float a[4], b[4];
+    load_vec<float, 4>(p, a);
+    load_vec<float, 4>(p + 4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+  } else {
+    load_vec<S, 8>(p, v);
+  }
+}
 
 constexpr int GEMM_MAX_SEGMENTS = 12;
-enum { EPI_STORE = 0, EPI_GATE = 1, EPI_DACT = 2 };
+enum { EPI_STORE, EPI_GATE, EPI_GATE_F32, EPI_DACT, EPI_DACT_F32 };  // _F32: of split fp32 operands
 
 struct GemmArgs {
   const void* a[GEMM_MAX_SEGMENTS];
@@ -118,26 +144,36 @@ struct GemmArgs {
   int64_t M;
   int N, K;                           // N: of one projection for EPI_GATE.  K: true length; a KC row is zero from there to the end of its piece
   int tiles_m, tiles_n, splits;
-  Out out, out2, out3;                // STORE: out.  GATE: out = h, out2 = g, out3 = u (null: not kept).  DACT: dg, du, h
-  const void *bias, *bias2;           // of the element type given by bias_f32
-  int bias_f32;
-  const void *g, *u;                  // DACT: saved projections, rows of ldg
+  Out out, out2, out3;                // STORE: out.  GATE: out = h, and for the backward pass (null: not kept) out2 = u act'(g), out3 = act(g).
+                                      // DACT: out = dg, out2 = du
+  const void *bias, *bias2;           // of the result's type; GATE: of the operands'
+  const void *ug, *ag;                // DACT: u act'(g) and act(g), rows of ldg
   int64_t ldg;
-  int gu_f32, act;
+  int act;
   int64_t split_stride;               // STORE with splits > 1: fp32 partial products, elements from one split to the next
+  void* sums;                         // STORE with both operands KS: sum over k of A[m, k] over the segments of sum_segments, or null.  One split:
+  int sum_segments, sums_f32;         // of the type that sums_f32 gives; several: fp32, M apart
 };
 
 template <int N>  // piece of 16 bytes that holds piece `c` of row k of a KS tile with N columns
 __device__ __forceinline__ int ks_swizzle(int k, int c) { return N >= 128 ? c ^ ((k & 3) << 2) : c ^ (((k >> 1) & 1) << 2); }
 
+// The n side of a 32 x 32 product is permuted in blocks of four rows, so that a lane's sixteen results are sixteen consecutive n: row r of
+// the instruction is n = permuted(r), and its piece c of a KC stage lies at c ^ key(n): sixteen lanes read sixteen pieces of all 64 banks.
+__device__ __forceinline__ int permuted(int r) { return ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3); }
+template <bool PERM>
+__device__ __forceinline__ int kc_key(int row) { return PERM ? ((row >> 1) & 3) | ((row >> 2) & 4) : (row >> 1) & 7; }
+
 // One LDS stage of one operand: R rows (of A or B) x 64 k, 16-bit elements, by the NW waves of the block.
-template <int R, bool KS, int NW>
+template <int R, bool KS, int NW, bool PERM>
 struct Stager {
   static constexpr int PASSES = R * 8 / (64 * NW);  // 16-byte pieces per lane
   static constexpr int CPR = KS ? R / 8 : 8;        // pieces per LDS row
   static constexpr int RPW = 64 / CPR;              // LDS rows that one wave's load fills
   uint32_t off[PASSES];                             // byte offset from the tile's corner, 2^31 where the piece lies outside
   int kpos[PASSES];                                 // k of the piece within the step
+  // GATE: rows 64 i .. +31 of the tile are rows 32 i of the first projection's weights, +32 .. +63 the second's
+  template <bool GATE>
   __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int64_t rows_left) {
 #pragma unroll
     for (int j = 0; j < PASSES; ++j) {
@@ -147,8 +183,9 @@ struct Stager {
         off[j] = c * 8 < rows_left ? (uint32_t)(row * ld * 2 + c * 16) : 0x80000000u;
         kpos[j] = row;
       } else {
-        const int c = slot ^ ((row >> 1) & 7);
-        off[j] = row < rows_left ? (uint32_t)(row * ld * 2 + c * 16) : 0x80000000u;
+        const int c = slot ^ kc_key<PERM>(row);
+        const int r = GATE ? row / 64 * 32 + row % 32 : row;
+        off[j] = r < rows_left ? (uint32_t)(r * ld * 2 + c * 16) : 0x80000000u;
         kpos[j] = c * 8;
       }
     }
@@ -166,45 +203,36 @@ __device__ __forceinline__ i32x4 buffer_of(const void* p) {
 __device__ __forceinline__ void stage_arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Fragments of 32 rows x 16 k (step s of 4) out of a stage.
-template <int R, bool KS>
-struct Fragments {
-  uint32_t base;
-  int tile;  // first 32-row tile of this wave
-  __device__ __forceinline__ void init(int lane, int tile0) {
-    tile = tile0;
-    if constexpr (KS) {
-      const int g = lane >> 4, j = (lane >> 2) & 3, c = lane & 3;
-      base = ((g >> 1) * 8 + j) * R * 2 + (c & 1) * 8;  // + the swizzled piece
-    } else {
-      base = (lane & 31) * 128;
-    }
-  }
-  __device__ __forceinline__ s16x8 get(const char DM_LDS* stage, int lane, int t, int s) const {
-    if constexpr (KS) {
-      const int g = lane >> 4, j = (lane >> 2) & 3, c = lane & 3;
-      const int k = (g >> 1) * 8 + j;  // plus multiples of 4: the swizzle sees only its low bits
-      const int piece = (tile + t) * 4 + (g & 1) * 2 + (c >> 1);
-      s16x4 h[2];
+template <int R, bool KS, bool PERM>
+__device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, int tile, int s) {
+  if constexpr (KS) {
+    // A lane asks for 4 consecutive rows of one k; of 16 lanes' answers, lane i receives row i of four k.
+    const int g = lane >> 4, j = (lane >> 2) & 3;
+    const int blk = (g & 1) * 4 + (lane & 3), four = PERM ? (blk & 1) * 4 + (blk >> 1) : blk;
+    const int piece = tile * 4 + (four >> 1);
+    s16x4 h[2];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int kk = s * 16 + q * 4 + k;
-        h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DM_LDS s16x4*)(stage + kk * (R * 2) + ks_swizzle<R>(kk, piece) * 16 + (c & 1) * 8));
-      }
-      return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
-    } else {
-      const int row = (tile + t) * 32 + (lane & 31);
-      const int c = (2 * s + (lane >> 5)) ^ ((lane >> 1) & 7);  // (row >> 1) & 7 of a row that is lane & 31 above a multiple of 32
-      return *(const DM_LDS s16x8*)(stage + row * 128 + c * 16);
+    for (int q = 0; q < 2; ++q) {
+      const int k = s * 16 + (g >> 1) * 8 + q * 4 + j;
+      h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DM_LDS s16x4*)(stage + k * (R * 2) + ks_swizzle<R>(k, piece) * 16 + (four & 1) * 8));
     }
+    return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
+  } else {
+    const int r = PERM ? permuted(lane & 31) : lane & 31;
+    return *(const DM_LDS s16x8*)(stage + (tile * 32 + r) * 128 + ((2 * s + (lane >> 5)) ^ kc_key<PERM>(r)) * 16);
   }
-};
+}
 
 template <typename T, int BM, int BN, int WM, int WN, bool AKS, bool BKS, int EPI>
-__global__ void __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 2)
+__global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm_kernel(const GemmArgs p) {
   constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
-  static_assert(EPI != EPI_GATE || (NI == 2 && !BKS), "a wave of the gated product owns 32 columns of each projection");
+  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
+  using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
+  constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
+  static_assert(!GATE || (NI == 2 && !BKS), "a wave of the gated product owns 32 columns of each projection");
+  static_assert(!SUMS || MI == WN, "each of the waves of a tile row sums one of its 32-row blocks");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -223,172 +251,177 @@ gemm_kernel(const GemmArgs p) {
   const int rows = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
   const int tm = first + tile % band % rows, tn = tile % band / rows;
   const int64_t m0 = (int64_t)tm * BM;
-  constexpr int BROWS = EPI == EPI_GATE ? BN / 2 : BN;  // columns of one projection in the tile
-  const int n0 = tn * BROWS;
+  const int n0 = tn * (GATE ? BN / 2 : BN);
 
   const int total = p.segments * p.iters;
   const int per = (total + p.splits - 1) / p.splits;
   const int it0 = blockIdx.y * per, it1 = it0 + per < total ? it0 + per : total;
 
-  Stager<BM, AKS, NW> sa;
-  Stager<BN, BKS, NW> sb;
-  sa.init(wave, lane, p.lda, p.M - m0);
-  if constexpr (EPI == EPI_GATE) {  // rows 64 i .. +31 of the tile are the first projection's, +32 .. +63 the second's
-#pragma unroll
-    for (int j = 0; j < sb.PASSES; ++j) {
-      const int row = (j * NW + wave) * 8 + lane / 8, slot = lane % 8, c = slot ^ ((row >> 1) & 7);
-      const int f = row / 64 * 32 + row % 32;
-      sb.off[j] = n0 + f < p.N ? (uint32_t)(f * p.ldb * 2 + c * 16) : 0x80000000u;
-      sb.kpos[j] = c * 8;
-    }
-  } else {
-    sb.init(wave, lane, p.ldb, p.N - n0);
-  }
-  Fragments<BM, AKS> fa;
-  Fragments<BN, BKS> fb;
-  fa.init(lane, wm * MI);
-  fb.init(lane, wn * NI);
+  Stager<BM, AKS, NW, false> sa;
+  Stager<BN, BKS, NW, true> sb;
+  sa.template init<false>(wave, lane, p.lda, p.M - m0);
+  sb.template init<GATE>(wave, lane, p.ldb, p.N - n0);
 
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
   // (the segments' pointers are read where the launch put the arguments: indexing the parameter itself would copy it to scratch)
   const auto* args = (const __attribute__((address_space(4))) GemmArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-  auto issue = [&](int it, uint32_t stage) {
-    const int seg = it / p.iters, k0 = (it - seg * p.iters) * 64;
-    const int left = p.K - k0;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
+  int seg = it0 / p.iters, step = it0 - seg * p.iters;  // of the next stage to be asked for
+  auto issue = [&](uint32_t stage) {
+    const int k0 = step * 64, left = p.K - k0;
     const i32x4 ra = buffer_of((const char*)args->a[seg] + (AKS ? (int64_t)k0 * p.lda + m0 : m0 * p.lda + k0) * 2);
 #pragma unroll
     for (int j = 0; j < sa.PASSES; ++j)
       load_to_lds(ra, sa.kpos[j] < left ? sa.off[j] : 0x80000000u, lds0 + stage + (j * NW + wave) * 1024);
     const int64_t bo = (BKS ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0) * 2;
     const i32x4 rb = buffer_of((const char*)args->b[seg] + bo);
-    if constexpr (EPI == EPI_GATE) {
-      const i32x4 rb2 = buffer_of((const char*)args->b2[seg] + bo);
+    i32x4 rb2 = rb;
+    if constexpr (GATE) rb2 = buffer_of((const char*)args->b2[seg] + bo);
 #pragma unroll
-      for (int j = 0; j < sb.PASSES; ++j)
-        load_to_lds((j * NW + wave) / 4 % 2 ? rb2 : rb, sb.kpos[j] < left ? sb.off[j] : 0x80000000u,
-                    lds0 + stage + ABYTES + (j * NW + wave) * 1024);
-    } else {
-#pragma unroll
-      for (int j = 0; j < sb.PASSES; ++j)
-        load_to_lds(rb, sb.kpos[j] < left ? sb.off[j] : 0x80000000u, lds0 + stage + ABYTES + (j * NW + wave) * 1024);
-    }
+    for (int j = 0; j < sb.PASSES; ++j)
+      load_to_lds(GATE && (j * NW + wave) / 4 % 2 ? rb2 : rb, sb.kpos[j] < left ? sb.off[j] : 0x80000000u,
+                  lds0 + stage + ABYTES + (j * NW + wave) * 1024);
+    if (++step == p.iters) { step = 0; ++seg; }
   };
 
-  f32x16 acc[MI][NI];
+  f32x16 acc[MI][NI], asum;
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int e = 0; e < 16; ++e) {
+    asum[e] = 0.f;
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      for (int j = 0; j < NI; ++j) acc[i][j][e] = 0.f;
+  }
+  const short unit = __builtin_bit_cast(short, (T)1.f);
+  const s16x8 ones = {unit, unit, unit, unit, unit, unit, unit, unit};
 
   uint32_t cur = 0;
-  if (it0 < it1) issue(it0, 0);
+  int now = seg;  // the segment of the stage at hand
+  if (it0 < it1) issue(0);
   for (int it = it0; it < it1; ++it) {
+    const bool sum = SUMS && p.sums && tn == 0 && (p.sum_segments >> now & 1);
+    now = seg;
     stage_arrived();  // this step's tiles are in LDS, and every wave is done with the other stage
-    if (it + 1 < it1) issue(it + 1, cur ^ STAGE);
+    if (it + 1 < it1) issue(cur ^ STAGE);
     const char DM_LDS* st = (const char DM_LDS*)smem + cur;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       s16x8 a[MI], b[NI];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = fa.get(st, lane, i, s);
+      for (int i = 0; i < MI; ++i) a[i] = fragment<BM, AKS, false>(st, lane, wm * MI + i, s);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = fb.get(st + ABYTES, lane, j, s);
+      for (int j = 0; j < NI; ++j) b[j] = fragment<BN, BKS, true>(st + ABYTES, lane, wn * NI + j, s);
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(b[j], a[i], acc[i][j], T());
+      if constexpr (SUMS) {
+        if (sum) asum = mfma16(ones, fragment<BM, AKS, false>(st, lane, wm * MI + wn, s), asum, T());
+      }
     }
     cur ^= STAGE;
   }
 
-  // acc[i][j][4 q + e] belongs to m = lane & 31 and n = 8 q + 4 (lane >> 5) + e of the 32 x 32 block (i, j).
+  // acc[i][j][e] belongs to m = lane & 31 and n = 16 (lane >> 5) + e of the 32 x 32 block (i, j).
   const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces (with zeros: rows of B out of range are zero)
+  const int half = (lane >> 5) * 16;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int64_t m = m0 + (wm * MI + i) * 32 + (lane & 31);
     if (m >= p.M) continue;
-    if constexpr (EPI == EPI_GATE) {
+    if constexpr (GATE) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn * 32 + q * 8 + (lane >> 5) * 4;
+      for (int q = 0; q < 2; ++q) {
+        const int n = n0 + wn * 32 + half + q * 8;
         if (n >= np) continue;
-        float g[4], u[4], h[4];
+        float g[8], u[8], h[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] = acc[i][0][q * 4 + e];
-          u[e] = acc[i][1][q * 4 + e];
-          if (n + e < p.N) {
-            if (p.bias) g[e] += p.bias_f32 ? ((const float*)p.bias)[n + e] : (float)((const T*)p.bias)[n + e];
-            if (p.bias2) u[e] += p.bias_f32 ? ((const float*)p.bias2)[n + e] : (float)((const T*)p.bias2)[n + e];
-          }
-          h[e] = act_value(p.act, g[e]) * u[e];
+        for (int e = 0; e < 8; ++e) {
+          g[e] = acc[i][0][q * 8 + e] + bias_at<Kept>(p.bias, n + e, p.N);
+          u[e] = acc[i][NI - 1][q * 8 + e] + bias_at<Kept>(p.bias2, n + e, p.N);
         }
-        store4<T>(p.out, m, n, np, h);
-        if (p.out2.p) { store4<T>(p.out2, m, n, np, g); store4<T>(p.out3, m, n, np, u); }
+        with_activation(p.act, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float value, slope;
+            activation<decltype(act)::value, !F32>(g[e], value, slope);
+            h[e] = value * u[e];
+            u[e] *= slope;
+            g[e] = value;
+          }
+        });
+        store8<T, BETWEEN>(p.out, m, n, np, h);
+        if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, g); }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + (wn * NI + j) * 32 + q * 8 + (lane >> 5) * 4;
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e];
+        for (int q = 0; q < 2; ++q) {
+          const int n = n0 + (wn * NI + j) * 32 + half + q * 8;
+          float v[8];
           if constexpr (EPI == EPI_STORE) {
             if (n >= p.N) continue;
-            if (p.bias)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n + e < p.N) v[e] += p.bias_f32 ? ((const float*)p.bias)[n + e] : (float)((const T*)p.bias)[n + e];
+            for (int e = 0; e < 8; ++e)
+              v[e] = acc[i][j][q * 8 + e] + (p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N));
             Out o = p.out;
             if (p.splits > 1) o.p = (float*)o.p + blockIdx.y * p.split_stride;
-            store4<T>(o, m, n, p.N, v);
+            if (o.f32) store8<T, OUT_F32>(o, m, n, p.N, v);
+            else store8<T, OUT_16>(o, m, n, p.N, v);
           } else {
             if (n >= np) continue;
-            float g[4], u[4], dg[4], du[4], h[4];
-            if (p.gu_f32) { load4((const float*)p.g + m * p.ldg + n, g); load4((const float*)p.u + m * p.ldg + n, u); }
-            else { load4((const T*)p.g + m * p.ldg + n, g); load4((const T*)p.u + m * p.ldg + n, u); }
+            float ug[8], ag[8];
+            load8((const Kept*)p.ug + m * p.ldg + n, ug);
+            load8((const Kept*)p.ag + m * p.ldg + n, ag);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float value, slope;
-              act_slope(p.act, g[e], value, slope);
-              dg[e] = v[e] * u[e] * slope;
-              du[e] = v[e] * value;
-              h[e] = value * u[e];
-            }
-            store4<T>(p.out, m, n, np, dg);
-            store4<T>(p.out2, m, n, np, du);
-            store4<T>(p.out3, m, n, np, h);
+            for (int e = 0; e < 8; ++e) { v[e] = acc[i][j][q * 8 + e] * ug[e]; ag[e] *= acc[i][j][q * 8 + e]; }
+            store8<T, BETWEEN>(p.out, m, n, np, v);
+            store8<T, BETWEEN>(p.out2, m, n, np, ag);
           }
         }
     }
   }
+  if constexpr (EPI == EPI_STORE) {
+    if constexpr (SUMS) {  // every n of the product with ones holds the sum
+      const int64_t m = m0 + (wm * MI + wn) * 32 + lane;
+      if (p.sums && tn == 0 && lane < 32 && m < p.M) {
+        if (p.splits > 1) ((float*)p.sums)[blockIdx.y * p.M + m] = asum[0];
+        else if (p.sums_f32) ((float*)p.sums)[m] = asum[0];
+        else ((T*)p.sums)[m] = (T)asum[0];
+      }
+    }
+  }
 }
 
-// Adds the partial products of a split k range, the bias, and rounds once.
+// Adds the partial products of a split k range (and the partial sums of A), the bias, and rounds once.
 template <typename T>
 __global__ void __launch_bounds__(256)
-gemm_join_kernel(const float* __restrict__ part, int splits, int64_t stride, const void* bias, int bias_f32, Out out, int64_t M, int N, int ldp) {
-  const int quads = ldp / 4;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < M * quads; id += (int64_t)gridDim.x * 256) {
-    const int64_t m = id / quads;
-    const int n = (int)(id % quads) * 4;
-    if (n >= N) continue;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+gemm_join_kernel(const float* __restrict__ part, int splits, int64_t stride, const void* bias, const Out out, int64_t M, int N, int ldp,
+                 const float* __restrict__ sum_part, void* sums) {
+  const int pieces = ldp / 8;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < M * pieces; id += (int64_t)gridDim.x * 256) {
+    const int64_t m = id / pieces;
+    const int n = (int)(id % pieces) * 8;
+    float v[8] = {};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-      float w[4];
-      load4(part + s * stride + m * ldp + n, w);
+      float w[8];
+      load8(part + s * stride + m * ldp + n, w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += w[e];
+      for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
-    if (bias)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < N) v[e] += bias_f32 ? ((const float*)bias)[n + e] : (float)((const T*)bias)[n + e];
-    store4<T>(out, m, n, N, v);
+    for (int e = 0; e < 8; ++e) v[e] += out.f32 ? bias_at<float>(bias, n + e, N) : bias_at<T>(bias, n + e, N);
+    if (out.f32) store8<T, OUT_F32>(out, m, n, N, v);
+    else store8<T, OUT_16>(out, m, n, N, v);
+  }
+  if (!sums) return;
+  for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < M; m += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += sum_part[s * M + m];
+    if (out.f32) ((float*)sums)[m] = v;
+    else ((T*)sums)[m] = (T)v;
   }
 }
 
@@ -414,13 +447,13 @@ inline GemmPlan gemm_plan(int64_t M, int N, int iters, bool can_split) {
       if (c < cost) { cost = c; best.big = big; best.splits = s; }
     }
   }
-  if (best.splits > 1) best.part_bytes = (size_t)best.splits * M * round_up(N, 4) * 4;
+  if (best.splits > 1) best.part_bytes = (size_t)best.splits * M * (round_up(N, 8) + 1) * 4;  // products, and sums of A
   return best;
 }
 
 template <typename T, bool AKS, bool BKS, int EPI>
 int gemm_launch(GemmArgs a, bool big, hipStream_t st) {
-  const int bm = big ? 256 : 128, bn = EPI == EPI_GATE ? bm / 2 : bm;
+  const int bm = big ? 256 : 128, bn = EPI == EPI_GATE || EPI == EPI_GATE_F32 ? bm / 2 : bm;
   a.tiles_m = (int)((a.M + bm - 1) / bm);
   a.tiles_n = (a.N + bn - 1) / bn;
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
@@ -435,6 +468,14 @@ int gemm_launch(GemmArgs a, bool big, hipStream_t st) {
   }
   return e == hipSuccess ? 0 : fail("gated feed-forward block: launch failed: %s", hipGetErrorString(e));
 }
+
+// The fused products are compiled in translation units of their own (dm_block_ffn_gate.hip, dm_block_ffn_dact.hip).
+extern template int gemm_launch<bf16, false, false, EPI_GATE>(GemmArgs, bool, hipStream_t);
+extern template int gemm_launch<f16, false, false, EPI_GATE>(GemmArgs, bool, hipStream_t);
+extern template int gemm_launch<bf16, false, false, EPI_GATE_F32>(GemmArgs, bool, hipStream_t);
+extern template int gemm_launch<bf16, false, true, EPI_DACT>(GemmArgs, bool, hipStream_t);
+extern template int gemm_launch<f16, false, true, EPI_DACT>(GemmArgs, bool, hipStream_t);
+extern template int gemm_launch<bf16, false, true, EPI_DACT_F32>(GemmArgs, bool, hipStream_t);
 
 }  // namespace dmb
 #endif

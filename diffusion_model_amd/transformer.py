@@ -251,8 +251,8 @@ def _ffn_check(x, w_gate, w_up, w_down, activation):
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation="silu", save=False):
     """(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down, with weights as nn.Linear holds them: w_gate and w_up
     [hidden, width], w_down [out, hidden].  All tensors are of one type.  ``activation``: silu, gelu (erf), gelu_tanh, relu, sigmoid.
-    ``save``: (y, saved), with ``saved`` (opaque) for ``gated_ffn_backward``.  16-bit types round the projections and their product to
-    that type between the matrix products; fp32 keeps fp32 accuracy."""
+    ``save``: (y, saved), with ``saved`` (opaque) for ``gated_ffn_backward``.  16-bit types round the hidden values to that type
+    between the matrix products; fp32 keeps fp32 accuracy."""
     dt, d, f, n, w_gate, w_up, w_down = _ffn_check(x, w_gate, w_up, w_down, activation)
     b_gate, b_up, b_down = _vector(b_gate, f, x, "b_gate"), _vector(b_up, f, x, "b_up"), _vector(b_down, n, x, "b_down")
     with torch.cuda.device(x.device):
@@ -261,7 +261,7 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
         m = r.shape[0]
         y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
         saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt), dtype=torch.uint8, device=x.device) if save else None
-        ws = _workspace(x, L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt))
+        ws = _workspace(x, L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt, int(save)))
         _lib.check(L.dm_gated_ffn(
             _lib.ptr(r), stride, _lib.ptr(w_gate), _lib.ptr(w_up), _lib.ptr(w_down), _lib.ptr(b_gate), _lib.ptr(b_up), _lib.ptr(b_down),
             _lib.ptr(y), _lib.ptr(saved), m, d, f, n, _ACTIVATIONS[activation], dt, _lib.ptr(ws), ws.numel(), _stream(x)))

@@ -78,11 +78,11 @@ def test_rotary_refusals():
 
 def test_gated_ffn_refusals():
     L = _lib.lib()
-    need = L.dm_gated_ffn_workspace_bytes(100, 64, 128, 64, 1)
+    need = L.dm_gated_ffn_workspace_bytes(100, 64, 128, 64, 1, 0)
     assert need >= 100 * 128 * 2
-    assert L.dm_gated_ffn_workspace_bytes(100, 64, 128, 64, 0) >= 3 * 2 * (100 * 64 + 3 * 64 * 128 + 100 * 128)  # three planes of every operand
-    assert L.dm_gated_ffn_saved_bytes(100, 129, 1) == 2 * 100 * 136 * 2 and L.dm_gated_ffn_saved_bytes(0, 129, 1) == 0
-    assert L.dm_gated_ffn_workspace_bytes(0, 64, 128, 64, 1) == 0 and L.dm_gated_ffn_workspace_bytes(10, 0, 128, 64, 1) == 0
+    assert L.dm_gated_ffn_workspace_bytes(100, 64, 128, 64, 0, 0) >= 3 * 2 * (100 * 64 + 3 * 64 * 128 + 100 * 128)  # three planes of every operand
+    assert L.dm_gated_ffn_saved_bytes(100, 129, 1) == 3 * 100 * 136 * 2 and L.dm_gated_ffn_saved_bytes(0, 129, 1) == 0
+    assert L.dm_gated_ffn_workspace_bytes(0, 64, 128, 64, 1, 0) == 0 and L.dm_gated_ffn_workspace_bytes(10, 0, 128, 64, 1, 0) == 0
     ok = dict(x=P, xs=64, wg=P, wu=P, wd=P, y=P, saved=None, M=100, D=64, F=128, N=64, act=0, dt=1, ws=P, n=need)
 
     def call(**kw):
@@ -107,13 +107,14 @@ def test_gated_ffn_refusals():
     assert call(M=0) == 0
     need_b = L.dm_gated_ffn_backward_workspace_bytes(100, 64, 128, 64, 1)
 
-    def back(dy=P, dys=64, saved=P, n=need_b):
-        return L.dm_gated_ffn_backward(dy, dys, P, 64, P, P, P, saved, P, P, P, P, None, None, None, 100, 64, 128, 64, 0, 1, P, n, None)
+    def back(dy=P, dys=64, saved=P, n=need_b, dw=P, db=None):
+        return L.dm_gated_ffn_backward(dy, dys, P, 64, P, P, P, saved, P, dw, P, P, db, None, None, 100, 64, 128, 64, 0, 1, P, n, None)
     refused(back(dy=None), "null")
     refused(back(dy=ODD), "16")
     refused(back(dys=63), "stride")
     refused(back(saved=None), "saved")
     refused(back(n=need_b - 1), "workspace")
+    refused(back(dw=None, db=P), "weight's")
 
 
 def test_functions_need_the_gpu():
