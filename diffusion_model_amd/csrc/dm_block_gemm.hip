@@ -193,8 +193,11 @@ struct Stager {
 };
 
 // 16 bytes per lane from a bounds-checked buffer straight into LDS at `lds` + lane * 16.  The caller waits (vmcnt) and synchronises.
+// NEW: the first load from this resource (five wait states, should a vector instruction have written its scalar registers).
+template <bool NEW>
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
+  if (NEW) asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
+  else asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
 }
 __device__ __forceinline__ i32x4 buffer_of(const void* p) {
   const uint64_t u = (uint64_t)p;
@@ -265,22 +268,42 @@ gemm_kernel(const GemmArgs p) {
   // (the segments' pointers are read where the launch put the arguments: indexing the parameter itself would copy it to scratch)
   const auto* args = (const __attribute__((address_space(4))) GemmArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
-  int seg = it0 / p.iters, step = it0 - seg * p.iters;  // of the next stage to be asked for
+  // The next stage to be asked for: its segment, step, and the corners of its tiles.
+  int seg = it0 / p.iters, step = it0 - seg * p.iters;
+  const int64_t astep = AKS ? p.lda * 128 : 128, bstep = BKS ? p.ldb * 128 : 128;  // bytes from one step to the next
+  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2;
+  const char *pa, *pb, *pb2;
+  auto corner = [&]() {
+    pa = (const char*)args->a[seg] + a0 + step * astep;
+    pb = (const char*)args->b[seg] + b0 + step * bstep;
+    pb2 = GATE ? (const char*)args->b2[seg] + b0 + step * bstep : pb;
+  };
   auto issue = [&](uint32_t stage) {
-    const int k0 = step * 64, left = p.K - k0;
-    const i32x4 ra = buffer_of((const char*)args->a[seg] + (AKS ? (int64_t)k0 * p.lda + m0 : m0 * p.lda + k0) * 2);
-#pragma unroll
-    for (int j = 0; j < sa.PASSES; ++j)
-      load_to_lds(ra, sa.kpos[j] < left ? sa.off[j] : 0x80000000u, lds0 + stage + (j * NW + wave) * 1024);
-    const int64_t bo = (BKS ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0) * 2;
-    const i32x4 rb = buffer_of((const char*)args->b[seg] + bo);
+    const int left = p.K - step * 64;
+    const uint32_t to = lds0 + stage + wave * 1024;
+    const i32x4 ra = buffer_of(pa), rb = buffer_of(pb);
     i32x4 rb2 = rb;
-    if constexpr (GATE) rb2 = buffer_of((const char*)args->b2[seg] + bo);
+    if constexpr (GATE) rb2 = buffer_of(pb2);
 #pragma unroll
-    for (int j = 0; j < sb.PASSES; ++j)
-      load_to_lds(GATE && (j * NW + wave) / 4 % 2 ? rb2 : rb, sb.kpos[j] < left ? sb.off[j] : 0x80000000u,
-                  lds0 + stage + ABYTES + (j * NW + wave) * 1024);
-    if (++step == p.iters) { step = 0; ++seg; }
+    for (int j = 0; j < sa.PASSES; ++j) {
+      const uint32_t off = sa.kpos[j] < left ? sa.off[j] : 0x80000000u;
+      if (j == 0) load_to_lds<true>(ra, off, to);
+      else load_to_lds<false>(ra, off, to + j * NW * 1024);
+    }
+#pragma unroll
+    for (int j = 0; j < sb.PASSES; ++j) {
+      const uint32_t off = sb.kpos[j] < left ? sb.off[j] : 0x80000000u;
+      const i32x4 r = GATE && (j * NW + wave) / 4 % 2 ? rb2 : rb;
+      if (j == 0 || GATE) load_to_lds<true>(r, off, to + ABYTES + j * NW * 1024);
+      else load_to_lds<false>(r, off, to + ABYTES + j * NW * 1024);
+    }
+    pa += astep;
+    pb += bstep;
+    if (GATE) pb2 += bstep;
+    if (++step == p.iters) {
+      step = 0;
+      if (++seg < p.segments) corner();
+    }
   };
 
   f32x16 acc[MI][NI], asum;
@@ -295,31 +318,61 @@ gemm_kernel(const GemmArgs p) {
   const short unit = __builtin_bit_cast(short, (T)1.f);
   const s16x8 ones = {unit, unit, unit, unit, unit, unit, unit, unit};
 
-  uint32_t cur = 0;
-  int now = seg;  // the segment of the stage at hand
-  if (it0 < it1) issue(0);
-  for (int it = it0; it < it1; ++it) {
-    const bool sum = SUMS && p.sums && tn == 0 && (p.sum_segments >> now & 1);
-    now = seg;
-    stage_arrived();  // this step's tiles are in LDS, and every wave is done with the other stage
-    if (it + 1 < it1) issue(cur ^ STAGE);
-    const char DM_LDS* st = (const char DM_LDS*)smem + cur;
+  // Fragments are read a quarter step ahead of the products that take them.  The last quarter's are in registers before the barrier,
+  // so its products run while the next stage's first fragments arrive and the stage just left is filled again.
+  struct Frag { s16x8 a[MI], b[NI], x; } f[2];
+  auto read = [&](Frag& f, uint32_t stage, int s, bool sum) __attribute__((always_inline)) {
+    const char DM_LDS* st = (const char DM_LDS*)smem + stage;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      s16x8 a[MI], b[NI];
+    for (int j = 0; j < NI; ++j) f.b[j] = fragment<BN, BKS, true>(st + ABYTES, lane, wn * NI + j, s);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = fragment<BM, AKS, false>(st, lane, wm * MI + i, s);
+    for (int i = 0; i < MI; ++i) f.a[i] = fragment<BM, AKS, false>(st, lane, wm * MI + i, s);
+    if (SUMS && sum) f.x = fragment<BM, AKS, false>(st, lane, wm * MI + wn, s);
+  };
+  auto multiply = [&](const Frag& f, bool sum) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = fragment<BN, BKS, true>(st + ABYTES, lane, wn * NI + j, s);
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(f.b[j], f.a[i], acc[i][j], T());
+    if (SUMS && sum) asum = mfma16(ones, f.x, asum, T());
+  };
+  auto interleave = []() __attribute__((always_inline)) {  // a read, a product, and so on
+    constexpr int READS = (AKS ? 2 : 1) * MI + (BKS ? 2 : 1) * NI, PER = (READS + MI * NI - 1) / (MI * NI);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(b[j], a[i], acc[i][j], T());
-      if constexpr (SUMS) {
-        if (sum) asum = mfma16(ones, fragment<BM, AKS, false>(st, lane, wm * MI + wn, s), asum, T());
-      }
+    for (int i = 0; i < MI * NI; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
-    cur ^= STAGE;
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t cur = 0;
+  if (it0 < it1) {
+    corner();
+    bool sum = SUMS && p.sums && tn == 0 && (p.sum_segments >> seg & 1);  // of the stage at hand
+    issue(0);
+    stage_arrived();
+    bool next = SUMS && p.sums && tn == 0 && (p.sum_segments >> seg & 1);
+    read(f[0], 0, 0, sum);
+    if (it0 + 1 < it1) issue(STAGE);
+    for (int it = it0; it < it1; ++it) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        read(f[(s + 1) & 1], cur, s + 1, sum);
+        multiply(f[s & 1], sum);
+        interleave();
+      }
+      const bool last = sum;
+      if (it + 1 < it1) {
+        stage_arrived();  // the next stage's tiles are in LDS, and every wave is done with this one
+        sum = next;
+        next = SUMS && p.sums && tn == 0 && (p.sum_segments >> seg & 1);
+        read(f[0], cur ^ STAGE, 0, sum);
+        if (it + 2 < it1) issue(cur);
+        cur ^= STAGE;
+      }
+      multiply(f[1], last);
+    }
   }
 
   // acc[i][j][e] belongs to m = lane & 31 and n = 16 (lane >> 5) + e of the 32 x 32 block (i, j).
