@@ -49,8 +49,6 @@ pack_rows_kernel(const S* __restrict__ src, int64_t ld, D* __restrict__ dst, int
 }
 
 // ---- up to SKINNY_ROWS rows
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 template <typename T> struct Skinny;
 template <> struct Skinny<bf16> {
   static constexpr int V = 8;
@@ -293,7 +291,7 @@ int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part
   return launched("gated feed-forward block");
 }
 
-inline int iters_of(int64_t K) { return (int)((K + 63) / 64); }
+inline int iters_of(int64_t K) { return (int)((K + GEMM_BK - 1) / GEMM_BK); }
 inline int64_t pad8(int64_t v) { return round_up(v, 8); }
 
 struct FfnIn { const void *x, *wg, *wu, *wd, *bg, *bu, *bd; int64_t xs; };

@@ -5,7 +5,7 @@
 // is transposed on its way out of LDS (ds_read_tr).  The k range may be a chain of up to 12 segments, each with base pointers of its
 // own: the two terms of dx = dg Wg + du Wu, and the six products of fp32 operands that were split into three bf16 terms.
 //
-// A workgroup owns a BM x BN tile and walks k in steps of 64: two LDS stages, filled by buffer loads that write LDS directly (16 bytes
+// A workgroup owns a BM x BN tile and walks k in steps of GEMM_BK: GEMM_STAGES LDS stages, filled by buffer loads that write LDS directly (16 bytes
 // per lane, rows and columns out of range are bounds-checked to zero by the buffer resource), one barrier per step.  The LDS image
 // is swizzled in 16-byte pieces so that fragment reads touch all 64 banks once.  Fragments feed v_mfma_f32_32x32x16 with the n side as
 // the first operand, its rows permuted: a lane then holds sixteen consecutive n of one m, which the epilogue stores as whole vectors.
@@ -24,6 +24,7 @@ typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 #define DM_LDS __attribute__((address_space(3)))
@@ -132,6 +133,17 @@ __device__ __forceinline__ void load8(const S* p, float (&v)[8]) {
   }
 }
 
+#ifndef DM_BK
+#define DM_BK 64
+#define DM_ST 2
+#endif
+constexpr int GEMM_BK = DM_BK, GEMM_STAGES = DM_ST;
+__device__ __forceinline__ void from_lds(const char DM_LDS* p, float (&v)[8]) {
+  const f32x4 a = *(const DM_LDS f32x4*)p, b = *(const DM_LDS f32x4*)(p + 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
+
 constexpr int GEMM_MAX_SEGMENTS = 12;
 enum { EPI_STORE, EPI_GATE, EPI_GATE_F32, EPI_DACT, EPI_DACT_F32 };  // _F32: of split fp32 operands
 
@@ -139,7 +151,7 @@ struct GemmArgs {
   const void* a[GEMM_MAX_SEGMENTS];
   const void* b[GEMM_MAX_SEGMENTS];
   const void* b2[GEMM_MAX_SEGMENTS];  // EPI_GATE: the second projection's weights
-  int segments, iters;                // iters: k steps of 64 per segment
+  int segments, iters;                // iters: k steps of GEMM_BK per segment
   int64_t lda, ldb;                   // elements
   int64_t M;
   int N, K;                           // N: of one projection for EPI_GATE.  K: true length; a KC row is zero from there to the end of its piece
@@ -162,16 +174,19 @@ __device__ __forceinline__ int ks_swizzle(int k, int c) { return N >= 128 ? c ^ 
 // the instruction is n = permuted(r), and its piece c of a KC stage lies at c ^ key(n): sixteen lanes read sixteen pieces of all 64 banks.
 __device__ __forceinline__ int permuted(int r) { return ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3); }
 template <bool PERM>
-__device__ __forceinline__ int kc_key(int row) { return PERM ? ((row >> 1) & 3) | ((row >> 2) & 4) : (row >> 1) & 7; }
+__device__ __forceinline__ int kc_key(int row) {
+  if constexpr (GEMM_BK == 64) return PERM ? ((row >> 1) & 3) | ((row >> 2) & 4) : (row >> 1) & 7;
+  else return PERM ? ((row >> 2) & 1) | ((row >> 3) & 2) : (row >> 2) & 3;
+}
 
-// One LDS stage of one operand: R rows (of A or B) x 64 k, 16-bit elements, by the NW waves of the block.
+// One LDS stage of one operand: R rows (of A or B) x GEMM_BK k, 16-bit elements, by the NW waves of the block.
 template <int R, bool KS, int NW, bool PERM>
 struct Stager {
-  static constexpr int PASSES = R * 8 / (64 * NW);  // 16-byte pieces per lane
-  static constexpr int CPR = KS ? R / 8 : 8;        // pieces per LDS row
-  static constexpr int RPW = 64 / CPR;              // LDS rows that one wave's load fills
-  uint32_t off[PASSES];                             // byte offset from the tile's corner, 2^31 where the piece lies outside
-  int kpos[PASSES];                                 // k of the piece within the step
+  static constexpr int PASSES = R * GEMM_BK / 8 / (64 * NW);  // 16-byte pieces per lane
+  static constexpr int CPR = KS ? R / 8 : GEMM_BK / 8;        // pieces per LDS row
+  static constexpr int RPW = 64 / CPR;                        // LDS rows that one wave's load fills
+  uint32_t off[PASSES];                                       // byte offset from the tile's corner, 2^31 where the piece lies outside
+  int kpos[PASSES];                                           // k of the piece within the step
   // GATE: rows 64 i .. +31 of the tile are rows 32 i of the first projection's weights, +32 .. +63 the second's
   template <bool GATE>
   __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int64_t rows_left) {
@@ -193,19 +208,19 @@ struct Stager {
 };
 
 // 16 bytes per lane from a bounds-checked buffer straight into LDS at `lds` + lane * 16.  The caller waits (vmcnt) and synchronises.
-// NEW: the first load from this resource (five wait states, should a vector instruction have written its scalar registers).
-template <bool NEW>
+// (Five wait states, should a vector instruction have written the scalar registers.)
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off, uint32_t lds) {
-  if (NEW) asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
-  else asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
 }
 __device__ __forceinline__ i32x4 buffer_of(const void* p) {
   const uint64_t u = (uint64_t)p;
   return i32x4{(int)(uint32_t)u, (int)(uint32_t)(u >> 32) & 0xffff, (int)0x80000000u, 0x00020000};
 }
-__device__ __forceinline__ void stage_arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// All but the LEFT newest loads of every wave are in LDS, and every wave has its fragments of the stage at hand in registers.
+template <int LEFT>
+__device__ __forceinline__ void stage_arrived() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
 
-// Fragments of 32 rows x 16 k (step s of 4) out of a stage.
+// Fragments of 32 rows x 16 k (the s-th of the step) out of a stage.
 template <int R, bool KS, bool PERM>
 __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, int tile, int s) {
   if constexpr (KS) {
@@ -222,7 +237,7 @@ __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, in
     return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
   } else {
     const int r = PERM ? permuted(lane & 31) : lane & 31;
-    return *(const DM_LDS s16x8*)(stage + (tile * 32 + r) * 128 + ((2 * s + (lane >> 5)) ^ kc_key<PERM>(r)) * 16);
+    return *(const DM_LDS s16x8*)(stage + (tile * 32 + r) * (GEMM_BK * 2) + ((2 * s + (lane >> 5)) ^ kc_key<PERM>(r)) * 16);
   }
 }
 
@@ -230,12 +245,12 @@ template <typename T, int BM, int BN, int WM, int WN, bool AKS, bool BKS, int EP
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm_kernel(const GemmArgs p) {
   constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
-  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  constexpr int ABYTES = BM * GEMM_BK * 2, STAGE = (BM + BN) * GEMM_BK * 2;
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
   using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
-  static_assert(!GATE || (NI == 2 && !BKS), "a wave of the gated product owns 32 columns of each projection");
-  static_assert(!SUMS || MI == WN, "each of the waves of a tile row sums one of its 32-row blocks");
+  constexpr int XS = (MI + WN - 1) / WN;  // the waves of a tile row share its sums of A: XS blocks of 32 rows each
+  static_assert(!GATE || (NI % 2 == 0 && !BKS), "blocks of 32 columns of the two projections alternate");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -257,7 +272,7 @@ gemm_kernel(const GemmArgs p) {
   const int n0 = tn * (GATE ? BN / 2 : BN);
 
   const int total = p.segments * p.iters;
-  const int per = (total + p.splits - 1) / p.splits;
+  const int per = ((total + p.splits - 1) / p.splits + 7) / 8 * 8;  // whole eights: see `place`
   const int it0 = blockIdx.y * per, it1 = it0 + per < total ? it0 + per : total;
 
   Stager<BM, AKS, NW, false> sa;
@@ -268,48 +283,57 @@ gemm_kernel(const GemmArgs p) {
   // (the segments' pointers are read where the launch put the arguments: indexing the parameter itself would copy it to scratch)
   const auto* args = (const __attribute__((address_space(4))) GemmArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
-  // The next stage to be asked for: its segment, step, and the corners of its tiles.
-  int seg = it0 / p.iters, step = it0 - seg * p.iters;
-  const int64_t astep = AKS ? p.lda * 128 : 128, bstep = BKS ? p.ldb * 128 : 128;  // bytes from one step to the next
-  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2;
-  const char *pa, *pb, *pb2;
-  auto corner = [&]() {
-    pa = (const char*)args->a[seg] + a0 + step * astep;
-    pb = (const char*)args->b[seg] + b0 + step * bstep;
-    pb2 = GATE ? (const char*)args->b2[seg] + b0 + step * bstep : pb;
+  // Steps are taken in an order of the tile's own within each eight (where the range has all eight): the blocks of an XCD would
+  // otherwise ask for the same columns of all rows at once, which lie on few of the L2's channels when rows are a power of two apart.
+#ifndef DM_SHIFT
+#define DM_SHIFT ((tm + 2 * tn) & 7)
+#endif
+  const int shift = DM_SHIFT;
+  const uint32_t magic = (uint32_t)((1ull << 32) / (uint32_t)p.iters - (p.iters == 1));
+  auto place = [&](int it, int& seg, int& step) {  // segment, and step within it, of the range's it-th step
+    const int at = (it | 7) < it1 ? it ^ shift : it;
+    seg = (int)(((uint64_t)(uint32_t)at * magic) >> 32);
+    if (at - seg * p.iters >= p.iters) ++seg;
+    step = at - seg * p.iters;
   };
-  auto issue = [&](uint32_t stage) {
-    const int left = p.K - step * 64;
-    const uint32_t to = lds0 + stage + wave * 1024;
-    const i32x4 ra = buffer_of(pa), rb = buffer_of(pb);
-    i32x4 rb2 = rb;
-    if constexpr (GATE) rb2 = buffer_of(pb2);
-#pragma unroll
-    for (int j = 0; j < sa.PASSES; ++j) {
-      const uint32_t off = sa.kpos[j] < left ? sa.off[j] : 0x80000000u;
-      if (j == 0) load_to_lds<true>(ra, off, to);
-      else load_to_lds<false>(ra, off, to + j * NW * 1024);
+  const int64_t astep = (AKS ? p.lda : 1) * GEMM_BK * 2, bstep = (BKS ? p.ldb : 1) * GEMM_BK * 2;  // bytes from one step to the next
+  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2;
+  const char *sega = nullptr, *segb = nullptr, *segb2 = nullptr;  // the corners of the segment last asked for
+  int have = -1;
+  constexpr int LOADS = sa.PASSES + sb.PASSES;
+  struct Request { i32x4 a, b, b2; int left; uint32_t to; };
+  auto request = [&](int it, uint32_t stage) {  // what the loads of a stage have in common; behind the range every piece lies outside
+    int seg, step;
+    place(it < it1 ? it : it1 - 1, seg, step);
+    if (seg != have) {
+      have = seg;
+      sega = (const char*)args->a[seg] + a0;
+      segb = (const char*)args->b[seg] + b0;
+      if (GATE) segb2 = (const char*)args->b2[seg] + b0;
     }
-#pragma unroll
-    for (int j = 0; j < sb.PASSES; ++j) {
-      const uint32_t off = sb.kpos[j] < left ? sb.off[j] : 0x80000000u;
-      const i32x4 r = GATE && (j * NW + wave) / 4 % 2 ? rb2 : rb;
-      if (j == 0 || GATE) load_to_lds<true>(r, off, to + ABYTES + j * NW * 1024);
-      else load_to_lds<false>(r, off, to + ABYTES + j * NW * 1024);
-    }
-    pa += astep;
-    pb += bstep;
-    if (GATE) pb2 += bstep;
-    if (++step == p.iters) {
-      step = 0;
-      if (++seg < p.segments) corner();
+    Request r;
+    r.a = buffer_of(sega + step * astep);
+    r.b = buffer_of(segb + step * bstep);
+    r.b2 = GATE ? buffer_of(segb2 + step * bstep) : r.b;
+    r.left = it < it1 ? p.K - step * GEMM_BK : 0;
+    r.to = lds0 + stage + wave * 1024;
+    return r;
+  };
+  auto load = [&](const Request& r, int l) __attribute__((always_inline)) {  // the l-th of a wave's LOADS loads of a stage
+    if (l < sa.PASSES) {
+      load_to_lds(r.a, sa.kpos[l] < r.left ? sa.off[l] : 0x80000000u, r.to + l * NW * 1024);
+    } else {
+      const int j = l - sa.PASSES;
+      load_to_lds(GATE && (j * NW + wave) * sb.RPW / 32 % 2 ? r.b2 : r.b, sb.kpos[j] < r.left ? sb.off[j] : 0x80000000u,
+                  r.to + ABYTES + j * NW * 1024);
     }
   };
 
-  f32x16 acc[MI][NI], asum;
+  f32x16 acc[MI][NI], asum[XS];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    asum[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < XS; ++x) asum[x][e] = 0.f;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -318,23 +342,27 @@ gemm_kernel(const GemmArgs p) {
   const short unit = __builtin_bit_cast(short, (T)1.f);
   const s16x8 ones = {unit, unit, unit, unit, unit, unit, unit, unit};
 
-  // Fragments are read a quarter step ahead of the products that take them.  The last quarter's are in registers before the barrier,
-  // so its products run while the next stage's first fragments arrive and the stage just left is filled again.
-  struct Frag { s16x8 a[MI], b[NI], x; } f[2];
+  // Fragments are read 16 k ahead of the products that take them.  The last ones of a step are in registers before the barrier, so their
+  // products run while the next stage's first fragments arrive and the stage just left is filled again.
+  struct Frag { s16x8 a[MI], b[NI], x[XS]; } f[2];
   auto read = [&](Frag& f, uint32_t stage, int s, bool sum) __attribute__((always_inline)) {
     const char DM_LDS* st = (const char DM_LDS*)smem + stage;
 #pragma unroll
     for (int j = 0; j < NI; ++j) f.b[j] = fragment<BN, BKS, true>(st + ABYTES, lane, wn * NI + j, s);
 #pragma unroll
     for (int i = 0; i < MI; ++i) f.a[i] = fragment<BM, AKS, false>(st, lane, wm * MI + i, s);
-    if (SUMS && sum) f.x = fragment<BM, AKS, false>(st, lane, wm * MI + wn, s);
+    if (SUMS && sum)
+#pragma unroll
+      for (int x = 0; x < XS; ++x) f.x[x] = fragment<BM, AKS, false>(st, lane, wm * MI + wn * XS + x, s);
   };
-  auto multiply = [&](const Frag& f, bool sum) __attribute__((always_inline)) {
+  auto multiply_row = [&](const Frag& f, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(f.b[j], f.a[i], acc[i][j], T());
+  };
+  auto multiply_sums = [&](const Frag& f, bool sum) __attribute__((always_inline)) {
+    if (SUMS && sum)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(f.b[j], f.a[i], acc[i][j], T());
-    if (SUMS && sum) asum = mfma16(ones, f.x, asum, T());
+      for (int x = 0; x < XS; ++x) asum[x] = mfma16(ones, f.x[x], asum[x], T());
   };
   auto interleave = []() __attribute__((always_inline)) {  // a read, a product, and so on
     constexpr int READS = (AKS ? 2 : 1) * MI + (BKS ? 2 : 1) * NI, PER = (READS + MI * NI - 1) / (MI * NI);
@@ -345,103 +373,129 @@ gemm_kernel(const GemmArgs p) {
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  uint32_t cur = 0;
+  constexpr int PARTS = GEMM_BK / 16;
+  const bool sums = SUMS && p.sums && tn == 0;
+  auto summed = [&](int it) {  // does the range's it-th step count for the sums of A
+    int seg, step;
+    if (!sums) return false;
+    place(it, seg, step);
+    return (p.sum_segments >> seg & 1) != 0;
+  };
   if (it0 < it1) {
-    corner();
-    bool sum = SUMS && p.sums && tn == 0 && (p.sum_segments >> seg & 1);  // of the stage at hand
-    issue(0);
-    stage_arrived();
-    bool next = SUMS && p.sums && tn == 0 && (p.sum_segments >> seg & 1);
+    uint32_t cur = 0;
+#pragma unroll
+    for (int k = 0; k < GEMM_STAGES; ++k) {
+      const Request r = request(it0 + k, k * STAGE);
+#pragma unroll
+      for (int l = 0; l < LOADS; ++l) load(r, l);
+    }
+    stage_arrived<LOADS * (GEMM_STAGES - 1)>();
+    bool sum = summed(it0);
     read(f[0], 0, 0, sum);
-    if (it0 + 1 < it1) issue(STAGE);
     for (int it = it0; it < it1; ++it) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 3; ++s) {
+      for (int s = 0; s < PARTS - 1; ++s) {
         read(f[(s + 1) & 1], cur, s + 1, sum);
-        multiply(f[s & 1], sum);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) multiply_row(f[s & 1], i);
+        multiply_sums(f[s & 1], sum);
         interleave();
       }
       const bool last = sum;
-      if (it + 1 < it1) {
-        stage_arrived();  // the next stage's tiles are in LDS, and every wave is done with this one
-        sum = next;
-        next = SUMS && p.sums && tn == 0 && (p.sum_segments >> seg & 1);
-        read(f[0], cur ^ STAGE, 0, sum);
-        if (it + 2 < it1) issue(cur);
-        cur ^= STAGE;
+      const uint32_t left = cur;
+      cur = cur + STAGE == GEMM_STAGES * STAGE ? 0 : cur + STAGE;
+      sum = it + 1 < it1 && summed(it + 1);
+      stage_arrived<LOADS * (GEMM_STAGES - 2)>();
+      read(f[0], cur, 0, sum);  // (behind the range: zeros, and nobody's)
+      const Request r = request(it + GEMM_STAGES, left);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {  // loads among the products: a burst of them would hold up the wave
+        __builtin_amdgcn_sched_barrier(0);
+        multiply_row(f[(PARTS - 1) & 1], i);
+#pragma unroll
+        for (int l = i * LOADS / MI; l < (i + 1) * LOADS / MI; ++l) load(r, l);
       }
-      multiply(f[1], last);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply_sums(f[(PARTS - 1) & 1], last);
     }
   }
+  stage_arrived<0>();  // the loads behind the range are done with LDS, and so is every wave
 
-  // acc[i][j][e] belongs to m = lane & 31 and n = 16 (lane >> 5) + e of the 32 x 32 block (i, j).
+  // acc[i][j][e] belongs to m = lane & 31 and n = 16 (lane >> 5) + e of the 32 x 32 block (i, j).  The i-th blocks of all waves meet in LDS
+  // as rows of fp32 (a pitch of 16 bytes more than the row: no bank conflicts), two buffers in turn, and leave as whole pieces of
+  // eight columns, neighbouring lanes next to each other: written straight from the accumulators, rows a power of two apart crowd
+  // on few of the L2's channels (41 us of a 256 x 256 tile's time, measured at a row of 8 KB).
+  constexpr int ROWS = WM * 32, PITCH = BN * 4 + 16, COLS = GATE ? BN / 2 : BN, PIECES = COLS / 8, TASKS = ROWS * PIECES / (NW * 64);
   const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces (with zeros: rows of B out of range are zero)
-  const int half = (lane >> 5) * 16;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int64_t m = m0 + (wm * MI + i) * 32 + (lane & 31);
-    if (m >= p.M) continue;
-    if constexpr (GATE) {
+    char DM_LDS* buf = (char DM_LDS*)smem + (i & 1) * ROWS * PITCH;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int n = n0 + wn * 32 + half + q * 8;
-        if (n >= np) continue;
-        float g[8], u[8], h[8];
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& c = acc[i][j];
+        *(DM_LDS f32x4*)(buf + (wm * 32 + (lane & 31)) * PITCH + ((wn * NI + j) * 32 + (lane >> 5) * 16 + q * 4) * 4) =
+            f32x4{c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
+      }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TASKS; ++t) {
+      const int id = t * NW * 64 + threadIdx.x, row = id / PIECES, col = id % PIECES * 8;
+      const int64_t m = m0 + (row / 32 * MI + i) * 32 + row % 32;
+      const int n = n0 + col;
+      if (m >= p.M || n >= (EPI == EPI_STORE ? p.N : np)) continue;
+      const char DM_LDS* at = buf + row * PITCH + (GATE ? col / 32 * 64 + col % 32 : col) * 4;
+      float v[8];
+      from_lds(at, v);
+      if constexpr (GATE) {
+        float u[8], h[8];
+        from_lds(at + 128, u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          g[e] = acc[i][0][q * 8 + e] + bias_at<Kept>(p.bias, n + e, p.N);
-          u[e] = acc[i][NI - 1][q * 8 + e] + bias_at<Kept>(p.bias2, n + e, p.N);
+          v[e] += bias_at<Kept>(p.bias, n + e, p.N);
+          u[e] += bias_at<Kept>(p.bias2, n + e, p.N);
         }
         with_activation(p.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float value, slope;
-            activation<decltype(act)::value, !F32>(g[e], value, slope);
+            activation<decltype(act)::value, !F32>(v[e], value, slope);
             h[e] = value * u[e];
             u[e] *= slope;
-            g[e] = value;
+            v[e] = value;
           }
         });
         store8<T, BETWEEN>(p.out, m, n, np, h);
-        if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, g); }
+        if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
+      } else if constexpr (EPI == EPI_STORE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
+        Out o = p.out;
+        if (p.splits > 1) o.p = (float*)o.p + blockIdx.y * p.split_stride;
+        if (o.f32) store8<T, OUT_F32>(o, m, n, p.N, v);
+        else store8<T, OUT_16>(o, m, n, p.N, v);
+      } else {
+        float ug[8], ag[8];
+        load8((const Kept*)p.ug + m * p.ldg + n, ug);
+        load8((const Kept*)p.ag + m * p.ldg + n, ag);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { ug[e] *= v[e]; ag[e] *= v[e]; }
+        store8<T, BETWEEN>(p.out, m, n, np, ug);
+        store8<T, BETWEEN>(p.out2, m, n, np, ag);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int n = n0 + (wn * NI + j) * 32 + half + q * 8;
-          float v[8];
-          if constexpr (EPI == EPI_STORE) {
-            if (n >= p.N) continue;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v[e] = acc[i][j][q * 8 + e] + (p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N));
-            Out o = p.out;
-            if (p.splits > 1) o.p = (float*)o.p + blockIdx.y * p.split_stride;
-            if (o.f32) store8<T, OUT_F32>(o, m, n, p.N, v);
-            else store8<T, OUT_16>(o, m, n, p.N, v);
-          } else {
-            if (n >= np) continue;
-            float ug[8], ag[8];
-            load8((const Kept*)p.ug + m * p.ldg + n, ug);
-            load8((const Kept*)p.ag + m * p.ldg + n, ag);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { v[e] = acc[i][j][q * 8 + e] * ug[e]; ag[e] *= acc[i][j][q * 8 + e]; }
-            store8<T, BETWEEN>(p.out, m, n, np, v);
-            store8<T, BETWEEN>(p.out2, m, n, np, ag);
-          }
-        }
     }
   }
   if constexpr (EPI == EPI_STORE) {
     if constexpr (SUMS) {  // every n of the product with ones holds the sum
-      const int64_t m = m0 + (wm * MI + wn) * 32 + lane;
-      if (p.sums && tn == 0 && lane < 32 && m < p.M) {
-        if (p.splits > 1) ((float*)p.sums)[blockIdx.y * p.M + m] = asum[0];
-        else if (p.sums_f32) ((float*)p.sums)[m] = asum[0];
-        else ((T*)p.sums)[m] = (T)asum[0];
+#pragma unroll
+      for (int x = 0; x < XS; ++x) {
+        const int64_t m = m0 + (wm * MI + wn * XS + x) * 32 + lane;
+        if (!p.sums || tn || lane >= 32 || m >= p.M) continue;
+        if (p.splits > 1) ((float*)p.sums)[blockIdx.y * p.M + m] = asum[x][0];
+        else if (p.sums_f32) ((float*)p.sums)[m] = asum[x][0];
+        else ((T*)p.sums)[m] = (T)asum[x][0];
       }
     }
   }
@@ -512,7 +566,7 @@ int gemm_launch(GemmArgs a, bool big, hipStream_t st) {
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > (1 << 22)) return fail("gated feed-forward block: %lld output tiles in one product", (long long)tiles);
   const dim3 grid((unsigned)tiles, a.splits);
-  const int bytes = 2 * 2 * bm * 128;
+  const int stages = GEMM_STAGES * 2 * bm * GEMM_BK * 2, rows = 2 * 64 * (bm * 4 + 16), bytes = stages > rows ? stages : rows;
   const void* f = big ? (const void*)gemm_kernel<T, 256, 256, 2, 4, AKS, BKS, EPI> : (const void*)gemm_kernel<T, 128, 128, 2, 2, AKS, BKS, EPI>;
   hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == hipSuccess) {
