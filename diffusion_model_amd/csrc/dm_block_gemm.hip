@@ -7,8 +7,8 @@
 //
 // A workgroup owns a BM x BN tile and walks k in steps of GEMM_BK: GEMM_STAGES LDS stages, filled by buffer loads that write LDS directly (16 bytes
 // per lane, rows and columns out of range are bounds-checked to zero by the buffer resource), one barrier per step.  The LDS image
-// is swizzled in 16-byte pieces so that fragment reads touch all 64 banks once.  Fragments feed v_mfma_f32_32x32x16 with the n side as
-// the first operand, its rows permuted: a lane then holds sixteen consecutive n of one m, which the epilogue stores as whole vectors.
+// is swizzled in 16-byte pieces so that fragment reads touch all 64 banks once.  Fragments feed v_mfma_f32_16x16x32 with the n side as
+// the first operand: a lane then holds four consecutive n of one m.
 // A bias' gradient, the sum of A over k, is one more product with ones from the same fragments.
 #ifndef DM_BLOCK_GEMM_HIP
 #define DM_BLOCK_GEMM_HIP
@@ -18,7 +18,6 @@
 
 namespace dmb {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -29,11 +28,11 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 #define DM_LDS __attribute__((address_space(3)))
 
-__device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c, bf16) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c, f16) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c, f16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 // Three bf16 terms of an fp32 value, each the rest rounded to nearest: together they hold all 24 bits.  A value that would round to
@@ -133,17 +132,14 @@ __device__ __forceinline__ void load8(const S* p, float (&v)[8]) {
   }
 }
 
-#ifndef DM_BK
-#define DM_BK 64
-#define DM_ST 2
-#endif
-constexpr int GEMM_BK = DM_BK, GEMM_STAGES = DM_ST;
+constexpr int GEMM_BK = 64, GEMM_STAGES = 2;
 __device__ __forceinline__ void from_lds(const char DM_LDS* p, float (&v)[8]) {
   const f32x4 a = *(const DM_LDS f32x4*)p, b = *(const DM_LDS f32x4*)(p + 16);
 #pragma unroll
   for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
 }
 
+constexpr int LDS_BIAS = 3072;  // see load_to_lds
 constexpr int GEMM_MAX_SEGMENTS = 12;
 enum { EPI_STORE, EPI_GATE, EPI_GATE_F32, EPI_DACT, EPI_DACT_F32 };  // _F32: of split fp32 operands
 
@@ -167,90 +163,86 @@ struct GemmArgs {
   int sum_segments, sums_f32;         // of the type that sums_f32 gives; several: fp32, M apart
 };
 
-template <int N>  // piece of 16 bytes that holds piece `c` of row k of a KS tile with N columns
-__device__ __forceinline__ int ks_swizzle(int k, int c) { return N >= 128 ? c ^ ((k & 3) << 2) : c ^ (((k >> 1) & 1) << 2); }
-
-// The n side of a 32 x 32 product is permuted in blocks of four rows, so that a lane's sixteen results are sixteen consecutive n: row r of
-// the instruction is n = permuted(r), and its piece c of a KC stage lies at c ^ key(n): sixteen lanes read sixteen pieces of all 64 banks.
-__device__ __forceinline__ int permuted(int r) { return ((r >> 2) & 1) * 16 + (r >> 3) * 4 + (r & 3); }
-template <bool PERM>
-__device__ __forceinline__ int kc_key(int row) {
-  if constexpr (GEMM_BK == 64) return PERM ? ((row >> 1) & 3) | ((row >> 2) & 4) : (row >> 1) & 7;
-  else return PERM ? ((row >> 2) & 1) | ((row >> 3) & 2) : (row >> 2) & 3;
-}
+// Where a stage keeps a piece of 16 bytes.  KS (one LDS row per k, R columns): piece c of row k lies at c ^ ks_key(k), so that the 32
+// lanes of two fragment reads (k .. k + 3 and k + 8 .. k + 11, two pieces each) find 16 pieces of all 64 banks.  KC (one LDS row per
+// operand row, 8 pieces): piece c of a row lies at c ^ kc_key(row), so that 16 rows' pieces do.
+__device__ __forceinline__ int ks_key(int k) { return ((k & 3) | ((k >> 1) & 4)) << 1; }
+__device__ __forceinline__ int kc_key(int row) { return (row >> 1) & 7; }
 
 // One LDS stage of one operand: R rows (of A or B) x GEMM_BK k, 16-bit elements, by the NW waves of the block.
-template <int R, bool KS, int NW, bool PERM>
+template <int R, bool KS, int NW>
 struct Stager {
   static constexpr int PASSES = R * GEMM_BK / 8 / (64 * NW);  // 16-byte pieces per lane
   static constexpr int CPR = KS ? R / 8 : GEMM_BK / 8;        // pieces per LDS row
   static constexpr int RPW = 64 / CPR;                        // LDS rows that one wave's load fills
   uint32_t off[PASSES];                                       // byte offset from the tile's corner, 2^31 where the piece lies outside
-  int kpos[PASSES];                                           // k of the piece within the step
+  static __device__ __forceinline__ int row_of(int wave, int lane, int j) { return (wave * PASSES + j) * RPW + lane / CPR; }
+  static __device__ __forceinline__ int piece_of(int lane, int row) { return (lane % CPR) ^ (KS ? ks_key(row) : kc_key(row)); }
+  static __device__ __forceinline__ int k_of(int wave, int lane, int j) {  // k of the piece within the step
+    const int row = row_of(wave, lane, j);
+    return KS ? row : piece_of(lane, row) * 8;
+  }
   // GATE: rows 64 i .. +31 of the tile are rows 32 i of the first projection's weights, +32 .. +63 the second's
   template <bool GATE>
   __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int64_t rows_left) {
 #pragma unroll
     for (int j = 0; j < PASSES; ++j) {
-      const int row = (j * NW + wave) * RPW + lane / CPR, slot = lane % CPR;
-      if constexpr (KS) {
-        const int c = ks_swizzle<R>(row, slot);
-        off[j] = c * 8 < rows_left ? (uint32_t)(row * ld * 2 + c * 16) : 0x80000000u;
-        kpos[j] = row;
-      } else {
-        const int c = slot ^ kc_key<PERM>(row);
-        const int r = GATE ? row / 64 * 32 + row % 32 : row;
-        off[j] = r < rows_left ? (uint32_t)(r * ld * 2 + c * 16) : 0x80000000u;
-        kpos[j] = c * 8;
-      }
+      const int row = row_of(wave, lane, j), c = piece_of(lane, row);
+      const uint32_t bias = LDS_BIAS - j % 4 * 1024;  // see load_to_lds
+      const int r = GATE ? row / 64 * 32 + row % 32 : row;
+      off[j] = (KS ? c * 8 : r) < rows_left ? (uint32_t)(r * ld * 2 + c * 16) + bias : 0x80000000u;
     }
   }
 };
 
-// 16 bytes per lane from a bounds-checked buffer straight into LDS at `lds` + lane * 16.  The caller waits (vmcnt) and synchronises.
-// (Five wait states, should a vector instruction have written the scalar registers.)
-__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory");
+// Two loads of 16 bytes per lane from a bounds-checked buffer straight into LDS, at `lds` + FIRST + lane * 16 and 1024 bytes further on.
+// The instruction's offset (FIRST, FIRST + 1024) counts on both sides: the buffer starts LDS_BIAS bytes before its memory, and `off`
+// makes up for the difference.  The caller waits (vmcnt) and synchronises.  (s_nop: five wait states, should a vector instruction
+// have written the scalar registers.)
+template <int FIRST>
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off0, uint32_t off1, uint32_t lds) {
+  static_assert(FIRST + 1024 <= LDS_BIAS && LDS_BIAS < 4096, "offsets of the instruction");
+  asm volatile(
+      "s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %2, 0 offen offset:%4 lds\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:%5 lds" ::"v"(off0),
+      "v"(off1), "s"(rsrc), "s"(lds), "n"(FIRST), "n"(FIRST + 1024)
+      : "memory");
 }
 __device__ __forceinline__ i32x4 buffer_of(const void* p) {
-  const uint64_t u = (uint64_t)p;
-  return i32x4{(int)(uint32_t)u, (int)(uint32_t)(u >> 32) & 0xffff, (int)0x80000000u, 0x00020000};
+  const uint64_t u = (uint64_t)p - LDS_BIAS;
+  return i32x4{(int)(uint32_t)u, (int)(uint32_t)(u >> 32), (int)0x80000000u, 0x00020000};  // (addresses have 48 bits: no stride)
 }
 // All but the LEFT newest loads of every wave are in LDS, and every wave has its fragments of the stage at hand in registers.
 template <int LEFT>
 __device__ __forceinline__ void stage_arrived() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
 
-// Fragments of 32 rows x 16 k (the s-th of the step) out of a stage.
-template <int R, bool KS, bool PERM>
+// Fragment of 16 rows x 32 k (the s-th of the step) out of a stage: lane l holds row l & 15, k 8 (l >> 4) .. +7.
+template <int R, bool KS>
 __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, int tile, int s) {
   if constexpr (KS) {
     // A lane asks for 4 consecutive rows of one k; of 16 lanes' answers, lane i receives row i of four k.
-    const int g = lane >> 4, j = (lane >> 2) & 3;
-    const int blk = (g & 1) * 4 + (lane & 3), four = PERM ? (blk & 1) * 4 + (blk >> 1) : blk;
-    const int piece = tile * 4 + (four >> 1);
+    const int k0 = s * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3), piece = tile * 2 + ((lane >> 1) & 1);
     s16x4 h[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int k = s * 16 + (g >> 1) * 8 + q * 4 + j;
-      h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DM_LDS s16x4*)(stage + k * (R * 2) + ks_swizzle<R>(k, piece) * 16 + (four & 1) * 8));
+      const int k = k0 + q * 4;
+      h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DM_LDS s16x4*)(stage + k * (R * 2) + (piece ^ ks_key(k)) * 16 + (lane & 1) * 8));
     }
     return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
   } else {
-    const int r = PERM ? permuted(lane & 31) : lane & 31;
-    return *(const DM_LDS s16x8*)(stage + (tile * 32 + r) * (GEMM_BK * 2) + ((2 * s + (lane >> 5)) ^ kc_key<PERM>(r)) * 16);
+    const int row = tile * 16 + (lane & 15);
+    return *(const DM_LDS s16x8*)(stage + row * (GEMM_BK * 2) + ((s * 4 + (lane >> 4)) ^ kc_key(lane & 15)) * 16);
   }
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool AKS, bool BKS, int EPI>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm_kernel(const GemmArgs p) {
-  constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
+  constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
   constexpr int ABYTES = BM * GEMM_BK * 2, STAGE = (BM + BN) * GEMM_BK * 2;
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
   using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
-  constexpr int XS = (MI + WN - 1) / WN;  // the waves of a tile row share its sums of A: XS blocks of 32 rows each
-  static_assert(!GATE || (NI % 2 == 0 && !BKS), "blocks of 32 columns of the two projections alternate");
+  constexpr int XS = MI / WN;  // the waves of a tile row share its sums of A: XS blocks of 16 rows each
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -275,63 +267,65 @@ gemm_kernel(const GemmArgs p) {
   const int per = ((total + p.splits - 1) / p.splits + 7) / 8 * 8;  // whole eights: see `place`
   const int it0 = blockIdx.y * per, it1 = it0 + per < total ? it0 + per : total;
 
-  Stager<BM, AKS, NW, false> sa;
-  Stager<BN, BKS, NW, true> sb;
+  Stager<BM, AKS, NW> sa;
+  Stager<BN, BKS, NW> sb;
   sa.template init<false>(wave, lane, p.lda, p.M - m0);
   sb.template init<GATE>(wave, lane, p.ldb, p.N - n0);
 
   // (the segments' pointers are read where the launch put the arguments: indexing the parameter itself would copy it to scratch)
   const auto* args = (const __attribute__((address_space(4))) GemmArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
-  // Steps are taken in an order of the tile's own within each eight (where the range has all eight): the blocks of an XCD would
-  // otherwise ask for the same columns of all rows at once, which lie on few of the L2's channels when rows are a power of two apart.
-#ifndef DM_SHIFT
-#define DM_SHIFT ((tm + 2 * tn) & 7)
-#endif
-  const int shift = DM_SHIFT;
-  const uint32_t magic = (uint32_t)((1ull << 32) / (uint32_t)p.iters - (p.iters == 1));
-  auto place = [&](int it, int& seg, int& step) {  // segment, and step within it, of the range's it-th step
-    const int at = (it | 7) < it1 ? it ^ shift : it;
-    seg = (int)(((uint64_t)(uint32_t)at * magic) >> 32);
-    if (at - seg * p.iters >= p.iters) ++seg;
-    step = at - seg * p.iters;
-  };
+  // Steps are taken in an order of the tile's own within each eight of a segment: the blocks of an XCD would otherwise ask for the same
+  // columns of all rows at once, which lie on few of the L2's channels when rows are a power of two apart.  An eight that the block's
+  // range or the segment does not hold whole keeps its order (several segments of no whole eights: all of them).
+  const int shift = p.segments > 1 && p.iters % 8 ? 0 : (tm + 2 * tn) & 7;
+  int seg = it0 / p.iters, step = it0 - seg * p.iters;  // of the next stage to be asked for
+  const int whole = p.segments > 1 ? p.iters : it1;     // the end of the segment's steps in this range
   const int64_t astep = (AKS ? p.lda : 1) * GEMM_BK * 2, bstep = (BKS ? p.ldb : 1) * GEMM_BK * 2;  // bytes from one step to the next
   const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2;
-  const char *sega = nullptr, *segb = nullptr, *segb2 = nullptr;  // the corners of the segment last asked for
-  int have = -1;
+  const char *sega = (const char*)args->a[seg] + a0, *segb = (const char*)args->b[seg] + b0;  // the corners of the segment at hand
+  const char* segb2 = GATE ? (const char*)args->b2[seg] + b0 : nullptr;
   constexpr int LOADS = sa.PASSES + sb.PASSES;
-  struct Request { i32x4 a, b, b2; int left; uint32_t to; };
-  auto request = [&](int it, uint32_t stage) {  // what the loads of a stage have in common; behind the range every piece lies outside
-    int seg, step;
-    place(it < it1 ? it : it1 - 1, seg, step);
-    if (seg != have) {
-      have = seg;
+  struct Request { i32x4 a, b, b2; int left; bool sum; };
+  auto request = [&](int it) __attribute__((always_inline)) {  // what the loads of the range's it-th step have in common
+    const int at = (step | 7) < whole ? step ^ shift : step;
+    Request r;
+    r.a = buffer_of(sega + at * astep);
+    r.b = buffer_of(segb + at * bstep);
+    r.b2 = GATE ? buffer_of(segb2 + at * bstep) : r.b;
+    r.left = it < it1 ? p.K - at * GEMM_BK : 0;  // behind the range every piece lies outside
+    r.sum = SUMS && it < it1 && (p.sum_segments >> seg & 1);
+    if (++step == p.iters && seg + 1 < p.segments) {
+      step = 0;
+      ++seg;
       sega = (const char*)args->a[seg] + a0;
       segb = (const char*)args->b[seg] + b0;
       if (GATE) segb2 = (const char*)args->b2[seg] + b0;
     }
-    Request r;
-    r.a = buffer_of(sega + step * astep);
-    r.b = buffer_of(segb + step * bstep);
-    r.b2 = GATE ? buffer_of(segb2 + step * bstep) : r.b;
-    r.left = it < it1 ? p.K - step * GEMM_BK : 0;
-    r.to = lds0 + stage + wave * 1024;
     return r;
   };
-  auto load = [&](const Request& r, int l) __attribute__((always_inline)) {  // the l-th of a wave's LOADS loads of a stage
-    if (l < sa.PASSES) {
-      load_to_lds(r.a, sa.kpos[l] < r.left ? sa.off[l] : 0x80000000u, r.to + l * NW * 1024);
-    } else {
-      const int j = l - sa.PASSES;
-      load_to_lds(GATE && (j * NW + wave) * sb.RPW / 32 % 2 ? r.b2 : r.b, sb.kpos[j] < r.left ? sb.off[j] : 0x80000000u,
-                  r.to + ABYTES + j * NW * 1024);
+  // Pairs [first, last) of a wave's loads of a stage.  A wave fills a contiguous part of each operand's tile.
+  auto load = [&](const Request& r, uint32_t stage, int first, int last) __attribute__((always_inline)) {
+#pragma unroll
+    for (int l = first * 2; l < last * 2; l += 2) {
+      const bool A = l < sa.PASSES;
+      const int j = A ? l : l - sa.PASSES;
+      uint32_t o0 = A ? sa.off[j] : sb.off[j], o1 = A ? sa.off[j + 1] : sb.off[j + 1];
+      if (r.left < GEMM_BK) {  // the last step of a k range of no whole steps
+        if ((A ? sa.k_of(wave, lane, j) : sb.k_of(wave, lane, j)) >= r.left) o0 = 0x80000000u;
+        if ((A ? sa.k_of(wave, lane, j + 1) : sb.k_of(wave, lane, j + 1)) >= r.left) o1 = 0x80000000u;
+      }
+      const i32x4 rs = A ? r.a : GATE && (wave * sb.PASSES + j) * sb.RPW / 32 % 2 ? r.b2 : r.b;
+      const uint32_t to = lds0 + stage + (A ? wave * sa.PASSES * 1024 : ABYTES + wave * sb.PASSES * 1024) + j / 4 * 4096;
+      if (j % 4 == 0) load_to_lds<0>(rs, o0, o1, to);
+      else load_to_lds<2048>(rs, o0, o1, to);
     }
   };
+  static_assert(sa.PASSES % 2 == 0 && sb.PASSES % 2 == 0, "loads go in pairs");
 
-  f32x16 acc[MI][NI], asum[XS];
+  f32x4 acc[MI][NI], asum[XS];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
+  for (int e = 0; e < 4; ++e) {
 #pragma unroll
     for (int x = 0; x < XS; ++x) asum[x][e] = 0.f;
 #pragma unroll
@@ -342,108 +336,88 @@ gemm_kernel(const GemmArgs p) {
   const short unit = __builtin_bit_cast(short, (T)1.f);
   const s16x8 ones = {unit, unit, unit, unit, unit, unit, unit, unit};
 
-  // Fragments are read 16 k ahead of the products that take them.  The last ones of a step are in registers before the barrier, so their
-  // products run while the next stage's first fragments arrive and the stage just left is filled again.
-  struct Frag { s16x8 a[MI], b[NI], x[XS]; } f[2];
-  auto read = [&](Frag& f, uint32_t stage, int s, bool sum) __attribute__((always_inline)) {
-    const char DM_LDS* st = (const char DM_LDS*)smem + stage;
-#pragma unroll
-    for (int j = 0; j < NI; ++j) f.b[j] = fragment<BN, BKS, true>(st + ABYTES, lane, wn * NI + j, s);
-#pragma unroll
-    for (int i = 0; i < MI; ++i) f.a[i] = fragment<BM, AKS, false>(st, lane, wm * MI + i, s);
-    if (SUMS && sum)
-#pragma unroll
-      for (int x = 0; x < XS; ++x) f.x[x] = fragment<BM, AKS, false>(st, lane, wm * MI + wn * XS + x, s);
+  // A step is PARTS parts of 32 k.  While a part's products run, the fragments of the part after are read into a second set, the first
+  // ones needed first and the last ones early enough to be there.  Before a step's last part every wave's fragments of the stage are in
+  // registers: behind the barrier there, the next stage is read and the one just left is asked for again, between the products.
+  constexpr int PARTS = GEMM_BK / 32, READS = MI + NI, PER = (READS + MI - 3) / (MI - 2);
+  s16x8 fa[2][MI], fb[2][NI];
+  auto read = [&](int q, uint32_t from, int s, int l) __attribute__((always_inline)) {  // the l-th fragment: B's, and A's in order
+    const char DM_LDS* st = (const char DM_LDS*)smem + from;
+    if (l == 0) fa[q][0] = fragment<BM, AKS>(st, lane, wm * MI, s);
+    else if (l <= NI) fb[q][l - 1] = fragment<BN, BKS>(st + ABYTES, lane, wn * NI + l - 1, s);
+    else fa[q][l - NI] = fragment<BM, AKS>(st, lane, wm * MI + l - NI, s);
   };
-  auto multiply_row = [&](const Frag& f, int i) __attribute__((always_inline)) {
+  auto part = [&](int q, uint32_t from, int s, bool refill, const Request& r, uint32_t to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(f.b[j], f.a[i], acc[i][j], T());
-  };
-  auto multiply_sums = [&](const Frag& f, bool sum) __attribute__((always_inline)) {
-    if (SUMS && sum)
+    for (int i = 0; i < MI; ++i) {
 #pragma unroll
-      for (int x = 0; x < XS; ++x) asum[x] = mfma16(ones, f.x[x], asum[x], T());
-  };
-  auto interleave = []() __attribute__((always_inline)) {  // a read, a product, and so on
-    constexpr int READS = (AKS ? 2 : 1) * MI + (BKS ? 2 : 1) * NI, PER = (READS + MI * NI - 1) / (MI * NI);
+      for (int l = i * PER; l < (i + 1) * PER; ++l)
+        if (l < READS) read(q ^ 1, from, s, l);
 #pragma unroll
-    for (int i = 0; i < MI * NI; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(fb[q][j], fa[q][i], acc[i][j], T());
+      if (refill) load(r, to, i * (LOADS / 2) / MI, (i + 1) * (LOADS / 2) / MI);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
   };
-  constexpr int PARTS = GEMM_BK / 16;
+  auto add_sums = [&](uint32_t from) __attribute__((always_inline)) {  // the stage's share of the sums of A
+    const char DM_LDS* st = (const char DM_LDS*)smem + from;
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+      for (int x = 0; x < XS; ++x) asum[x] = mfma16(ones, fragment<BM, AKS>(st, lane, wm * MI + wn * XS + x, s), asum[x], T());
+  };
   const bool sums = SUMS && p.sums && tn == 0;
-  auto summed = [&](int it) {  // does the range's it-th step count for the sums of A
-    int seg, step;
-    if (!sums) return false;
-    place(it, seg, step);
-    return (p.sum_segments >> seg & 1) != 0;
-  };
   if (it0 < it1) {
     uint32_t cur = 0;
+    bool sum = false, next[GEMM_STAGES];  // do the stage at hand, and those asked for, count for the sums of A
 #pragma unroll
     for (int k = 0; k < GEMM_STAGES; ++k) {
-      const Request r = request(it0 + k, k * STAGE);
-#pragma unroll
-      for (int l = 0; l < LOADS; ++l) load(r, l);
+      const Request r = request(it0 + k);
+      next[k] = sums && r.sum;
+      load(r, k * STAGE, 0, LOADS / 2);
     }
     stage_arrived<LOADS * (GEMM_STAGES - 1)>();
-    bool sum = summed(it0);
-    read(f[0], 0, 0, sum);
+    sum = next[0];
+#pragma unroll
+    for (int l = 0; l < READS; ++l) read(0, 0, 0, l);
     for (int it = it0; it < it1; ++it) {
+      const Request r = request(it + GEMM_STAGES);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < PARTS - 1; ++s) {
-        read(f[(s + 1) & 1], cur, s + 1, sum);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) multiply_row(f[s & 1], i);
-        multiply_sums(f[s & 1], sum);
-        interleave();
-      }
-      const bool last = sum;
+      for (int s = 0; s < PARTS - 1; ++s) part(s & 1, cur, s + 1, false, r, 0);
+      static_assert(PARTS % 2 == 0, "a step ends with the set that it began with");
+      if (sum) add_sums(cur);
       const uint32_t left = cur;
       cur = cur + STAGE == GEMM_STAGES * STAGE ? 0 : cur + STAGE;
-      sum = it + 1 < it1 && summed(it + 1);
+#pragma unroll
+      for (int k = 0; k < GEMM_STAGES - 1; ++k) next[k] = next[k + 1];
+      next[GEMM_STAGES - 1] = sums && r.sum;
+      sum = next[0];
       stage_arrived<LOADS * (GEMM_STAGES - 2)>();
-      read(f[0], cur, 0, sum);  // (behind the range: zeros, and nobody's)
-      const Request r = request(it + GEMM_STAGES, left);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {  // loads among the products: a burst of them would hold up the wave
-        __builtin_amdgcn_sched_barrier(0);
-        multiply_row(f[(PARTS - 1) & 1], i);
-#pragma unroll
-        for (int l = i * LOADS / MI; l < (i + 1) * LOADS / MI; ++l) load(r, l);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      multiply_sums(f[(PARTS - 1) & 1], last);
+      part((PARTS - 1) & 1, cur, 0, true, r, left);  // (behind the range it reads zeros, and nobody uses them)
     }
   }
   stage_arrived<0>();  // the loads behind the range are done with LDS, and so is every wave
 
-  // acc[i][j][e] belongs to m = lane & 31 and n = 16 (lane >> 5) + e of the 32 x 32 block (i, j).  The i-th blocks of all waves meet in LDS
+  // acc[i][j][e] belongs to m = lane & 15 and n = 4 (lane >> 4) + e of the 16 x 16 block (i, j).  Two block rows of all waves meet in LDS
   // as rows of fp32 (a pitch of 16 bytes more than the row: no bank conflicts), two buffers in turn, and leave as whole pieces of
   // eight columns, neighbouring lanes next to each other: written straight from the accumulators, rows a power of two apart crowd
   // on few of the L2's channels (41 us of a 256 x 256 tile's time, measured at a row of 8 KB).
   constexpr int ROWS = WM * 32, PITCH = BN * 4 + 16, COLS = GATE ? BN / 2 : BN, PIECES = COLS / 8, TASKS = ROWS * PIECES / (NW * 64);
   const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces (with zeros: rows of B out of range are zero)
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
+  for (int i = 0; i < MI / 2; ++i) {
     char DM_LDS* buf = (char DM_LDS*)smem + (i & 1) * ROWS * PITCH;
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x16& c = acc[i][j];
-        *(DM_LDS f32x4*)(buf + (wm * 32 + (lane & 31)) * PITCH + ((wn * NI + j) * 32 + (lane >> 5) * 16 + q * 4) * 4) =
-            f32x4{c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
-      }
+      for (int j = 0; j < NI; ++j)
+        *(DM_LDS f32x4*)(buf + (wm * 32 + h * 16 + (lane & 15)) * PITCH + ((wn * NI + j) * 16 + (lane >> 4) * 4) * 4) = acc[i * 2 + h][j];
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < TASKS; ++t) {
       const int id = t * NW * 64 + threadIdx.x, row = id / PIECES, col = id % PIECES * 8;
-      const int64_t m = m0 + (row / 32 * MI + i) * 32 + row % 32;
+      const int64_t m = m0 + row / 32 * (MI * 16) + i * 32 + row % 32;
       const int n = n0 + col;
       if (m >= p.M || n >= (EPI == EPI_STORE ? p.N : np)) continue;
       const char DM_LDS* at = buf + row * PITCH + (GATE ? col / 32 * 64 + col % 32 : col) * 4;
@@ -491,8 +465,8 @@ gemm_kernel(const GemmArgs p) {
     if constexpr (SUMS) {  // every n of the product with ones holds the sum
 #pragma unroll
       for (int x = 0; x < XS; ++x) {
-        const int64_t m = m0 + (wm * MI + wn * XS + x) * 32 + lane;
-        if (!p.sums || tn || lane >= 32 || m >= p.M) continue;
+        const int64_t m = m0 + (wm * MI + wn * XS + x) * 16 + lane;
+        if (!p.sums || tn || lane >= 16 || m >= p.M) continue;
         if (p.splits > 1) ((float*)p.sums)[blockIdx.y * p.M + m] = asum[x][0];
         else if (p.sums_f32) ((float*)p.sums)[m] = asum[x][0];
         else ((T*)p.sums)[m] = (T)asum[x][0];
