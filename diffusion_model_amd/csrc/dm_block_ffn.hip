@@ -13,7 +13,8 @@
 
 namespace dmb {
 
-constexpr int SKINNY_ROWS = 64;
+constexpr int TOKEN_ROWS = 4;  // gemv_kernel
+constexpr int SKINNY_ROWS = 64;  // skinny_kernel, fp32
 
 // ---- operands that the products cannot read as they are: fp32 (three bf16 planes) and rows of no whole number of 16-byte pieces
 template <typename S, typename D, bool PLANES>
@@ -48,86 +49,210 @@ pack_rows_kernel(const S* __restrict__ src, int64_t ld, D* __restrict__ dst, int
   }
 }
 
-// ---- up to SKINNY_ROWS rows
-template <typename T> struct Skinny;
-template <> struct Skinny<bf16> {
-  static constexpr int V = 8;
-  static __device__ __forceinline__ f32x4 mul(const Vec<bf16, 8>& a, const Vec<bf16, 8>& b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
-};
-template <> struct Skinny<f16> {
-  static constexpr int V = 8;
-  static __device__ __forceinline__ f32x4 mul(const Vec<f16, 8>& a, const Vec<f16, 8>& b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-};
-template <> struct Skinny<float> {  // four instructions of four k each: instruction i takes element i of every lane's piece, on both sides
-  static constexpr int V = 4;
-  static __device__ __forceinline__ f32x4 mul(const Vec<float, 4>& a, const Vec<float, 4>& b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
-    return c;
-  }
+template <typename T>
+struct Streamed {  // arguments of gemv_kernel and skinny_kernel
+  const T *x; int64_t xs; const T *w, *w2; int64_t ldw; const T *bias, *bias2; T* out; int64_t ldo; T *ug, *ag; bf16* planes; int M, N, K, act;
 };
 
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_piece(const T* row, int k, int K, bool vec) {
-  Vec<T, V> r;
-  if (vec) {
-    if (k < K) return *reinterpret_cast<const Vec<T, V>*>(row + k);
+// h, and what the backward pass needs, of one element from its two sums; the padding of a row holds zeros.
+template <typename T>
+__device__ __forceinline__ void finish_gate(const Streamed<T>& p, int n, int64_t at, float g, float u) {
+  if (n >= ((p.N + 7) & ~7)) return;
+  float h = 0.f, ag = 0.f;
+  if (n < p.N) {
+    g += p.bias ? (float)p.bias[n] : 0.f;
+    u += p.bias2 ? (float)p.bias2[n] : 0.f;
+    float slope;
+    with_activation(p.act, [&](auto a) __attribute__((always_inline)) { activation<decltype(a)::value, sizeof(T) == 2>(g, ag, slope); });
+    h = ag * u;
+    u *= slope;
+  } else {
+    u = 0.f;
+  }
+  p.out[at] = (T)h;
+  if (p.ug) { p.ug[at] = (T)u; p.ag[at] = (T)ag; }
+  if (p.planes) {
+    bf16 t[3];
+    split3(h, t);
+    for (int k = 0; k < 3; ++k) p.planes[k * p.M * p.ldo + at] = t[k];
+  }
+}
+
+// ---- up to TOKEN_ROWS rows: the weights' bandwidth.  A wave takes R rows of w (and of w2) and multiplies them with all of x in vector
+// instructions, a row's piece of 64 V elements per load; the KSPLIT waves that share rows split the k range and meet in LDS.
+template <int NV>  // v[i] summed over the wave; lane l < NV gets the i = l-th sum
+__device__ __forceinline__ float wave_sums(float (&v)[NV], int lane) {
+  int n = NV;
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = (T)0.f;
+  for (int b = 0; (1 << b) < NV; ++b) {  // half of the values go to the other lane, which keeps those
+    n /= 2;
+    const bool up = lane >> b & 1;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = up ? v[2 * i + 1] : v[2 * i], send = up ? v[2 * i] : v[2 * i + 1];
+      v[i] = keep + __shfl_xor(send, 1 << b, 64);
+    }
+  }
+  float s = v[0];
+#pragma unroll
+  for (int o = NV; o < 64; o *= 2) s += __shfl_xor(s, o, 64);
+  return s;
+}
+
+template <typename T, int MR, bool GATE, int V, int KSPLIT>
+__global__ void __launch_bounds__(256)
+gemv_kernel(const Streamed<T> p) {
+  constexpr int R = 4, P = GATE ? 2 : 1, GROUPS = 4 / KSPLIT, NV = MR * R;
+  __shared__ float red[KSPLIT > 1 ? KSPLIT : 1][GROUPS][P][NV];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave / KSPLIT, part = wave % KSPLIT;
+  const int n0 = (blockIdx.x * GROUPS + group) * R;
+  const T* rows[P][R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1;
+    rows[0][r] = p.w + n * p.ldw;
+    if (GATE) rows[P - 1][r] = p.w2 + n * p.ldw;
+  }
+  float acc[P][NV] = {};
+#pragma unroll 2
+  for (int k = part * 64 * V + lane * V; k < p.K; k += KSPLIT * 64 * V) {
+    Vec<T, V> a[P][R], b[MR];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < P; ++q) a[q][r] = *reinterpret_cast<const Vec<T, V>*>(rows[q][r] + k);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) b[m] = *reinterpret_cast<const Vec<T, V>*>(p.x + (m < p.M ? m : p.M - 1) * p.xs + k);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+          for (int m = 0; m < MR; ++m) acc[q][m * R + r] = fmaf((float)a[q][r].v[i], (float)b[m].v[i], acc[q][m * R + r]);
+  }
+  float s[P];
+#pragma unroll
+  for (int q = 0; q < P; ++q) s[q] = wave_sums<NV>(acc[q], lane);
+  if constexpr (KSPLIT > 1) {
+    if (lane < NV)
+#pragma unroll
+      for (int q = 0; q < P; ++q) red[part][group][q][lane] = s[q];
+    __syncthreads();
+    if (part || lane >= NV) return;
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      s[q] = red[0][group][q][lane];
+#pragma unroll
+      for (int i = 1; i < KSPLIT; ++i) s[q] += red[i][group][q][lane];
+    }
+  }
+  const int m = lane / R, n = n0 + lane % R;
+  if (lane >= NV || m >= p.M) return;
+  const int64_t at = (int64_t)m * p.ldo + n;
+  if constexpr (GATE) finish_gate(p, n, at, s[0], s[P - 1]);
+  else if (n < p.N) p.out[at] = (T)(s[0] + (p.bias ? (float)p.bias[n] : 0.f));
+}
+
+template <typename T, bool GATE, int V>
+int gemv_launch(const Streamed<T>& a, hipStream_t st) {
+  const int groups = (int)(((int64_t)a.N + 7) / 8 * 8 + 3) / 4;  // of four rows, the padding of h among them
+  int split = 1;  // sixteen waves for every CU, as long as each has a load of its own
+  while (split < 4 && groups * split < 4096 && a.K > split * 64 * V) split *= 2;
+  auto run = [&](auto mr, auto ks) {
+    constexpr int MR = decltype(mr)::value, KS = decltype(ks)::value;
+    gemv_kernel<T, MR, GATE, V, KS><<<dim3((groups + 4 / KS - 1) / (4 / KS)), dim3(256), 0, st>>>(a);
+  };
+  auto rows = [&](auto ks) {
+    if (a.M == 1) run(std::integral_constant<int, 1>{}, ks);
+    else if (a.M == 2) run(std::integral_constant<int, 2>{}, ks);
+    else run(std::integral_constant<int, 4>{}, ks);
+  };
+  if (split == 1) rows(std::integral_constant<int, 1>{});
+  else if (split == 2) rows(std::integral_constant<int, 2>{});
+  else rows(std::integral_constant<int, 4>{});
+  return launched("dm_gated_ffn");
+}
+
+// ---- fp32, up to SKINNY_ROWS rows
+// Four instructions of four k each: instruction i takes element i of every lane's piece, on both sides.
+__device__ __forceinline__ f32x4 mfma_f32(const Vec<float, 4>& a, const Vec<float, 4>& b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+  return c;
+}
+
+__device__ __forceinline__ Vec<float, 4> load_piece(const float* row, int k, int K, bool vec) {
+  Vec<float, 4> r;
+  if (vec) {
+    if (k < K) return *reinterpret_cast<const Vec<float, 4>*>(row + k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = 0.f;
     return r;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = k + i < K ? row[k + i] : (T)0.f;
+  for (int i = 0; i < 4; ++i) r.v[i] = k + i < K ? row[k + i] : 0.f;
   return r;
 }
 
 constexpr int SKINNY_WAVES = 8;
 
-// out[m, n] for 16 n per block: the waves deal the k range among themselves in pieces, and their sums meet in LDS.
-template <typename T, int MT, bool GATE, bool VEC>
-__global__ void __launch_bounds__(SKINNY_WAVES * 64)
-skinny_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ w, const T* __restrict__ w2, int64_t ldw, const T* __restrict__ bias,
-              const T* __restrict__ bias2, T* __restrict__ out, int64_t ldo, T* __restrict__ ug_out, T* __restrict__ ag_out, bf16* __restrict__ planes, int M, int N, int K, int act) {
-  constexpr int V = Skinny<T>::V, STEP = 4 * V, P = GATE ? 2 : 1;
+// out[m, n] for 16 n per block: the waves deal the k range among themselves in chunks, and their sums meet in LDS.  A chunk is U pieces
+// of every row (U * 64 bytes on end), and the next chunk is on its way while one is multiplied.  Blocks begin at different chunks: in
+// step they would all ask for the same columns of rows a power of two apart, which lie on few of the memory's channels.
+template <int MT, bool GATE, bool VEC>
+__global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const Streamed<float> p) {
+  constexpr int V = 4, STEP = 4 * V, P = GATE ? 2 : 1;
+  constexpr int U = MT == 4 ? 2 : 4;
   __shared__ f32x4 red[SKINNY_WAVES][P][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = blockIdx.x * 16 + (lane & 15);
-  const int nc = n < N ? n : N - 1;
-  const T* w1r = w + nc * ldw;
-  const T* w2r = GATE ? w2 + nc * ldw : nullptr;
-  const T* xr[MT];
+  const int64_t nc = n < p.N ? n : p.N - 1;
+  const float* w1r = p.w + nc * p.ldw;
+  const float* w2r = GATE ? p.w2 + nc * p.ldw : nullptr;
+  const float* xr[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int m = t * 16 + (lane & 15);
-    xr[t] = x + (m < M ? m : M - 1) * xs;
+    xr[t] = p.x + (m < p.M ? m : p.M - 1) * p.xs;
   }
   f32x4 acc[P][MT] = {};
-  constexpr int U = 4;  // pieces in flight
-  for (int k0 = wave * STEP; k0 < K; k0 += SKINNY_WAVES * STEP * U) {
-    Vec<T, V> a[U], a2[U], b[U][MT];
+  struct Chunk { Vec<float, V> a[P][U], b[U][MT]; } one, two;
+  const int chunks = (p.K + U * STEP - 1) / (U * STEP), turn = (int)(blockIdx.x * 7u % (unsigned)chunks);
+  auto load = [&](Chunk& c, int at) __attribute__((always_inline)) {
+    if (at >= chunks) return;
+    at += turn;
+    if (at >= chunks) at -= chunks;
+    const int k0 = at * U * STEP + (lane >> 4) * V;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int k = k0 + i * SKINNY_WAVES * STEP + (lane >> 4) * V;
-      a[i] = load_piece<T, V>(w1r, k, K, VEC);
-      if (GATE) a2[i] = load_piece<T, V>(w2r, k, K, VEC);
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int k = k0 + i * SKINNY_WAVES * STEP + (lane >> 4) * V;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) b[i][t] = load_piece<T, V>(xr[t], k, K, VEC);
+      c.a[0][i] = load_piece(w1r, k0 + i * STEP, p.K, VEC);
+      if (GATE) c.a[P - 1][i] = load_piece(w2r, k0 + i * STEP, p.K, VEC);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        acc[0][t] = Skinny<T>::mul(a[i], b[i][t], acc[0][t]);
-        if constexpr (GATE) acc[1][t] = Skinny<T>::mul(a2[i], b[i][t], acc[1][t]);
-      }
+      for (int t = 0; t < MT; ++t) c.b[i][t] = load_piece(xr[t], k0 + i * STEP, p.K, VEC);
+  };
+  auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int q = 0; q < P; ++q) acc[q][t] = mfma_f32(c.a[q][i], c.b[i][t], acc[q][t]);
+  };
+  int at = wave;
+  load(one, at);
+  while (at < chunks) {
+    load(two, at + SKINNY_WAVES);
+    multiply(one);
+    at += SKINNY_WAVES;
+    if (at >= chunks) break;
+    load(one, at + SKINNY_WAVES);
+    multiply(two);
+    at += SKINNY_WAVES;
   }
 #pragma unroll
   for (int q = 0; q < P; ++q)
@@ -143,49 +268,32 @@ skinny_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ w, cons
     for (int v = 1; v < SKINNY_WAVES; ++v) s[q] += red[v][q][wave][lane];
   }
   const int m = wave * 16 + (lane & 15);
-  if (m >= M) return;
-  const int c0 = blockIdx.x * 16 + (lane >> 4) * 4;
-  if constexpr (GATE) {
-    with_activation(act, [&](auto a) __attribute__((always_inline)) {
+  if (m >= p.M) return;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = c0 + e;
-        if (c >= ((N + 7) & ~7)) continue;
-        float h = 0.f, ug = 0.f, ag = 0.f;  // the padding of a row holds zeros
-        if (c < N) {
-          const float g = s[0][e] + (bias ? (float)bias[c] : 0.f), u = s[P - 1][e] + (bias2 ? (float)bias2[c] : 0.f);
-          float slope;
-          activation<decltype(a)::value, sizeof(T) == 2>(g, ag, slope);
-          h = ag * u;
-          ug = u * slope;
-        }
-        const int64_t at = (int64_t)m * ldo + c;
-        out[at] = (T)h;
-        if (ug_out) { ug_out[at] = (T)ug; ag_out[at] = (T)ag; }
-        if (planes) {
-          bf16 t[3];
-          split3(h, t);
-          for (int k = 0; k < 3; ++k) planes[k * M * ldo + at] = t[k];
-        }
-      }
-    });
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c0 + e < N) out[(int64_t)m * ldo + c0 + e] = (T)(s[0][e] + (bias ? (float)bias[c0 + e] : 0.f));
+  for (int e = 0; e < 4; ++e) {
+    const int c = blockIdx.x * 16 + (lane >> 4) * 4 + e;
+    const int64_t to = (int64_t)m * p.ldo + c;
+    if constexpr (GATE) finish_gate(p, c, to, s[0][e], s[P - 1][e]);
+    else if (c < p.N) p.out[to] = s[0][e] + (p.bias ? p.bias[c] : 0.f);
   }
 }
 
-template <typename T, bool GATE, bool VEC>
-int skinny_launch(const T* x, int64_t xs, const T* w, const T* w2, int64_t ldw, const T* bias, const T* bias2, T* out, int64_t ldo, T* ug, T* ag,
-                  bf16* planes, int M, int N, int K, int act, hipStream_t st) {
-  const dim3 grid((N + 15) / 16), block(SKINNY_WAVES * 64);
-  switch ((M + 15) / 16) {
-    case 1: skinny_kernel<T, 1, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, ug, ag, planes, M, N, K, act); break;
-    case 2: skinny_kernel<T, 2, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, ug, ag, planes, M, N, K, act); break;
-    default: skinny_kernel<T, 4, GATE, VEC><<<grid, block, 0, st>>>(x, xs, w, w2, ldw, bias, bias2, out, ldo, ug, ag, planes, M, N, K, act);
-  }
+template <bool GATE, bool VEC>
+int skinny_launch(const Streamed<float>& a, hipStream_t st) {
+  const dim3 grid((a.N + 15) / 16), block(SKINNY_WAVES * 64);
+  if (a.M <= 16) skinny_kernel<1, GATE, VEC><<<grid, block, 0, st>>>(a);
+  else if (a.M <= 32) skinny_kernel<2, GATE, VEC><<<grid, block, 0, st>>>(a);
+  else skinny_kernel<4, GATE, VEC><<<grid, block, 0, st>>>(a);
   return launched("dm_gated_ffn");
+}
+
+template <typename T, bool GATE>
+int streamed(const Streamed<T>& a, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool whole = a.K % V == 0;  // (rows start at multiples of 16 bytes then: ffn_check_matrix)
+  if constexpr (std::is_same<T, float>::value)
+    if (a.M > TOKEN_ROWS) return whole ? skinny_launch<GATE, true>(a, st) : skinny_launch<GATE, false>(a, st);
+  return whole ? gemv_launch<T, GATE, V>(a, st) : gemv_launch<T, GATE, 1>(a, st);
 }
 
 // ---- workspace
@@ -269,7 +377,7 @@ Out between(const Operand& o) {  // an operand of a later product
 template <typename T, bool AKS, bool BKS>
 int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part, hipStream_t st) {
   constexpr bool F32 = std::is_same<T, float>::value;
-  const GemmPlan plan = gemm_plan(g.M, g.N, g.iters * g.segments, part != nullptr);
+  const GemmPlan plan = gemm_plan(g.M, g.N, g.iters * g.segments, 1, true, !AKS);
   g.splits = plan.splits;
   g.sums_f32 = F32;
   g.sum_segments = F32 ? 1 << 1 | 1 << 4 | 1 << 5 : 1;  // add_segments: each plane of A once
@@ -277,14 +385,15 @@ int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part
     g.out = out;
     g.bias = bias;
     g.sums = sums;
-    return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.big, st);
+    return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.tile, st);
   }
   const int ldp = (int)round_up(g.N, 8);
+  g.part = part;
+  g.ldpart = ldp;
   g.split_stride = g.M * ldp;
-  g.out = {part, ldp, 0, 1, 1};
   float* sum_part = (float*)part + plan.splits * g.split_stride;
   g.sums = sums ? sum_part : nullptr;
-  if (const int rc = gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.big, st)) return rc;
+  if (const int rc = gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.tile, st)) return rc;
   const int64_t blocks = (g.M * (ldp / 8) + 255) / 256;
   gemm_join_kernel<Mat<T>><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(
       (const float*)part, plan.splits, g.split_stride, bias, out, g.M, g.N, ldp, sum_part, sums);
@@ -316,18 +425,15 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   constexpr bool F32 = std::is_same<T, float>::value;
   const int64_t Fp = pad8(z.F);
   const Saved<T> kept(saved, z.M, z.F);
-  if (z.M <= SKINNY_ROWS) {
+  if (z.M <= TOKEN_ROWS || (F32 && z.M <= SKINNY_ROWS)) {
     T* h = saved && !F32 ? (T*)kept.h.p : (T*)ws.take((size_t)z.M * Fp * sizeof(T));
     if (!run) return 0;
-    constexpr int V = Skinny<T>::V;
     const int M = (int)z.M;
-    const bool vg = z.D % V == 0;  // (rows are 16-byte aligned then: ffn_check)
-    auto gate = vg ? skinny_launch<T, true, true> : skinny_launch<T, true, false>;
-    if (const int rc = gate((const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp, kept.ug, kept.ag,
-                            saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act, st))
-      return rc;
-    auto down = z.F % V == 0 ? skinny_launch<T, false, true> : skinny_launch<T, false, false>;
-    return down(h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, M, z.N, z.F, act, st);
+    const Streamed<T> gate = {(const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp, kept.ug, kept.ag,
+                              saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act};
+    if (const int rc = streamed<T, true>(gate, st)) return rc;
+    const Streamed<T> down = {h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, M, z.N, z.F, act};
+    return streamed<T, false>(down, st);
   }
   Operand x, wg, wu, wd, h;
   int rc = prepare_operand<T>(x, in.x, in.xs, z.M, z.D, ws, run, st);
@@ -337,19 +443,20 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   if (rc) return rc;
   h = saved ? kept.h : take_operand<T>(z.M, z.F, ws);
   const int segs = F32 ? 6 : 1;
-  const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F) * segs, true).part_bytes;
-  void* part = ws.take(part_bytes);
+  const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F) * segs, 1, true, true).part_bytes;
+  const GemmPlan gate = gemm_plan(z.M, z.F, iters_of(z.D) * segs, 2, true, true);
+  void* part = ws.take(gate.part_bytes > part_bytes ? gate.part_bytes : part_bytes);  // used by one product after the other
   if (!run) return 0;
 
   GemmArgs g = {};
   add_segments<T>(g, x, wg, &wu);
-  g.M = z.M; g.N = z.F; g.K = z.D; g.iters = iters_of(g.K); g.splits = 1;
+  g.M = z.M; g.N = z.F; g.K = z.D; g.iters = iters_of(g.K);
   g.out = between<T>(h);
   g.out2 = result<T>(kept.ug, Fp);
   g.out3 = result<T>(kept.ag, Fp);
   g.bias = in.bg; g.bias2 = in.bu; g.act = act;
-  const bool big = gemm_plan(z.M, 2 * z.F, g.iters * g.segments, false).big;
-  if ((rc = gemm_launch<Mat<T>, false, false, F32 ? EPI_GATE_F32 : EPI_GATE>(g, big, st))) return rc;
+  g.splits = gate.splits; g.part = part; g.ldpart = Fp; g.split_stride = z.M * Fp;
+  if ((rc = gemm_launch<Mat<T>, false, false, F32 ? EPI_GATE_F32 : EPI_GATE>(g, gate.tile, st))) return rc;
 
   GemmArgs d = {};
   add_segments<T>(d, h, wd);
@@ -374,8 +481,8 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws);
   const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
   const int rows_it = iters_of(z.M) * segs;
-  size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F) * segs * 2, true).part_bytes;
-  const size_t more[] = {gemm_plan(z.F, z.D, rows_it, true).part_bytes, gemm_plan(z.N, z.F, rows_it, true).part_bytes};
+  size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F) * segs * 2, 1, true, true).part_bytes;
+  const size_t more[] = {gemm_plan(z.F, z.D, rows_it, 1, true, false).part_bytes, gemm_plan(z.N, z.F, rows_it, 1, true, false).part_bytes};
   for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
   void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
   if (!run) return 0;
@@ -385,7 +492,7 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   a.M = z.M; a.N = z.F; a.K = z.N; a.iters = iters_of(a.K); a.splits = 1;
   a.out = between<T>(dg); a.out2 = between<T>(du);
   a.ug = kept.ug; a.ag = kept.ag; a.ldg = Fp;
-  if ((rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, gemm_plan(z.M, z.F, a.iters * a.segments, false).big, st))) return rc;
+  if ((rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, gemm_plan(z.M, z.F, a.iters * a.segments, 1, false, false).tile, st))) return rc;
 
   if (gr.dx) {
     GemmArgs g = {};

@@ -2,7 +2,7 @@
 #include "dm_block_gemm.hip"
 
 namespace dmb {
-template int gemm_launch<bf16, false, true, EPI_DACT>(GemmArgs, bool, hipStream_t);
-template int gemm_launch<f16, false, true, EPI_DACT>(GemmArgs, bool, hipStream_t);
-template int gemm_launch<bf16, false, true, EPI_DACT_F32>(GemmArgs, bool, hipStream_t);
+template int gemm_launch<bf16, false, true, EPI_DACT>(GemmArgs, int, hipStream_t);
+template int gemm_launch<f16, false, true, EPI_DACT>(GemmArgs, int, hipStream_t);
+template int gemm_launch<bf16, false, true, EPI_DACT_F32>(GemmArgs, int, hipStream_t);
 }  // namespace dmb

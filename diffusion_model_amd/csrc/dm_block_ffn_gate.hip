@@ -2,7 +2,7 @@
 #include "dm_block_gemm.hip"
 
 namespace dmb {
-template int gemm_launch<bf16, false, false, EPI_GATE>(GemmArgs, bool, hipStream_t);
-template int gemm_launch<f16, false, false, EPI_GATE>(GemmArgs, bool, hipStream_t);
-template int gemm_launch<bf16, false, false, EPI_GATE_F32>(GemmArgs, bool, hipStream_t);
+template int gemm_launch<bf16, false, false, EPI_GATE>(GemmArgs, int, hipStream_t);
+template int gemm_launch<f16, false, false, EPI_GATE>(GemmArgs, int, hipStream_t);
+template int gemm_launch<bf16, false, false, EPI_GATE_F32>(GemmArgs, int, hipStream_t);
 }  // namespace dmb

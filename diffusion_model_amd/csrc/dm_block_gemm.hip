@@ -5,13 +5,14 @@
 // is transposed on its way out of LDS (ds_read_tr).  The k range may be a chain of up to 12 segments, each with base pointers of its
 // own: the two terms of dx = dg Wg + du Wu, and the six products of fp32 operands that were split into three bf16 terms.
 //
-// A workgroup owns a BM x BN tile and walks k in steps of GEMM_BK: GEMM_STAGES LDS stages, filled by buffer loads that write LDS directly (16 bytes
+// A workgroup owns a BM x BN tile and walks k in steps of GEMM_BK: two LDS stages (three of the smallest tile), filled by buffer loads that write LDS directly (16 bytes
 // per lane, rows and columns out of range are bounds-checked to zero by the buffer resource), one barrier per step.  The LDS image
 // is swizzled in 16-byte pieces so that fragment reads touch all 64 banks once.  Fragments feed v_mfma_f32_16x16x32 with the n side as
 // the first operand: a lane then holds four consecutive n of one m.
 // A bias' gradient, the sum of A over k, is one more product with ones from the same fragments.
 #ifndef DM_BLOCK_GEMM_HIP
 #define DM_BLOCK_GEMM_HIP
+#include <atomic>
 #include <type_traits>
 
 #include "dm_block_common.h"
@@ -50,6 +51,12 @@ enum { OUT_16 = 0, OUT_F32 = 1, OUT_PLANES = 2 };
 // Where a result goes: rows of `ld` elements; OUT_PLANES: three bf16 planes, `plane` elements apart.  `vec`: rows take 16-byte stores.
 struct Out { void* p; int64_t ld, plane; int f32, vec; };
 
+__device__ __forceinline__ void store_f32(float* p, const float (&v)[8]) {
+  const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+  store_vec<float, 4>(p, a);
+  store_vec<float, 4>(p + 4, b);
+}
+
 template <typename T, int MODE>
 __device__ __forceinline__ void store8(const Out& o, int64_t m, int n, int N, const float (&v)[8]) {
   const int64_t at = m * o.ld + n;
@@ -57,9 +64,7 @@ __device__ __forceinline__ void store8(const Out& o, int64_t m, int n, int N, co
     if constexpr (MODE == OUT_16) {
       store_vec<T, 8>((T*)o.p + at, v);
     } else if constexpr (MODE == OUT_F32) {
-      const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-      store_vec<float, 4>((float*)o.p + at, a);
-      store_vec<float, 4>((float*)o.p + at + 4, b);
+      store_f32((float*)o.p + at, v);
     } else {
       Vec<bf16, 8> r[3];
 #pragma unroll
@@ -117,6 +122,21 @@ __device__ __forceinline__ void with_activation(int act, F&& f) {
   }
 }
 
+// h = act(g) u; g and u become what the backward pass needs: act(g) and u act'(g)
+template <bool FAST>
+__device__ __forceinline__ void gate_values(int act, float (&g)[8], float (&u)[8], float (&h)[8]) {
+  with_activation(act, [&](auto a) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float value, slope;
+      activation<decltype(a)::value, FAST>(g[e], value, slope);
+      h[e] = value * u[e];
+      u[e] *= slope;
+      g[e] = value;
+    }
+  });
+}
+
 template <typename S>
 __device__ __forceinline__ float bias_at(const void* b, int n, int N) { return b && n < N ? (float)((const S*)b)[n] : 0.f; }
 template <typename S>
@@ -132,7 +152,7 @@ __device__ __forceinline__ void load8(const S* p, float (&v)[8]) {
   }
 }
 
-constexpr int GEMM_BK = 64, GEMM_STAGES = 2;
+constexpr int GEMM_BK = 64;
 __device__ __forceinline__ void from_lds(const char DM_LDS* p, float (&v)[8]) {
   const f32x4 a = *(const DM_LDS f32x4*)p, b = *(const DM_LDS f32x4*)(p + 16);
 #pragma unroll
@@ -158,7 +178,8 @@ struct GemmArgs {
   const void *ug, *ag;                // DACT: u act'(g) and act(g), rows of ldg
   int64_t ldg;
   int act;
-  int64_t split_stride;               // STORE with splits > 1: fp32 partial products, elements from one split to the next
+  void* part;                         // splits > 1: fp32 partial products (GATE: of both projections in turn), rows of ldpart,
+  int64_t split_stride, ldpart;       // split_stride elements from one to the next; joined by a second launch
   void* sums;                         // STORE with both operands KS: sum over k of A[m, k] over the segments of sum_segments, or null.  One split:
   int sum_segments, sums_f32;         // of the type that sums_f32 gives; several: fp32, M apart
 };
@@ -234,7 +255,7 @@ __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, in
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool AKS, bool BKS, int EPI>
+template <typename T, int BM, int BN, int WM, int WN, int GEMM_STAGES, bool AKS, bool BKS, int EPI>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm_kernel(const GemmArgs p) {
   constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
@@ -242,7 +263,7 @@ gemm_kernel(const GemmArgs p) {
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
   using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
-  constexpr int XS = MI / WN;  // the waves of a tile row share its sums of A: XS blocks of 16 rows each
+  constexpr int XS = MI >= WN ? MI / WN : 1;  // the waves of a tile row share its sums of A: XS blocks of 16 rows each
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -426,30 +447,26 @@ gemm_kernel(const GemmArgs p) {
       if constexpr (GATE) {
         float u[8], h[8];
         from_lds(at + 128, u);
+        if (p.splits > 1) {  // finished by gate_join_kernel
+          float* part = (float*)p.part + 2 * blockIdx.y * p.split_stride + m * p.ldpart + n;
+          store_f32(part, v);
+          store_f32(part + p.split_stride, u);
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           v[e] += bias_at<Kept>(p.bias, n + e, p.N);
           u[e] += bias_at<Kept>(p.bias2, n + e, p.N);
         }
-        with_activation(p.act, [&](auto act) __attribute__((always_inline)) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float value, slope;
-            activation<decltype(act)::value, !F32>(v[e], value, slope);
-            h[e] = value * u[e];
-            u[e] *= slope;
-            v[e] = value;
-          }
-        });
+        gate_values<!F32>(p.act, v, u, h);
         store8<T, BETWEEN>(p.out, m, n, np, h);
         if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
       } else if constexpr (EPI == EPI_STORE) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
-        Out o = p.out;
-        if (p.splits > 1) o.p = (float*)o.p + blockIdx.y * p.split_stride;
-        if (o.f32) store8<T, OUT_F32>(o, m, n, p.N, v);
-        else store8<T, OUT_16>(o, m, n, p.N, v);
+        for (int e = 0; e < 8 && p.splits == 1; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
+        if (p.splits > 1) store_f32((float*)p.part + blockIdx.y * p.split_stride + m * p.ldpart + n, v);
+        else if (p.out.f32) store8<T, OUT_F32>(p.out, m, n, p.N, v);
+        else store8<T, OUT_16>(p.out, m, n, p.N, v);
       } else {
         float ug[8], ag[8];
         load8((const Kept*)p.ug + m * p.ldg + n, ug);
@@ -506,57 +523,119 @@ gemm_join_kernel(const float* __restrict__ part, int splits, int64_t stride, con
   }
 }
 
-struct GemmPlan { int big, splits; size_t part_bytes; };
+// The same for the gated product: bias, activation and product of the joined projections.
+template <typename T, bool F32>
+__global__ void __launch_bounds__(256) gate_join_kernel(const GemmArgs p) {
+  using Kept = typename std::conditional<F32, float, T>::type;
+  const int np = (p.N + 7) & ~7, pieces = np / 8;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < p.M * pieces; id += (int64_t)gridDim.x * 256) {
+    const int64_t m = id / pieces;
+    const int n = (int)(id % pieces) * 8;
+    const float* part = (const float*)p.part + m * p.ldpart + n;
+    float g[8] = {}, u[8] = {}, h[8];
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      float a[8], b[8];
+      load8(part + 2 * s * p.split_stride, a);
+      load8(part + (2 * s + 1) * p.split_stride, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { g[e] += a[e]; u[e] += b[e]; }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { g[e] += bias_at<Kept>(p.bias, n + e, p.N); u[e] += bias_at<Kept>(p.bias2, n + e, p.N); }
+    gate_values<!F32>(p.act, g, u, h);
+    store8<T, F32 ? OUT_PLANES : OUT_16>(p.out, m, n, np, h);
+    if (p.out2.p) { store8<T, F32 ? OUT_F32 : OUT_16>(p.out2, m, n, np, u); store8<T, F32 ? OUT_F32 : OUT_16>(p.out3, m, n, np, g); }
+  }
+}
 
-// Tile and split of the k range.  A big tile (256 x 256, one workgroup per CU) moves half the bytes per product of a small one (128 x 128,
-// two per CU); the smaller one fills the chip with fewer rows.  Where even small tiles leave CUs idle and the k range is long, it is
-// split and the partial products are joined by a second launch.  The estimate is in units of one 64-step of a big tile on one CU.
-inline GemmPlan gemm_plan(int64_t M, int N, int iters, bool can_split) {
+// Tiles.  WIDE, 256 x 256: one workgroup of 8 waves per CU; the fewest bytes and LDS reads per product.  MID, 128 x 128: two of 4 waves per
+// CU.  SLIM, 64 x 128: two of 4 waves per CU with three stages each, for rows so few that the n side's bytes are what counts.
+enum { TILE_WIDE, TILE_MID, TILE_SLIM, TILES };
+constexpr int TILE_M[TILES] = {256, 128, 64}, TILE_N[TILES] = {256, 128, 128}, TILE_PER_CU[TILES] = {1, 2, 2};
+
+struct GemmPlan { int tile, splits; size_t part_bytes; };
+
+// Tile and split of the k range.  Estimated in microseconds: rounds of workgroups over the chip, each of its k steps (measured: 1.6 us a
+// step of a WIDE tile, 1.2 and 0.8 us of two MID or SLIM tiles on a CU) and a start and an end; not less than the bytes of the n side at
+// 5.5 TB/s; and, where the k range is split to fill the chip, the joining launch.  `outs`: products per n (2: both projections).
+inline GemmPlan gemm_plan(int64_t M, int N, int iters, int outs, bool can_split, bool slim) {
   const int cus = 256;
-  GemmPlan best = {0, 1, 0};
+  constexpr double STEP[TILES] = {1.6, 1.2, 0.8};
+  GemmPlan best = {TILE_MID, 1, 0};
   double cost = 1e300;
-  for (int big = 0; big < 2; ++big) {
-    const int bm = big ? 256 : 128;
-    const int64_t tiles = ((M + bm - 1) / bm) * ((N + bm - 1) / bm);
+  for (int t = 0; t < TILES; ++t) {
+    if (t == TILE_SLIM && !slim) continue;
+    const int64_t tiles = ((M + TILE_M[t] - 1) / TILE_M[t]) * (((int64_t)N * outs + TILE_N[t] - 1) / TILE_N[t]);
+    const int slots = cus * TILE_PER_CU[t];
     for (int s = 1; s <= 64; s *= 2) {
-      if (s > 1 && (!can_split || s > iters / 2 || tiles * (s / 2) >= 2 * cus)) break;
-      const int slots = big ? cus : 2 * cus;
+      if (s > 1 && (!can_split || s * 8 > iters || tiles * (s / 2) >= slots)) break;
       const double rounds = (double)((tiles * s + slots - 1) / slots);
-      const double step = big ? 1.0 : 0.7;  // two small tiles share a CU
-      double c = rounds * ((iters + s - 1) / s + 4.0) * step;
-      if (s > 1) c += 4.0 + (double)M * N * 4 * (s + 1) / 4.0e6;  // the joining launch at 4 TB/s, a step being about a microsecond
-      if (c < cost) { cost = c; best.big = big; best.splits = s; }
+      const double fill = tiles * s < slots / 2 && TILE_PER_CU[t] > 1 ? 0.6 : 1.0;  // alone on its CU a workgroup is faster
+      double c = rounds * (((iters + s - 1) / s) * STEP[t] * fill + 4.0);
+      const double stream = (double)N * outs * iters * GEMM_BK * 2 / 5.5e6;
+      if (c < stream) c = stream;
+      if (s > 1) c += 3.0 + (double)M * N * outs * 4 * 2 * s / 5.0e6;
+      if (c < cost) { cost = c; best.tile = t; best.splits = s; }
     }
   }
-  if (best.splits > 1) best.part_bytes = (size_t)best.splits * M * (round_up(N, 8) + 1) * 4;  // products, and sums of A
+  if (best.splits > 1) best.part_bytes = (size_t)best.splits * outs * M * (round_up(N, 8) + 1) * 4;  // products, and sums of A
   return best;
 }
 
+// The kernel's dynamic LDS on the current device, set at its first launch there (`done`: of the caller's own).
+inline hipError_t allow_lds(const void* f, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return hipSuccess;
+  e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename T, bool AKS, bool BKS, int EPI>
-int gemm_launch(GemmArgs a, bool big, hipStream_t st) {
-  const int bm = big ? 256 : 128, bn = EPI == EPI_GATE || EPI == EPI_GATE_F32 ? bm / 2 : bm;
+int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
+  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, SLIM = !AKS && (EPI == EPI_STORE || GATE);
+  const int bm = TILE_M[tile], bn = TILE_N[tile];
   a.tiles_m = (int)((a.M + bm - 1) / bm);
-  a.tiles_n = (a.N + bn - 1) / bn;
+  a.tiles_n = GATE ? (a.N + bn / 2 - 1) / (bn / 2) : (a.N + bn - 1) / bn;
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > (1 << 22)) return fail("gated feed-forward block: %lld output tiles in one product", (long long)tiles);
   const dim3 grid((unsigned)tiles, a.splits);
-  const int stages = GEMM_STAGES * 2 * bm * GEMM_BK * 2, rows = 2 * 64 * (bm * 4 + 16), bytes = stages > rows ? stages : rows;
-  const void* f = big ? (const void*)gemm_kernel<T, 256, 256, 2, 4, AKS, BKS, EPI> : (const void*)gemm_kernel<T, 128, 128, 2, 2, AKS, BKS, EPI>;
-  hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const void* f;
+  int bytes;  // the stages, or the epilogue's two buffers of rows
+  if (tile == TILE_WIDE) {
+    f = (const void*)gemm_kernel<T, 256, 256, 2, 4, 2, AKS, BKS, EPI>;
+    bytes = 2 * 64 * (256 * 4 + 16);
+  } else if (!SLIM || tile == TILE_MID) {
+    f = (const void*)gemm_kernel<T, 128, 128, 2, 2, 2, AKS, BKS, EPI>;
+    bytes = 2 * 64 * (128 * 4 + 16);
+  } else {
+    if constexpr (SLIM) f = (const void*)gemm_kernel<T, 64, 128, 1, 4, 3, AKS, BKS, EPI>;
+    bytes = 3 * (64 + 128) * GEMM_BK * 2;
+  }
+  static std::atomic<uint64_t> done[TILES];
+  hipError_t e = allow_lds(f, bytes, done[tile]);
   if (e == hipSuccess) {
     void* args[] = {&a};
-    e = hipLaunchKernel(f, grid, dim3(big ? 512 : 256), args, bytes, st);
+    e = hipLaunchKernel(f, grid, dim3(tile == TILE_WIDE ? 512 : 256), args, bytes, st);
+  }
+  if (e == hipSuccess && GATE && a.splits > 1) {  // (a.splits is 1 elsewhere: product joins its own)
+    const int64_t blocks = (a.M * ((a.N + 7) / 8) + 255) / 256;
+    gate_join_kernel<T, EPI == EPI_GATE_F32><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
+    e = hipGetLastError();
   }
   return e == hipSuccess ? 0 : fail("gated feed-forward block: launch failed: %s", hipGetErrorString(e));
 }
 
 // The fused products are compiled in translation units of their own (dm_block_ffn_gate.hip, dm_block_ffn_dact.hip).
-extern template int gemm_launch<bf16, false, false, EPI_GATE>(GemmArgs, bool, hipStream_t);
-extern template int gemm_launch<f16, false, false, EPI_GATE>(GemmArgs, bool, hipStream_t);
-extern template int gemm_launch<bf16, false, false, EPI_GATE_F32>(GemmArgs, bool, hipStream_t);
-extern template int gemm_launch<bf16, false, true, EPI_DACT>(GemmArgs, bool, hipStream_t);
-extern template int gemm_launch<f16, false, true, EPI_DACT>(GemmArgs, bool, hipStream_t);
-extern template int gemm_launch<bf16, false, true, EPI_DACT_F32>(GemmArgs, bool, hipStream_t);
+extern template int gemm_launch<bf16, false, false, EPI_GATE>(GemmArgs, int, hipStream_t);
+extern template int gemm_launch<f16, false, false, EPI_GATE>(GemmArgs, int, hipStream_t);
+extern template int gemm_launch<bf16, false, false, EPI_GATE_F32>(GemmArgs, int, hipStream_t);
+extern template int gemm_launch<bf16, false, true, EPI_DACT>(GemmArgs, int, hipStream_t);
+extern template int gemm_launch<f16, false, true, EPI_DACT>(GemmArgs, int, hipStream_t);
+extern template int gemm_launch<bf16, false, true, EPI_DACT_F32>(GemmArgs, int, hipStream_t);
 
 }  // namespace dmb
 #endif

@@ -45,15 +45,18 @@ def _vector(t, n, x, name, dtypes=None):
 
 
 def _rows(t):
-    """[..., C] as rows the kernels can read: (tensor [M, C], row stride in elements)."""
+    """[..., C] as rows the kernels can read: (tensor, row stride in elements, number of rows)."""
     c = t.shape[-1]
+    if t.is_contiguous():
+        if t.data_ptr() % 16 == 0:
+            return t, c, t.numel() // c
+        return t.clone(), c, t.numel() // c
     r = t.reshape(-1, c)
-    whole = 16 // t.element_size()
-    if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and (r.stride(0) < c or r.stride(0) > 1 << 21)):
-        r = r.contiguous()
-    if c % whole == 0 and (r.data_ptr() % 16 or (r.shape[0] > 1 and r.stride(0) % whole)):
+    m, whole = r.shape[0], 16 // t.element_size()
+    if (c > 1 and r.stride(1) != 1) or (m > 1 and (r.stride(0) < c or r.stride(0) > 1 << 21)) or \
+            (c % whole == 0 and (r.data_ptr() % 16 or (m > 1 and r.stride(0) % whole))):
         r = r.clone(memory_format=torch.contiguous_format)
-    return r, (r.stride(0) if r.shape[0] > 1 else c)
+    return r, (r.stride(0) if m > 1 else c), m
 
 
 def _matrix(t, rows, cols, x, name):
@@ -64,12 +67,28 @@ def _matrix(t, rows, cols, x, name):
     return t.clone() if t.data_ptr() % 16 else t
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(t, fn, *args):
+    """fn(*args, stream) on the tensor's device and its current stream; raises what the library reports."""
+    index = t.get_device()
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _empty_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _workspace(t, nbytes):
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=t.device)
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=t.device)
 
 
 # ------------------------------------------------------------------ layer norm
@@ -85,16 +104,15 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     b = _vector(bias, c, x, "bias", (x.dtype, torch.float32) if w is None else (w.dtype,))
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    p = w if w is not None else b
-    with torch.cuda.device(x.device):
-        r, stride = _rows(x)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = rstd = None
-        if return_stats:
-            mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
-        _lib.check(_lib.lib().dm_layer_norm(
-            _lib.ptr(r), stride, _lib.ptr(w), _lib.ptr(b), dt if p is None else _DTYPES[p.dtype], _lib.ptr(y), _lib.ptr(mean),
-            _lib.ptr(rstd), r.shape[0], c, eps, dt, _stream(x)))
+    p = x if w is None and b is None else b if w is None else w
+    r, stride, m = _rows(x)
+    y = _empty_like(x)
+    mean = rstd = None
+    if return_stats:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+    _call(x, _lib.lib().dm_layer_norm, r.data_ptr(), stride, _ptr(w), _ptr(b), _DTYPES[p.dtype], y.data_ptr(), _ptr(mean), _ptr(rstd), m, c,
+          eps, dt)
     return (y, mean, rstd) if return_stats else y
 
 
@@ -111,19 +129,19 @@ def layer_norm_backward(grad, x, weight, mean, rstd):
         _like(t, x, name, (torch.float32,))
         if t.shape != x.shape[:-1]:
             raise RuntimeError(f"{name} must be {tuple(x.shape[:-1])} (got {tuple(t.shape)})")
-    with torch.cuda.device(x.device):
-        L = _lib.lib()
-        r, stride = _rows(x)
-        g, gstride = _rows(grad)
-        mean, rstd = mean.contiguous(), rstd.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = db = ws = None
-        if w is not None:
-            dw, db = torch.empty_like(w), torch.empty_like(w)
-            ws = _workspace(x, L.dm_layer_norm_backward_workspace_bytes(r.shape[0], c))
-        _lib.check(L.dm_layer_norm_backward(
-            _lib.ptr(g), gstride, _lib.ptr(r), stride, _lib.ptr(w), dt if w is None else _DTYPES[w.dtype], _lib.ptr(mean), _lib.ptr(rstd),
-            _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), r.shape[0], c, dt, _lib.ptr(ws), 0 if ws is None else ws.numel(), _stream(x)))
+    L = _lib.lib()
+    r, stride, m = _rows(x)
+    g, gstride, _ = _rows(grad)
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    dx = _empty_like(x)
+    dw = db = ws = None
+    nbytes = 0
+    if w is not None:
+        dw, db = torch.empty_like(w), torch.empty_like(w)
+        nbytes = L.dm_layer_norm_backward_workspace_bytes(m, c)
+        ws = _workspace(x, nbytes)
+    _call(x, L.dm_layer_norm_backward, g.data_ptr(), gstride, r.data_ptr(), stride, _ptr(w), dt if w is None else _DTYPES[w.dtype],
+          mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), m, c, dt, _ptr(ws), nbytes)
     return dx, dw, db
 
 
@@ -164,12 +182,11 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     return inv.repeat(axes).to(device if device is not None else "cpu"), scale
 
 
+_Strides = C.c_int64 * 3
+
+
 def _rotary_tensor(t, out):
-    r = _lib.RotaryTensor()
-    r.in_, r.out, r.heads = t.data_ptr(), out.data_ptr(), t.shape[2]
-    for i in range(3):
-        r.in_stride[i], r.out_stride[i] = t.stride(i), out.stride(i)
-    return r
+    return _lib.RotaryTensor(t.data_ptr(), out.data_ptr(), _Strides(*t.stride()[:3]), _Strides(*out.stride()[:3]), t.shape[2])
 
 
 def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inverse=False, inplace=False):
@@ -202,30 +219,30 @@ def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inver
             raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] (got {tuple(positions.shape)})")
         if any(have not in (1, want) for have, want in zip(positions.shape[::-1], (t, b))):
             raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] with B = {b}, T = {t} (got {tuple(positions.shape)})")
-        positions = positions.to(torch.int64).expand(axes, b, t)
-        strides = (C.c_int64 * 3)(*positions.stride())
+        positions = positions.to(torch.int64)
+        if positions.shape != (axes, b, t):
+            positions = positions.expand(axes, b, t)
+        strides = _Strides(*positions.stride())
     if inv_freq.numel() % axes:
         raise RuntimeError(f"{inv_freq.numel()} pairs do not divide into {axes} axes")
-    with torch.cuda.device(q.device):
-        ins, outs = [], []
-        for x in (q, k):
-            if x is None:
-                outs.append(None)
-                continue
-            if inplace:
-                if (d > 1 and x.stride(3) != 1) or any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-                    raise RuntimeError("in place needs contiguous head elements and no expanded dimension")
-                out = x
-            else:
-                x = x if d == 1 or x.stride(3) == 1 else x.contiguous()
-                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            ins.append(x)
-            outs.append(out)
-        args = [_rotary_tensor(x, o) for x, o in zip(ins, [o for o in outs if o is not None])]
-        inv_freq = inv_freq.contiguous()
-        _lib.check(_lib.lib().dm_rotary(
-            C.byref(args[0]), C.byref(args[1]) if len(args) > 1 else None, _lib.ptr(positions), strides, axes, _lib.ptr(inv_freq), b, t, d,
-            rotary_dim, int(layout == "interleaved"), scale, int(inverse), dt, _stream(q)))
+    args, outs = [], []
+    for x in (q, k):
+        if x is None:
+            args.append(None)
+            outs.append(None)
+            continue
+        if inplace:
+            if (d > 1 and x.stride(3) != 1) or any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+                raise RuntimeError("in place needs contiguous head elements and no expanded dimension")
+            out = x
+        else:
+            x = x if d == 1 or x.stride(3) == 1 else x.contiguous()
+            out = _empty_like(x)
+        args.append((x, _rotary_tensor(x, out)))
+        outs.append(out)
+    inv_freq = inv_freq.contiguous()
+    _call(q, _lib.lib().dm_rotary, C.byref(args[0][1]), None if k is None else C.byref(args[1][1]), _ptr(positions), strides, axes,
+          inv_freq.data_ptr(), b, t, d, rotary_dim, layout == "interleaved", scale, bool(inverse), dt)
     return tuple(outs)
 
 
@@ -238,11 +255,10 @@ def _ffn_check(x, w_gate, w_up, w_down, activation):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"x must be [..., width] (got {tuple(x.shape)})")
     d = x.shape[-1]
-    with torch.cuda.device(x.device):
-        w_gate = _matrix(w_gate, None, d, x, "w_gate")
-        f = w_gate.shape[0]
-        w_up = _matrix(w_up, f, d, x, "w_up")
-        w_down = _matrix(w_down, None, f, x, "w_down")
+    w_gate = _matrix(w_gate, None, d, x, "w_gate")
+    f = w_gate.shape[0]
+    w_up = _matrix(w_up, f, d, x, "w_up")
+    w_down = _matrix(w_down, None, f, x, "w_down")
     if f < 1 or w_down.shape[0] < 1:
         raise RuntimeError("the weights must not be empty")
     return dt, d, f, w_down.shape[0], w_gate, w_up, w_down
@@ -255,16 +271,14 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     between the matrix products; fp32 keeps fp32 accuracy."""
     dt, d, f, n, w_gate, w_up, w_down = _ffn_check(x, w_gate, w_up, w_down, activation)
     b_gate, b_up, b_down = _vector(b_gate, f, x, "b_gate"), _vector(b_up, f, x, "b_up"), _vector(b_down, n, x, "b_down")
-    with torch.cuda.device(x.device):
-        L = _lib.lib()
-        r, stride = _rows(x)
-        m = r.shape[0]
-        y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-        saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt), dtype=torch.uint8, device=x.device) if save else None
-        ws = _workspace(x, L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt, int(save)))
-        _lib.check(L.dm_gated_ffn(
-            _lib.ptr(r), stride, _lib.ptr(w_gate), _lib.ptr(w_up), _lib.ptr(w_down), _lib.ptr(b_gate), _lib.ptr(b_up), _lib.ptr(b_down),
-            _lib.ptr(y), _lib.ptr(saved), m, d, f, n, _ACTIVATIONS[activation], dt, _lib.ptr(ws), ws.numel(), _stream(x)))
+    L = _lib.lib()
+    r, stride, m = _rows(x)
+    y = _empty_like(x) if n == d else torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt), dtype=torch.uint8, device=x.device) if save else None
+    nbytes = L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt, save)
+    ws = _workspace(x, nbytes)
+    _call(x, L.dm_gated_ffn, r.data_ptr(), stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _ptr(b_gate), _ptr(b_up), _ptr(b_down),
+          y.data_ptr(), _ptr(saved), m, d, f, n, _ACTIVATIONS[activation], dt, ws.data_ptr(), nbytes)
     return (y, saved) if save else y
 
 
@@ -275,19 +289,17 @@ def gated_ffn_backward(grad, x, w_gate, w_up, w_down, saved, activation="silu", 
     _like(grad, x, "grad")
     if grad.shape != x.shape[:-1] + (n,):
         raise RuntimeError(f"grad must be {tuple(x.shape[:-1]) + (n,)} (got {tuple(grad.shape)})")
-    with torch.cuda.device(x.device):
-        L = _lib.lib()
-        r, stride = _rows(x)
-        g, gstride = _rows(grad)
-        m = r.shape[0]
-        if not torch.is_tensor(saved) or saved.device != x.device or saved.dtype != torch.uint8 or not saved.is_contiguous() or \
-                saved.numel() != L.dm_gated_ffn_saved_bytes(m, f, dt):
-            raise RuntimeError("saved must be what gated_ffn(..., save=True) returned for this input")
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dws = [torch.empty_like(w) for w in (w_gate, w_up, w_down)]
-        dbs = [torch.empty(size, dtype=x.dtype, device=x.device) if bias else None for size in (f, f, n)]
-        ws = _workspace(x, L.dm_gated_ffn_backward_workspace_bytes(m, d, f, n, dt))
-        _lib.check(L.dm_gated_ffn_backward(
-            _lib.ptr(g), gstride, _lib.ptr(r), stride, _lib.ptr(w_gate), _lib.ptr(w_up), _lib.ptr(w_down), _lib.ptr(saved), _lib.ptr(dx),
-            *(_lib.ptr(t) for t in dws + dbs), m, d, f, n, _ACTIVATIONS[activation], dt, _lib.ptr(ws), ws.numel(), _stream(x)))
+    L = _lib.lib()
+    r, stride, m = _rows(x)
+    g, gstride, _ = _rows(grad)
+    if not torch.is_tensor(saved) or saved.device != x.device or saved.dtype != torch.uint8 or not saved.is_contiguous() or \
+            saved.numel() != L.dm_gated_ffn_saved_bytes(m, f, dt):
+        raise RuntimeError("saved must be what gated_ffn(..., save=True) returned for this input")
+    dx = _empty_like(x)
+    dws = [torch.empty_like(w) for w in (w_gate, w_up, w_down)]
+    dbs = [torch.empty(size, dtype=x.dtype, device=x.device) if bias else None for size in (f, f, n)]
+    nbytes = L.dm_gated_ffn_backward_workspace_bytes(m, d, f, n, dt)
+    ws = _workspace(x, nbytes)
+    _call(x, L.dm_gated_ffn_backward, g.data_ptr(), gstride, r.data_ptr(), stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+          saved.data_ptr(), dx.data_ptr(), *(_ptr(t) for t in dws + dbs), m, d, f, n, _ACTIVATIONS[activation], dt, ws.data_ptr(), nbytes)
     return (dx, *dws, *dbs)
