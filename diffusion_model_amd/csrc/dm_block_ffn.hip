@@ -347,19 +347,18 @@ Operand take_operand(int64_t rows, int cols, Carver& ws) {
   return o;
 }
 
-// The product terms of two operands: one, or the six of split fp32.
+// The product terms of two operands (`second`: of two more, of the same shape): one, or the six of split fp32.
 template <typename T>
-void add_segments(GemmArgs& g, const Operand& a, const Operand& b, const Operand* b2 = nullptr) {
-  auto add = [&](int i, int j) {
-    g.a[g.segments] = (const bf16*)a.p + i * a.plane;
-    g.b[g.segments] = (const bf16*)b.p + j * b.plane;
-    g.b2[g.segments] = b2 ? (const bf16*)b2->p + j * b2->plane : nullptr;
-    ++g.segments;
-  };
+void add_terms(GemmArgs& g, const Operand& a, const Operand& b, bool second = false) {
+  auto add = [&](uint64_t i, uint64_t j) { g.terms |= (i | j << 2 | (second ? 16 : 0)) << 5 * g.segments++; };
   if (std::is_same<T, float>::value) { add(0, 2); add(2, 0); add(1, 1); add(0, 1); add(1, 0); }  // small terms first
   add(0, 0);
+  g.a[second] = a.p;
+  g.b[second] = b.p;
   g.lda = a.ld;
   g.ldb = b.ld;
+  g.plane_a = a.plane * 2;
+  g.plane_b = b.plane * 2;
 }
 
 template <typename T> using Mat = typename std::conditional<std::is_same<T, float>::value, bf16, T>::type;  // what the matrix pipe sees
@@ -373,31 +372,25 @@ Out between(const Operand& o) {  // an operand of a later product
   return {const_cast<void*>(o.p), o.ld, o.plane, 0, 1};
 }
 
-// out[M][N] = A B (+ bias), the k range split where that pays; sums: the sum of A over k (both operands KS).
+// The plan of a product, and where it keeps its parts (`part`: room for them).
+inline int planned(GemmArgs& g, const GemmPlan& plan, void* part) {
+  g.splits = plan.splits;
+  g.part = part;
+  g.ldpart = round_up(g.N, 8);
+  g.split_stride = g.M * g.ldpart;
+  return plan.tile;
+}
+
+// out[M][N] = A B (+ bias); sums: the sum of A over k (both operands KS).
 template <typename T, bool AKS, bool BKS>
 int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part, hipStream_t st) {
-  constexpr bool F32 = std::is_same<T, float>::value;
-  const GemmPlan plan = gemm_plan(g.M, g.N, g.iters * g.segments, 1, true, !AKS);
-  g.splits = plan.splits;
-  g.sums_f32 = F32;
-  g.sum_segments = F32 ? 1 << 1 | 1 << 4 | 1 << 5 : 1;  // add_segments: each plane of A once
-  if (plan.splits == 1) {
-    g.out = out;
-    g.bias = bias;
-    g.sums = sums;
-    return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.tile, st);
-  }
-  const int ldp = (int)round_up(g.N, 8);
-  g.part = part;
-  g.ldpart = ldp;
-  g.split_stride = g.M * ldp;
-  float* sum_part = (float*)part + plan.splits * g.split_stride;
-  g.sums = sums ? sum_part : nullptr;
-  if (const int rc = gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, plan.tile, st)) return rc;
-  const int64_t blocks = (g.M * (ldp / 8) + 255) / 256;
-  gemm_join_kernel<Mat<T>><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(
-      (const float*)part, plan.splits, g.split_stride, bias, out, g.M, g.N, ldp, sum_part, sums);
-  return launched("gated feed-forward block");
+  const int tile = planned(g, gemm_plan(g.M, g.N, g.iters, g.segments, 1, sizeof(T), !AKS), part);
+  g.out = out;
+  g.bias = bias;
+  g.sums = sums;
+  g.sum_part = (float*)part + g.splits * g.split_stride;
+  g.sum_segments = std::is_same<T, float>::value ? 1 << 1 | 1 << 4 | 1 << 5 : 1;  // add_terms: each plane of A once
+  return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, tile, st);
 }
 
 inline int iters_of(int64_t K) { return (int)((K + GEMM_BK - 1) / GEMM_BK); }
@@ -442,24 +435,25 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
   if (rc) return rc;
   h = saved ? kept.h : take_operand<T>(z.M, z.F, ws);
-  const int segs = F32 ? 6 : 1;
-  const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F) * segs, 1, true, true).part_bytes;
-  const GemmPlan gate = gemm_plan(z.M, z.F, iters_of(z.D) * segs, 2, true, true);
+  const int terms = F32 ? 6 : 1;
+  const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F), terms, 1, sizeof(T), true).part_bytes;
+  const GemmPlan gate = gemm_plan(z.M, z.F, iters_of(z.D), terms, 2, F32 ? 7 : 3, true);
   void* part = ws.take(gate.part_bytes > part_bytes ? gate.part_bytes : part_bytes);  // used by one product after the other
   if (!run) return 0;
 
   GemmArgs g = {};
-  add_segments<T>(g, x, wg, &wu);
+  add_terms<T>(g, x, wg);
+  g.b2 = wu.p;
   g.M = z.M; g.N = z.F; g.K = z.D; g.iters = iters_of(g.K);
   g.out = between<T>(h);
   g.out2 = result<T>(kept.ug, Fp);
   g.out3 = result<T>(kept.ag, Fp);
   g.bias = in.bg; g.bias2 = in.bu; g.act = act;
-  g.splits = gate.splits; g.part = part; g.ldpart = Fp; g.split_stride = z.M * Fp;
-  if ((rc = gemm_launch<Mat<T>, false, false, F32 ? EPI_GATE_F32 : EPI_GATE>(g, gate.tile, st))) return rc;
+  const int tile = planned(g, gate, part);
+  if ((rc = gemm_launch<Mat<T>, false, false, F32 ? EPI_GATE_F32 : EPI_GATE>(g, tile, st))) return rc;
 
   GemmArgs d = {};
-  add_segments<T>(d, h, wd);
+  add_terms<T>(d, h, wd);
   d.M = z.M; d.N = z.N; d.K = z.F; d.iters = iters_of(z.F);
   return product<T, false, false>(d, result<T>(y, z.N), in.bd, nullptr, part, st);
 }
@@ -470,7 +464,7 @@ template <typename T>
 int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys, const void* saved, const FfnGrads& gr, Carver& ws, bool run,
                  hipStream_t st) {
   const int64_t Fp = pad8(z.F);
-  const int segs = std::is_same<T, float>::value ? 6 : 1;
+  const int terms = std::is_same<T, float>::value ? 6 : 1;
   Operand x, wg, wu, wd, y;
   int rc = prepare_operand<T>(y, dy, dys, z.M, z.N, ws, run, st);
   if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
@@ -480,31 +474,32 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   if (rc) return rc;
   const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws);
   const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
-  const int rows_it = iters_of(z.M) * segs;
-  size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F) * segs * 2, 1, true, true).part_bytes;
-  const size_t more[] = {gemm_plan(z.F, z.D, rows_it, 1, true, false).part_bytes, gemm_plan(z.N, z.F, rows_it, 1, true, false).part_bytes};
+  size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F), terms * 2, 1, sizeof(T), true).part_bytes;
+  const GemmPlan dact = gemm_plan(z.M, z.F, iters_of(z.N), terms, 1, terms > 1 ? 20 : 8, true);
+  const size_t more[] = {dact.part_bytes, gemm_plan(z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes, gemm_plan(z.N, z.F, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes};
   for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
   void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
   if (!run) return 0;
 
   GemmArgs a = {};  // dh, and from it dg and du
-  add_segments<T>(a, y, wd);
-  a.M = z.M; a.N = z.F; a.K = z.N; a.iters = iters_of(a.K); a.splits = 1;
+  add_terms<T>(a, y, wd);
+  a.M = z.M; a.N = z.F; a.K = z.N; a.iters = iters_of(a.K);
   a.out = between<T>(dg); a.out2 = between<T>(du);
   a.ug = kept.ug; a.ag = kept.ag; a.ldg = Fp;
-  if ((rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, gemm_plan(z.M, z.F, a.iters * a.segments, 1, false, false).tile, st))) return rc;
+  const int tile = planned(a, dact, part);
+  if ((rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, tile, st))) return rc;
 
   if (gr.dx) {
     GemmArgs g = {};
-    add_segments<T>(g, dg, wg);
-    add_segments<T>(g, du, wu);
+    add_terms<T>(g, dg, wg);
+    add_terms<T>(g, du, wu, true);
     g.M = z.M; g.N = z.D; g.K = z.F; g.iters = iters_of(z.F);
     if ((rc = product<T, false, true>(g, result<T>(gr.dx, z.D), nullptr, nullptr, part, st))) return rc;
   }
   // (the sum of dg^T, du^T, dy^T over the rows of the batch is the bias' gradient)
   auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out, void* bias) {
     GemmArgs g = {};
-    add_segments<T>(g, l, r);
+    add_terms<T>(g, l, r);
     g.M = rows; g.N = cols; g.K = (int)z.M; g.iters = iters_of(z.M);
     return product<T, true, true>(g, result<T>(out, cols), nullptr, bias, part, st);
   };

@@ -2,8 +2,8 @@
 //
 // An operand is stored either with k contiguous ("KC": rows of the operand) or with its own rows contiguous ("KS": k is the slow
 // index), so that the forward pass and all three products of the backward pass run from the tensors as they lie in memory; a KS tile
-// is transposed on its way out of LDS (ds_read_tr).  The k range may be a chain of up to 12 segments, each with base pointers of its
-// own: the two terms of dx = dg Wg + du Wu, and the six products of fp32 operands that were split into three bf16 terms.
+// is transposed on its way out of LDS (ds_read_tr).  A product may have up to 12 terms, each
+// over all of k with operands of its own: the two of dx = dg Wg + du Wu, times the six of fp32 operands split into three bf16 planes.
 //
 // A workgroup owns a BM x BN tile and walks k in steps of GEMM_BK: two LDS stages (three of the smallest tile), filled by buffer loads that write LDS directly (16 bytes
 // per lane, rows and columns out of range are bounds-checked to zero by the buffer resource), one barrier per step.  The LDS image
@@ -160,14 +160,13 @@ __device__ __forceinline__ void from_lds(const char DM_LDS* p, float (&v)[8]) {
 }
 
 constexpr int LDS_BIAS = 3072;  // see load_to_lds
-constexpr int GEMM_MAX_SEGMENTS = 12;
 enum { EPI_STORE, EPI_GATE, EPI_GATE_F32, EPI_DACT, EPI_DACT_F32 };  // _F32: of split fp32 operands
 
 struct GemmArgs {
-  const void* a[GEMM_MAX_SEGMENTS];
-  const void* b[GEMM_MAX_SEGMENTS];
-  const void* b2[GEMM_MAX_SEGMENTS];  // EPI_GATE: the second projection's weights
-  int segments, iters;                // iters: k steps of GEMM_BK per segment
+  const void *a[2], *b[2], *b2;       // b2 (GATE): the second projection's weights
+  int64_t plane_a, plane_b;           // bytes from one plane of an operand to the next
+  uint64_t terms;                     // five bits per product term: plane of a, plane of b (two bits each), which of the two a and b
+  int segments, iters;                // number of terms, k steps of GEMM_BK
   int64_t lda, ldb;                   // elements
   int64_t M;
   int N, K;                           // N: of one projection for EPI_GATE.  K: true length; a KC row is zero from there to the end of its piece
@@ -180,8 +179,9 @@ struct GemmArgs {
   int act;
   void* part;                         // splits > 1: fp32 partial products (GATE: of both projections in turn), rows of ldpart,
   int64_t split_stride, ldpart;       // split_stride elements from one to the next; joined by a second launch
-  void* sums;                         // STORE with both operands KS: sum over k of A[m, k] over the segments of sum_segments, or null.  One split:
-  int sum_segments, sums_f32;         // of the type that sums_f32 gives; several: fp32, M apart
+  void* sums;                         // STORE with both operands KS: sum over k of A[m, k] over the segments of sum_segments, of the result's type,
+  float* sum_part;                    // or null; splits > 1: their parts, M apart
+  int sum_segments;
 };
 
 // Where a stage keeps a piece of 16 bytes.  KS (one LDS row per k, R columns): piece c of row k lies at c ^ ks_key(k), so that the 32
@@ -236,6 +236,9 @@ __device__ __forceinline__ i32x4 buffer_of(const void* p) {
 template <int LEFT>
 __device__ __forceinline__ void stage_arrived() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
 
+// Every wave's LDS accesses so far are done; loads and stores of global memory stay under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Fragment of 16 rows x 32 k (the s-th of the step) out of a stage: lane l holds row l & 15, k 8 (l >> 4) .. +7.
 template <int R, bool KS>
 __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, int tile, int s) {
@@ -255,12 +258,19 @@ __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, in
   }
 }
 
+// Steps of each part of a split k range: whole eights where it has two or more (see `shift` below).
+__host__ __device__ inline int split_steps(int iters, int splits) {
+  const int per = (iters + splits - 1) / splits;
+  return per < 16 ? per : (per + 7) / 8 * 8;
+}
+
 template <typename T, int BM, int BN, int WM, int WN, int GEMM_STAGES, bool AKS, bool BKS, int EPI>
 __global__ void __launch_bounds__(WM * WN * 64, 2)
 gemm_kernel(const GemmArgs p) {
   constexpr int NW = WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
   constexpr int ABYTES = BM * GEMM_BK * 2, STAGE = (BM + BN) * GEMM_BK * 2;
-  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
+  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32,
+                 DACT = EPI == EPI_DACT || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
   using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
   constexpr int XS = MI >= WN ? MI / WN : 1;  // the waves of a tile row share its sums of A: XS blocks of 16 rows each
@@ -284,44 +294,40 @@ gemm_kernel(const GemmArgs p) {
   const int64_t m0 = (int64_t)tm * BM;
   const int n0 = tn * (GATE ? BN / 2 : BN);
 
-  const int total = p.segments * p.iters;
-  const int per = ((total + p.splits - 1) / p.splits + 7) / 8 * 8;  // whole eights: see `place`
-  const int it0 = blockIdx.y * per, it1 = it0 + per < total ? it0 + per : total;
+  // The block's range: k steps, every term of the product in each (an operand's tile is then still in the L2 for its other terms).
+  const int per = split_steps(p.iters, p.splits);
+  const int step0 = blockIdx.y * per, step1 = step0 + per < p.iters ? step0 + per : p.iters;
+  const int turns = step0 < step1 ? (step1 - step0) * p.segments : 0;
 
   Stager<BM, AKS, NW> sa;
   Stager<BN, BKS, NW> sb;
   sa.template init<false>(wave, lane, p.lda, p.M - m0);
   sb.template init<GATE>(wave, lane, p.ldb, p.N - n0);
 
-  // (the segments' pointers are read where the launch put the arguments: indexing the parameter itself would copy it to scratch)
-  const auto* args = (const __attribute__((address_space(4))) GemmArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
-  // Steps are taken in an order of the tile's own within each eight of a segment: the blocks of an XCD would otherwise ask for the same
-  // columns of all rows at once, which lie on few of the L2's channels when rows are a power of two apart.  An eight that the block's
-  // range or the segment does not hold whole keeps its order (several segments of no whole eights: all of them).
-  const int shift = p.segments > 1 && p.iters % 8 ? 0 : (tm + 2 * tn) & 7;
-  int seg = it0 / p.iters, step = it0 - seg * p.iters;  // of the next stage to be asked for
-  const int whole = p.segments > 1 ? p.iters : it1;     // the end of the segment's steps in this range
+  // Steps are taken in an order of the tile's own within each eight: the blocks of an XCD would otherwise ask for the same columns of all
+  // rows at once, which lie on few of the L2's channels when rows are a power of two apart.  (Eights that the range does not hold whole
+  // keep their order.)
+  const int shift = per % 8 && p.splits > 1 ? 0 : (tm + 2 * tn) & 7;
+  int seg = 0, step = step0;  // of the next stage to be asked for
   const int64_t astep = (AKS ? p.lda : 1) * GEMM_BK * 2, bstep = (BKS ? p.ldb : 1) * GEMM_BK * 2;  // bytes from one step to the next
   const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2;
-  const char *sega = (const char*)args->a[seg] + a0, *segb = (const char*)args->b[seg] + b0;  // the corners of the segment at hand
-  const char* segb2 = GATE ? (const char*)args->b2[seg] + b0 : nullptr;
   constexpr int LOADS = sa.PASSES + sb.PASSES;
   struct Request { i32x4 a, b, b2; int left; bool sum; };
-  auto request = [&](int it) __attribute__((always_inline)) {  // what the loads of the range's it-th step have in common
-    const int at = (step | 7) < whole ? step ^ shift : step;
+  auto request = [&](int turn) __attribute__((always_inline)) {  // what the loads of the range's turn-th stage have in common
+    const int at = (step | 7) < step1 ? step ^ shift : step;
+    const int term = (int)(p.terms >> 5 * seg) & 31;
+    const char* a = (const char*)(term & 16 ? p.a[1] : p.a[0]) + (term & 3) * p.plane_a;
+    const int64_t b = (term >> 2 & 3) * p.plane_b + b0 + at * bstep;
     Request r;
-    r.a = buffer_of(sega + at * astep);
-    r.b = buffer_of(segb + at * bstep);
-    r.b2 = GATE ? buffer_of(segb2 + at * bstep) : r.b;
-    r.left = it < it1 ? p.K - at * GEMM_BK : 0;  // behind the range every piece lies outside
-    r.sum = SUMS && it < it1 && (p.sum_segments >> seg & 1);
-    if (++step == p.iters && seg + 1 < p.segments) {
-      step = 0;
-      ++seg;
-      sega = (const char*)args->a[seg] + a0;
-      segb = (const char*)args->b[seg] + b0;
-      if (GATE) segb2 = (const char*)args->b2[seg] + b0;
+    r.a = buffer_of(a + a0 + at * astep);
+    r.b = buffer_of((const char*)(term & 16 ? p.b[1] : p.b[0]) + b);
+    r.b2 = GATE ? buffer_of((const char*)p.b2 + b) : r.b;
+    r.left = turn < turns ? p.K - at * GEMM_BK : 0;  // behind the range every piece lies outside
+    r.sum = SUMS && turn < turns && (p.sum_segments >> seg & 1);
+    if (++seg == p.segments) {
+      seg = 0;
+      ++step;
     }
     return r;
   };
@@ -388,12 +394,12 @@ gemm_kernel(const GemmArgs p) {
       for (int x = 0; x < XS; ++x) asum[x] = mfma16(ones, fragment<BM, AKS>(st, lane, wm * MI + wn * XS + x, s), asum[x], T());
   };
   const bool sums = SUMS && p.sums && tn == 0;
-  if (it0 < it1) {
+  if (turns) {
     uint32_t cur = 0;
     bool sum = false, next[GEMM_STAGES];  // do the stage at hand, and those asked for, count for the sums of A
 #pragma unroll
     for (int k = 0; k < GEMM_STAGES; ++k) {
-      const Request r = request(it0 + k);
+      const Request r = request(k);
       next[k] = sums && r.sum;
       load(r, k * STAGE, 0, LOADS / 2);
     }
@@ -401,8 +407,8 @@ gemm_kernel(const GemmArgs p) {
     sum = next[0];
 #pragma unroll
     for (int l = 0; l < READS; ++l) read(0, 0, 0, l);
-    for (int it = it0; it < it1; ++it) {
-      const Request r = request(it + GEMM_STAGES);
+    for (int turn = 0; turn < turns; ++turn) {
+      const Request r = request(turn + GEMM_STAGES);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < PARTS - 1; ++s) part(s & 1, cur, s + 1, false, r, 0);
@@ -426,6 +432,16 @@ gemm_kernel(const GemmArgs p) {
   // on few of the L2's channels (41 us of a 256 x 256 tile's time, measured at a row of 8 KB).
   constexpr int ROWS = WM * 32, PITCH = BN * 4 + 16, COLS = GATE ? BN / 2 : BN, PIECES = COLS / 8, TASKS = ROWS * PIECES / (NW * 64);
   const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces (with zeros: rows of B out of range are zero)
+  static_assert(NW * 64 % PIECES == 0, "a thread keeps its columns");
+  float b1[8], b2[8];
+  if constexpr (!DACT) {
+    const int n = n0 + threadIdx.x % PIECES * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      b1[e] = EPI == EPI_STORE && p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<Kept>(p.bias, n + e, p.N);
+      b2[e] = GATE ? bias_at<Kept>(p.bias2, n + e, p.N) : 0.f;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < MI / 2; ++i) {
     char DM_LDS* buf = (char DM_LDS*)smem + (i & 1) * ROWS * PITCH;
@@ -434,7 +450,30 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
       for (int j = 0; j < NI; ++j)
         *(DM_LDS f32x4*)(buf + (wm * 32 + h * 16 + (lane & 15)) * PITCH + ((wn * NI + j) * 16 + (lane >> 4) * 4) * 4) = acc[i * 2 + h][j];
-    __syncthreads();
+    Vec<Kept, 8> ug[DACT ? TASKS : 1], ag[DACT ? TASKS : 1];  // asked for ahead of the barrier
+    if constexpr (DACT) {
+#pragma unroll
+      for (int t = 0; t < TASKS; ++t) {
+        const int id = t * NW * 64 + threadIdx.x, row = id / PIECES, n = n0 + id % PIECES * 8;
+        const int64_t m = m0 + row / 32 * (MI * 16) + i * 32 + row % 32;
+        if (m >= p.M || n >= np || p.splits > 1) continue;
+        ug[t] = *reinterpret_cast<const Vec<Kept, 8>*>((const Kept*)p.ug + m * p.ldg + n);
+        ag[t] = *reinterpret_cast<const Vec<Kept, 8>*>((const Kept*)p.ag + m * p.ldg + n);
+      }
+    }
+    lds_barrier();
+    if (EPI == EPI_STORE && p.splits == 1 && !p.out.vec) {  // rows off 16-byte boundaries: neighbouring lanes store neighbouring elements
+#pragma unroll 8
+      for (int id = threadIdx.x; id < ROWS * BN; id += NW * 64) {
+        const int row = id / BN, n = n0 + id % BN;
+        const int64_t m = m0 + row / 32 * (MI * 16) + i * 32 + row % 32;
+        if (m >= p.M || n >= p.N) continue;
+        const float v = *(const DM_LDS float*)(buf + row * PITCH + id % BN * 4);
+        if (p.out.f32) ((float*)p.out.p)[m * p.out.ld + n] = v + bias_at<float>(p.bias, n, p.N);
+        else ((T*)p.out.p)[m * p.out.ld + n] = (T)(v + bias_at<T>(p.bias, n, p.N));
+      }
+      continue;
+    }
 #pragma unroll
     for (int t = 0; t < TASKS; ++t) {
       const int id = t * NW * 64 + threadIdx.x, row = id / PIECES, col = id % PIECES * 8;
@@ -442,39 +481,31 @@ gemm_kernel(const GemmArgs p) {
       const int n = n0 + col;
       if (m >= p.M || n >= (EPI == EPI_STORE ? p.N : np)) continue;
       const char DM_LDS* at = buf + row * PITCH + (GATE ? col / 32 * 64 + col % 32 : col) * 4;
-      float v[8];
+      float v[8], u[8], h[8];
       from_lds(at, v);
+      if constexpr (GATE) from_lds(at + 128, u);
+      if (p.splits > 1) {  // joined by a second launch
+        float* part = (float*)p.part + blockIdx.y * (GATE ? 2 : 1) * p.split_stride + m * p.ldpart + n;
+        store_f32(part, v);
+        if constexpr (GATE) store_f32(part + p.split_stride, u);
+        continue;
+      }
       if constexpr (GATE) {
-        float u[8], h[8];
-        from_lds(at + 128, u);
-        if (p.splits > 1) {  // finished by gate_join_kernel
-          float* part = (float*)p.part + 2 * blockIdx.y * p.split_stride + m * p.ldpart + n;
-          store_f32(part, v);
-          store_f32(part + p.split_stride, u);
-          continue;
-        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] += bias_at<Kept>(p.bias, n + e, p.N);
-          u[e] += bias_at<Kept>(p.bias2, n + e, p.N);
-        }
+        for (int e = 0; e < 8; ++e) { v[e] += b1[e]; u[e] += b2[e]; }
         gate_values<!F32>(p.act, v, u, h);
         store8<T, BETWEEN>(p.out, m, n, np, h);
         if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
-      } else if constexpr (EPI == EPI_STORE) {
+      } else if constexpr (DACT) {
 #pragma unroll
-        for (int e = 0; e < 8 && p.splits == 1; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
-        if (p.splits > 1) store_f32((float*)p.part + blockIdx.y * p.split_stride + m * p.ldpart + n, v);
-        else if (p.out.f32) store8<T, OUT_F32>(p.out, m, n, p.N, v);
-        else store8<T, OUT_16>(p.out, m, n, p.N, v);
+        for (int e = 0; e < 8; ++e) { u[e] = v[e] * (float)ug[t].v[e]; h[e] = v[e] * (float)ag[t].v[e]; }
+        store8<T, BETWEEN>(p.out, m, n, np, u);
+        store8<T, BETWEEN>(p.out2, m, n, np, h);
       } else {
-        float ug[8], ag[8];
-        load8((const Kept*)p.ug + m * p.ldg + n, ug);
-        load8((const Kept*)p.ag + m * p.ldg + n, ag);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { ug[e] *= v[e]; ag[e] *= v[e]; }
-        store8<T, BETWEEN>(p.out, m, n, np, ug);
-        store8<T, BETWEEN>(p.out2, m, n, np, ag);
+        for (int e = 0; e < 8; ++e) v[e] += b1[e];
+        if (p.out.f32) store8<T, OUT_F32>(p.out, m, n, p.N, v);
+        else store8<T, OUT_16>(p.out, m, n, p.N, v);
       }
     }
   }
@@ -484,69 +515,87 @@ gemm_kernel(const GemmArgs p) {
       for (int x = 0; x < XS; ++x) {
         const int64_t m = m0 + (wm * MI + wn * XS + x) * 16 + lane;
         if (!p.sums || tn || lane >= 16 || m >= p.M) continue;
-        if (p.splits > 1) ((float*)p.sums)[blockIdx.y * p.M + m] = asum[x][0];
-        else if (p.sums_f32) ((float*)p.sums)[m] = asum[x][0];
+        if (p.splits > 1) p.sum_part[blockIdx.y * p.M + m] = asum[x][0];
+        else if (p.out.f32) ((float*)p.sums)[m] = asum[x][0];
         else ((T*)p.sums)[m] = (T)asum[x][0];
       }
     }
   }
 }
 
-// Adds the partial products of a split k range (and the partial sums of A), the bias, and rounds once.
-template <typename T>
-__global__ void __launch_bounds__(256)
-gemm_join_kernel(const float* __restrict__ part, int splits, int64_t stride, const void* bias, const Out out, int64_t M, int N, int ldp,
-                 const float* __restrict__ sum_part, void* sums) {
-  const int pieces = ldp / 8;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < M * pieces; id += (int64_t)gridDim.x * 256) {
-    const int64_t m = id / pieces;
-    const int n = (int)(id % pieces) * 8;
-    float v[8] = {};
+// Eight columns' sums over the partial products of a split k range: four groups of 64 threads take every fourth of them and meet in LDS,
+// in a fixed order.  Threads of the first group get the result.
+__device__ __forceinline__ bool join8(const float* part, int splits, int64_t stride, bool live, float (&v)[8]) {
+  __shared__ float sum[3][64][9];
+  const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  if (live)
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
+    for (int s = group; s < splits; s += 4) {
       float w[8];
-      load8(part + s * stride + m * ldp + n, w);
+      load8(part + s * stride, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
+  __syncthreads();
+  if (group)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += out.f32 ? bias_at<float>(bias, n + e, N) : bias_at<T>(bias, n + e, N);
-    if (out.f32) store8<T, OUT_F32>(out, m, n, N, v);
-    else store8<T, OUT_16>(out, m, n, N, v);
-  }
-  if (!sums) return;
-  for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < M; m += (int64_t)gridDim.x * 256) {
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += sum_part[s * M + m];
-    if (out.f32) ((float*)sums)[m] = v;
-    else ((T*)sums)[m] = (T)v;
-  }
+    for (int e = 0; e < 8; ++e) sum[group - 1][lane][e] = v[e];
+  __syncthreads();
+  if (group) return false;
+#pragma unroll
+  for (int g = 0; g < 3; ++g)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += sum[g][lane][e];
+  return live;
 }
 
-// The same for the gated product: bias, activation and product of the joined projections.
-template <typename T, bool F32>
-__global__ void __launch_bounds__(256) gate_join_kernel(const GemmArgs p) {
+// The second launch of a product whose k range was split: partial products added, then what the epilogue would have done.
+template <typename T, int EPI>
+__global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
+  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32;
   using Kept = typename std::conditional<F32, float, T>::type;
+  constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
   const int np = (p.N + 7) & ~7, pieces = np / 8;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < p.M * pieces; id += (int64_t)gridDim.x * 256) {
-    const int64_t m = id / pieces;
+  const int64_t all = p.M * pieces;
+  for (int64_t base = (int64_t)blockIdx.x * 64; base < all; base += (int64_t)gridDim.x * 64) {
+    const int64_t id = base + (threadIdx.x & 63), m = id / pieces;
     const int n = (int)(id % pieces) * 8;
     const float* part = (const float*)p.part + m * p.ldpart + n;
-    float g[8] = {}, u[8] = {}, h[8];
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      float a[8], b[8];
-      load8(part + 2 * s * p.split_stride, a);
-      load8(part + (2 * s + 1) * p.split_stride, b);
+    float v[8], u[8], h[8];
+    const bool mine = join8(part, p.splits, (GATE ? 2 : 1) * p.split_stride, id < all, v);
+    if constexpr (GATE) join8(part + p.split_stride, p.splits, 2 * p.split_stride, id < all, u);
+    if (!mine) continue;
+    if constexpr (GATE) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { g[e] += a[e]; u[e] += b[e]; }
+      for (int e = 0; e < 8; ++e) { v[e] += bias_at<Kept>(p.bias, n + e, p.N); u[e] += bias_at<Kept>(p.bias2, n + e, p.N); }
+      gate_values<!F32>(p.act, v, u, h);
+      store8<T, BETWEEN>(p.out, m, n, np, h);
+      if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
+    } else if constexpr (EPI == EPI_STORE) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
+      if (p.out.f32) store8<T, OUT_F32>(p.out, m, n, p.N, v);
+      else store8<T, OUT_16>(p.out, m, n, p.N, v);
+    } else {
+      float ag[8];
+      load8((const Kept*)p.ug + m * p.ldg + n, u);
+      load8((const Kept*)p.ag + m * p.ldg + n, ag);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { u[e] *= v[e]; h[e] = ag[e] * v[e]; }
+      store8<T, BETWEEN>(p.out, m, n, np, u);
+      store8<T, BETWEEN>(p.out2, m, n, np, h);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { g[e] += bias_at<Kept>(p.bias, n + e, p.N); u[e] += bias_at<Kept>(p.bias2, n + e, p.N); }
-    gate_values<!F32>(p.act, g, u, h);
-    store8<T, F32 ? OUT_PLANES : OUT_16>(p.out, m, n, np, h);
-    if (p.out2.p) { store8<T, F32 ? OUT_F32 : OUT_16>(p.out2, m, n, np, u); store8<T, F32 ? OUT_F32 : OUT_16>(p.out3, m, n, np, g); }
   }
+  if (EPI == EPI_STORE && p.sums)
+    for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < p.M; m += (int64_t)gridDim.x * 256) {
+      float s = 0.f;
+#pragma unroll 16
+      for (int i = 0; i < p.splits; ++i) s += p.sum_part[i * p.M + m];
+      if (p.out.f32) ((float*)p.sums)[m] = s;
+      else ((T*)p.sums)[m] = (T)s;
+    }
 }
 
 // Tiles.  WIDE, 256 x 256: one workgroup of 8 waves per CU; the fewest bytes and LDS reads per product.  MID, 128 x 128: two of 4 waves per
@@ -556,26 +605,30 @@ constexpr int TILE_M[TILES] = {256, 128, 64}, TILE_N[TILES] = {256, 128, 128}, T
 
 struct GemmPlan { int tile, splits; size_t part_bytes; };
 
-// Tile and split of the k range.  Estimated in microseconds: rounds of workgroups over the chip, each of its k steps (measured: 1.6 us a
-// step of a WIDE tile, 1.2 and 0.8 us of two MID or SLIM tiles on a CU) and a start and an end; not less than the bytes of the n side at
-// 5.5 TB/s; and, where the k range is split to fill the chip, the joining launch.  `outs`: products per n (2: both projections).
-inline GemmPlan gemm_plan(int64_t M, int N, int iters, int outs, bool can_split, bool slim) {
+// Tile and split of the k range: the least of an estimate in microseconds.  A product's time is that of its stages - alone on a CU, or two
+// workgroups to a CU where they fit (WIDE: two rounds) - but not less than the n side's bytes take, then for each round of workgroups
+// a start and the tile's results on their way (`bytes` per element of the tile), and for a split k range the joining launch.  The
+// constants are fitted to the measured times of every tile and split at 52 sizes of the block (6 to 65536 rows, widths 64 to 11008,
+// bf16 and fp32, all products of both passes): what it picks takes 2 % longer than the best on average, 42 % at worst (products of
+// 10 us), where always taking MID unsplit would take 50 % longer.  `outs`: products per n (2: both projections).
+inline GemmPlan gemm_plan(int64_t M, int N, int steps, int terms, int outs, int bytes, bool slim) {
   const int cus = 256;
-  constexpr double STEP[TILES] = {1.6, 1.2, 0.8};
+  constexpr double ALONE[TILES] = {1.8, 1.55, 0.6}, PAIR[TILES] = {5.1, 1.3, 0.9}, START[TILES] = {1.7, 1.9, 1.5};
   GemmPlan best = {TILE_MID, 1, 0};
   double cost = 1e300;
+  const double stream = (double)N * outs * steps * (terms > 1 ? 3 : 1) * GEMM_BK * 2 / 7.8e6;
   for (int t = 0; t < TILES; ++t) {
     if (t == TILE_SLIM && !slim) continue;
     const int64_t tiles = ((M + TILE_M[t] - 1) / TILE_M[t]) * (((int64_t)N * outs + TILE_N[t] - 1) / TILE_N[t]);
-    const int slots = cus * TILE_PER_CU[t];
-    for (int s = 1; s <= 64; s *= 2) {
-      if (s > 1 && (!can_split || s * 8 > iters || tiles * (s / 2) >= slots)) break;
-      const double rounds = (double)((tiles * s + slots - 1) / slots);
-      const double fill = tiles * s < slots / 2 && TILE_PER_CU[t] > 1 ? 0.6 : 1.0;  // alone on its CU a workgroup is faster
-      double c = rounds * (((iters + s - 1) / s) * STEP[t] * fill + 4.0);
-      const double stream = (double)N * outs * iters * GEMM_BK * 2 / 5.5e6;
+    for (int want = 1; want <= 64; want *= 2) {
+      const int s = (steps + split_steps(steps, want) - 1) / split_steps(steps, want), per = split_steps(steps, s);
+      if (want > 1 && (s <= want / 2 || per * terms < 4 || tiles * (want / 2) >= cus)) break;
+      const int64_t blocks = tiles * s, full = blocks / (2 * cus), rest = blocks % (2 * cus);
+      const double alone = blocks <= cus / 2 ? 1.4 * ALONE[t] : ALONE[t];
+      double c = per * terms * (full * PAIR[t] + (rest > cus ? PAIR[t] : rest ? alone : 0.0));
       if (c < stream) c = stream;
-      if (s > 1) c += 3.0 + (double)M * N * outs * 4 * 2 * s / 5.0e6;
+      c += (double)((blocks + cus - 1) / cus) * (START[t] + TILE_M[t] * TILE_N[t] * (s > 1 ? 4 : bytes) / 18.0e3);
+      if (s > 1) c += 11.5 + (double)M * N * outs * 4 * s / 2.4e6;
       if (c < cost) { cost = c; best.tile = t; best.splits = s; }
     }
   }
@@ -596,7 +649,7 @@ inline hipError_t allow_lds(const void* f, int bytes, std::atomic<uint64_t>& don
 
 template <typename T, bool AKS, bool BKS, int EPI>
 int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
-  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, SLIM = !AKS && (EPI == EPI_STORE || GATE);
+  constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, SLIM = !AKS;
   const int bm = TILE_M[tile], bn = TILE_N[tile];
   a.tiles_m = (int)((a.M + bm - 1) / bm);
   a.tiles_n = GATE ? (a.N + bn / 2 - 1) / (bn / 2) : (a.N + bn - 1) / bn;
@@ -621,9 +674,9 @@ int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
     void* args[] = {&a};
     e = hipLaunchKernel(f, grid, dim3(tile == TILE_WIDE ? 512 : 256), args, bytes, st);
   }
-  if (e == hipSuccess && GATE && a.splits > 1) {  // (a.splits is 1 elsewhere: product joins its own)
-    const int64_t blocks = (a.M * ((a.N + 7) / 8) + 255) / 256;
-    gate_join_kernel<T, EPI == EPI_GATE_F32><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
+  if (e == hipSuccess && a.splits > 1) {
+    const int64_t blocks = (a.M * ((a.N + 7) / 8) + 63) / 64;
+    join_kernel<T, EPI><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
     e = hipGetLastError();
   }
   return e == hipSuccess ? 0 : fail("gated feed-forward block: launch failed: %s", hipGetErrorString(e));
