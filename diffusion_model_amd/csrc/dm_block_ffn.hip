@@ -351,8 +351,8 @@ Operand take_operand(int64_t rows, int cols, Carver& ws) {
 template <typename T>
 void add_terms(GemmArgs& g, const Operand& a, const Operand& b, bool second = false) {
   auto add = [&](uint64_t i, uint64_t j) { g.terms |= (i | j << 2 | (second ? 16 : 0)) << 5 * g.segments++; };
-  if (std::is_same<T, float>::value) { add(0, 2); add(2, 0); add(1, 1); add(0, 1); add(1, 0); }  // small terms first
   add(0, 0);
+  if (std::is_same<T, float>::value) { add(0, 1); add(1, 0); add(0, 2); add(2, 0); add(1, 1); }  // (no two plane tiles new at once but the first)
   g.a[second] = a.p;
   g.b[second] = b.p;
   g.lda = a.ld;
@@ -389,7 +389,7 @@ int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part
   g.bias = bias;
   g.sums = sums;
   g.sum_part = (float*)part + g.splits * g.split_stride;
-  g.sum_segments = std::is_same<T, float>::value ? 1 << 1 | 1 << 4 | 1 << 5 : 1;  // add_terms: each plane of A once
+  g.sum_segments = std::is_same<T, float>::value ? 1 << 0 | 1 << 2 | 1 << 4 : 1;  // add_terms: each plane of A once
   return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, tile, st);
 }
 

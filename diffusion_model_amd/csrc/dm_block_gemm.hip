@@ -159,7 +159,8 @@ __device__ __forceinline__ void from_lds(const char DM_LDS* p, float (&v)[8]) {
   for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
 }
 
-constexpr int LDS_BIAS = 3072;  // see load_to_lds
+constexpr int LDS_BIAS = 3 * 1024;  // see load_to_lds
+constexpr uint32_t UNBOUNDED = 0x80000000u, OUTSIDE = 0x80000000u;  // bytes of a buffer; an offset outside of every one
 enum { EPI_STORE, EPI_GATE, EPI_GATE_F32, EPI_DACT, EPI_DACT_F32 };  // _F32: of split fp32 operands
 
 struct GemmArgs {
@@ -196,7 +197,7 @@ struct Stager {
   static constexpr int PASSES = R * GEMM_BK / 8 / (64 * NW);  // 16-byte pieces per lane
   static constexpr int CPR = KS ? R / 8 : GEMM_BK / 8;        // pieces per LDS row
   static constexpr int RPW = 64 / CPR;                        // LDS rows that one wave's load fills
-  uint32_t off[PASSES];                                       // byte offset from the tile's corner, 2^31 where the piece lies outside
+  uint32_t off[PASSES];                                       // byte offset from LDS_BIAS before the tile's corner, OUTSIDE where the piece lies outside
   static __device__ __forceinline__ int row_of(int wave, int lane, int j) { return (wave * PASSES + j) * RPW + lane / CPR; }
   static __device__ __forceinline__ int piece_of(int lane, int row) { return (lane % CPR) ^ (KS ? ks_key(row) : kc_key(row)); }
   static __device__ __forceinline__ int k_of(int wave, int lane, int j) {  // k of the piece within the step
@@ -211,7 +212,7 @@ struct Stager {
       const int row = row_of(wave, lane, j), c = piece_of(lane, row);
       const uint32_t bias = LDS_BIAS - j % 4 * 1024;  // see load_to_lds
       const int r = GATE ? row / 64 * 32 + row % 32 : row;
-      off[j] = (KS ? c * 8 : r) < rows_left ? (uint32_t)(r * ld * 2 + c * 16) + bias : 0x80000000u;
+      off[j] = (KS ? c * 8 : r) < rows_left ? (uint32_t)(r * ld * 2 + c * 16) + bias : OUTSIDE;
     }
   }
 };
@@ -228,10 +229,18 @@ __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off0, uint32_t 
       "v"(off1), "s"(rsrc), "s"(lds), "n"(FIRST), "n"(FIRST + 1024)
       : "memory");
 }
-__device__ __forceinline__ i32x4 buffer_of(const void* p) {
-  const uint64_t u = (uint64_t)p - LDS_BIAS;
-  return i32x4{(int)(uint32_t)u, (int)(uint32_t)(u >> 32), (int)0x80000000u, 0x00020000};  // (addresses have 48 bits: no stride)
+// (addresses have 48 bits: no stride)
+__device__ __forceinline__ i32x4 buffer_of(uint64_t u, uint32_t bytes) {
+  return i32x4{(int)(uint32_t)u, (int)(uint32_t)(u >> 32), (int)bytes, 0x00020000};
 }
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+// The value, in scalar registers, is formed here: neither sunk to where it is used nor loaded again there.
+template <typename V>
+__device__ __forceinline__ void pin(V& v) { asm volatile("" : "+s"(v)); }
+__device__ __forceinline__ uint64_t product64(uint32_t a, uint32_t b) { return (uint64_t)__umulhi(a, b) << 32 | a * b; }  // (in scalar registers)
+
 // All but the LEFT newest loads of every wave are in LDS, and every wave has its fragments of the stage at hand in registers.
 template <int LEFT>
 __device__ __forceinline__ void stage_arrived() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
@@ -243,14 +252,14 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 template <int R, bool KS>
 __device__ __forceinline__ s16x8 fragment(const char DM_LDS* stage, int lane, int tile, int s) {
   if constexpr (KS) {
-    // A lane asks for 4 consecutive rows of one k; of 16 lanes' answers, lane i receives row i of four k.
-    const int k0 = s * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3), piece = tile * 2 + ((lane >> 1) & 1);
+    // A lane asks for 4 consecutive rows of one k; of 16 lanes' answers, lane i receives row i of four k.  (k's bits 2 and 5 are not in
+    // its key, and the stage and k lie above the bits of the tile: one exclusive or per fragment, the rest in the instructions' offsets.)
+    const int k0 = (lane >> 4) * 8 + ((lane >> 2) & 3);
+    const uint32_t at = ((uint32_t)(uintptr_t)stage + k0 * (R * 2) + (((lane >> 1) & 1) ^ ks_key(k0)) * 16 + (lane & 1) * 8) ^ tile * 32;
     s16x4 h[2];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int k = k0 + q * 4;
-      h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DM_LDS s16x4*)(stage + k * (R * 2) + (piece ^ ks_key(k)) * 16 + (lane & 1) * 8));
-    }
+    for (int q = 0; q < 2; ++q)
+      h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DM_LDS s16x4*)(uintptr_t)(at + (s * 32 + q * 4) * (R * 2)));
     return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
   } else {
     const int row = tile * 16 + (lane & 15);
@@ -274,7 +283,7 @@ gemm_kernel(const GemmArgs p) {
   using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
   constexpr int XS = MI >= WN ? MI / WN : 1;  // the waves of a tile row share its sums of A: XS blocks of 16 rows each
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -294,7 +303,7 @@ gemm_kernel(const GemmArgs p) {
   const int64_t m0 = (int64_t)tm * BM;
   const int n0 = tn * (GATE ? BN / 2 : BN);
 
-  // The block's range: k steps, every term of the product in each (an operand's tile is then still in the L2 for its other terms).
+  // The block's range: k steps, and every term of the product in each.
   const int per = split_steps(p.iters, p.splits);
   const int step0 = blockIdx.y * per, step1 = step0 + per < p.iters ? step0 + per : p.iters;
   const int turns = step0 < step1 ? (step1 - step0) * p.segments : 0;
@@ -307,29 +316,86 @@ gemm_kernel(const GemmArgs p) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)(DM_LDS char*)smem;
   // Steps are taken in an order of the tile's own within each eight: the blocks of an XCD would otherwise ask for the same columns of all
   // rows at once, which lie on few of the L2's channels when rows are a power of two apart.  (Eights that the range does not hold whole
-  // keep their order.)
-  const int shift = per % 8 && p.splits > 1 ? 0 : (tm + 2 * tn) & 7;
-  int seg = 0, step = step0;  // of the next stage to be asked for
-  const int64_t astep = (AKS ? p.lda : 1) * GEMM_BK * 2, bstep = (BKS ? p.ldb : 1) * GEMM_BK * 2;  // bytes from one step to the next
-  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2;
+  // keep their order, and so does the one with a step of fewer k: that step comes last.)
+  const int shift = per % 8 && p.splits > 1 ? 0 : (tm + 2 * tn) & (p.segments > 1 && !(AKS && p.splits > 1) ? 3 : 7);
+  const int whole = p.K / GEMM_BK < step1 ? p.K / GEMM_BK : step1;
+  // A term takes a group of steps, then the next term takes the same group (the last step, if it has fewer k, is one by itself).
+  const int group = p.segments > 1 ? AKS && p.splits > 1 ? 1 : 4 : p.iters;
+  auto group_end = [&](int from) __attribute__((always_inline)) { return from >= whole ? step1 : from + group < whole ? from + group : whole; };
+  int seg = 0, step = step0, group0 = step0, group1 = group_end(step0);  // of the next stage to be asked for
+  bool moved = false;
+  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2 - LDS_BIAS, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2 - LDS_BIAS;
   constexpr int LOADS = sa.PASSES + sb.PASSES;
-  struct Request { i32x4 a, b, b2; int left; bool sum; };
-  auto request = [&](int turn) __attribute__((always_inline)) {  // what the loads of the range's turn-th stage have in common
-    const int at = (step | 7) < step1 ? step ^ shift : step;
-    const int term = (int)(p.terms >> 5 * seg) & 31;
-    const char* a = (const char*)(term & 16 ? p.a[1] : p.a[0]) + (term & 3) * p.plane_a;
-    const int64_t b = (term >> 2 & 3) * p.plane_b + b0 + at * bstep;
-    Request r;
-    r.a = buffer_of(a + a0 + at * astep);
-    r.b = buffer_of((const char*)(term & 16 ? p.b[1] : p.b[0]) + b);
-    r.b2 = GATE ? buffer_of((const char*)p.b2 + b) : r.b;
-    r.left = turn < turns ? p.K - at * GEMM_BK : 0;  // behind the range every piece lies outside
-    r.sum = SUMS && turn < turns && (p.sum_segments >> seg & 1);
-    if (++seg == p.segments) {
-      seg = 0;
-      ++step;
+  // (kept in registers: a scalar load among the products would wait for every LDS read under way)
+  int segments = p.segments, k_end = p.K, sum_segments = p.sum_segments;
+  uint32_t lda2 = (uint32_t)p.lda * 2, ldb2 = (uint32_t)p.ldb * 2;  // bytes
+  pin(segments), pin(k_end), pin(lda2), pin(ldb2);
+  const uint32_t astep = (AKS ? lda2 : 2) * GEMM_BK, bstep = (BKS ? ldb2 : 2) * GEMM_BK;  // bytes from one step to the next
+  uint64_t corners[3];  // lane i: the corners of the i-th term's operands (GATE: and of the second projection's weights)
+  {
+    const int term = (int)(p.terms >> 5 * (lane < 12 ? lane : 0)) & 31;
+    const int64_t in_b = (term >> 2 & 3) * p.plane_b;
+    corners[0] = (uint64_t)(!GATE && term & 16 ? p.a[1] : p.a[0]) + a0 + (term & 3) * p.plane_a;
+    corners[1] = (uint64_t)(!GATE && term & 16 ? p.b[1] : p.b[0]) + b0 + in_b;
+    corners[2] = GATE ? (uint64_t)p.b2 + b0 + in_b : 0;
+  }
+  uint64_t term_a, term_b, term_b2 = 0;  // of the term at hand
+  auto take_term = [&](int piece) __attribute__((always_inline)) {
+    if (piece == 0) {
+      term_a = from_lane(corners[0], seg);
+    } else {
+      term_b = from_lane(corners[1], seg);
+      if (GATE) term_b2 = from_lane(corners[2], seg);
     }
-    return r;
+  };
+  take_term(0), take_term(1);
+  // What the loads of the range's turn-th stage have in common, formed in five pieces: scalar instructions, which cost nothing between
+  // products and 200 cycles of a step in one go (the asm keeps each piece where it stands).
+  struct Request { i32x4 a, b, b2; uint32_t at, a_bytes, b_bytes; bool sum; };
+  auto request = [&](Request& r, int piece, int turn) __attribute__((always_inline)) {
+    if (piece == 0) {
+      uint32_t at = (step | 7) < whole ? step ^ shift : step, a_bytes = UNBOUNDED, b_bytes = UNBOUNDED;
+      const int left = turn < turns ? k_end - (int)at * GEMM_BK : 0;
+      if (left < GEMM_BK) {  // the last step, of a k range of no whole steps (behind it come only its own terms), or behind the range
+        asm volatile("");    // (a branch: every step would pay for the selection)
+        a_bytes = !left ? 0 : AKS ? left * lda2 + LDS_BIAS : UNBOUNDED;  // rows of a KS tile end with the k range
+        b_bytes = !left ? 0 : BKS ? left * ldb2 + LDS_BIAS : UNBOUNDED;
+#pragma unroll
+        for (int j = 0; j < sa.PASSES; ++j)
+          if (!AKS && sa.k_of(wave, lane, j) >= left) sa.off[j] = OUTSIDE;
+#pragma unroll
+        for (int j = 0; j < sb.PASSES; ++j)
+          if (!BKS && sb.k_of(wave, lane, j) >= left) sb.off[j] = OUTSIDE;
+      }
+      r.sum = SUMS && turn < turns && (sum_segments >> seg & 1);
+      pin(at), pin(a_bytes), pin(b_bytes);
+      r.at = at;
+      r.a_bytes = a_bytes;
+      r.b_bytes = b_bytes;
+    } else if (piece == 1) {
+      r.a = buffer_of(term_a + product64(r.at, astep), r.a_bytes);
+      pin(r.a);
+    } else if (piece == 2) {
+      const uint64_t to = product64(r.at, bstep);
+      r.b = buffer_of(term_b + to, r.b_bytes);
+      r.b2 = GATE ? buffer_of(term_b2 + to, r.b_bytes) : r.b;
+      pin(r.b);
+      if (GATE) pin(r.b2);
+    } else if (piece == 3) {
+      ++step;
+      moved = segments != 1 && step == group1;
+      if (moved) {
+        if (++seg == segments) {
+          seg = 0;
+          group0 = group1;
+          group1 = group_end(group0);
+        }
+        step = group0;
+        take_term(0);
+      }
+    } else if (moved) {
+      take_term(1);
+    }
   };
   // Pairs [first, last) of a wave's loads of a stage.  A wave fills a contiguous part of each operand's tile.
   auto load = [&](const Request& r, uint32_t stage, int first, int last) __attribute__((always_inline)) {
@@ -337,11 +403,7 @@ gemm_kernel(const GemmArgs p) {
     for (int l = first * 2; l < last * 2; l += 2) {
       const bool A = l < sa.PASSES;
       const int j = A ? l : l - sa.PASSES;
-      uint32_t o0 = A ? sa.off[j] : sb.off[j], o1 = A ? sa.off[j + 1] : sb.off[j + 1];
-      if (r.left < GEMM_BK) {  // the last step of a k range of no whole steps
-        if ((A ? sa.k_of(wave, lane, j) : sb.k_of(wave, lane, j)) >= r.left) o0 = 0x80000000u;
-        if ((A ? sa.k_of(wave, lane, j + 1) : sb.k_of(wave, lane, j + 1)) >= r.left) o1 = 0x80000000u;
-      }
+      const uint32_t o0 = A ? sa.off[j] : sb.off[j], o1 = A ? sa.off[j + 1] : sb.off[j + 1];
       const i32x4 rs = A ? r.a : GATE && (wave * sb.PASSES + j) * sb.RPW / 32 % 2 ? r.b2 : r.b;
       const uint32_t to = lds0 + stage + (A ? wave * sa.PASSES * 1024 : ABYTES + wave * sb.PASSES * 1024) + j / 4 * 4096;
       if (j % 4 == 0) load_to_lds<0>(rs, o0, o1, to);
@@ -374,7 +436,7 @@ gemm_kernel(const GemmArgs p) {
     else if (l <= NI) fb[q][l - 1] = fragment<BN, BKS>(st + ABYTES, lane, wn * NI + l - 1, s);
     else fa[q][l - NI] = fragment<BM, AKS>(st, lane, wm * MI + l - NI, s);
   };
-  auto part = [&](int q, uint32_t from, int s, bool refill, const Request& r, uint32_t to) __attribute__((always_inline)) {
+  auto part = [&](int q, uint32_t from, int s, bool refill, Request& r, uint32_t to, int turn) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -383,6 +445,7 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(fb[q][j], fa[q][i], acc[i][j], T());
       if (refill) load(r, to, i * (LOADS / 2) / MI, (i + 1) * (LOADS / 2) / MI);
+      if (i < (refill ? 2 : 3)) request(r, refill ? 3 + i : i, turn);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -399,7 +462,9 @@ gemm_kernel(const GemmArgs p) {
     bool sum = false, next[GEMM_STAGES];  // do the stage at hand, and those asked for, count for the sums of A
 #pragma unroll
     for (int k = 0; k < GEMM_STAGES; ++k) {
-      const Request r = request(k);
+      Request r;
+#pragma unroll
+      for (int piece = 0; piece < 5; ++piece) request(r, piece, k);
       next[k] = sums && r.sum;
       load(r, k * STAGE, 0, LOADS / 2);
     }
@@ -408,11 +473,9 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
     for (int l = 0; l < READS; ++l) read(0, 0, 0, l);
     for (int turn = 0; turn < turns; ++turn) {
-      const Request r = request(turn + GEMM_STAGES);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < PARTS - 1; ++s) part(s & 1, cur, s + 1, false, r, 0);
-      static_assert(PARTS % 2 == 0, "a step ends with the set that it began with");
+      Request r;
+      static_assert(PARTS == 2 && MI >= 3, "a step ends with the set that it began with; its request takes three rows of products");
+      part(0, cur, 1, false, r, 0, turn + GEMM_STAGES);
       if (sum) add_sums(cur);
       const uint32_t left = cur;
       cur = cur + STAGE == GEMM_STAGES * STAGE ? 0 : cur + STAGE;
@@ -421,7 +484,7 @@ gemm_kernel(const GemmArgs p) {
       next[GEMM_STAGES - 1] = sums && r.sum;
       sum = next[0];
       stage_arrived<LOADS * (GEMM_STAGES - 2)>();
-      part((PARTS - 1) & 1, cur, 0, true, r, left);  // (behind the range it reads zeros, and nobody uses them)
+      part(1, cur, 0, true, r, left, 0);  // (behind the range it reads zeros, and nobody uses them)
     }
   }
   stage_arrived<0>();  // the loads behind the range are done with LDS, and so is every wave
@@ -523,21 +586,22 @@ gemm_kernel(const GemmArgs p) {
   }
 }
 
-// Eight columns' sums over the partial products of a split k range: four groups of 64 threads take every fourth of them and meet in LDS,
-// in a fixed order.  Threads of the first group get the result.
-__device__ __forceinline__ bool join8(const float* part, int splits, int64_t stride, bool live, float (&v)[8]) {
+// Eight columns' sums over the partial products of a split k range, in a fixed order: by one thread each, or where there are many parts
+// by four groups of 64 threads, every fourth part each, that meet in LDS.  Threads of the first group get the result.
+__device__ __forceinline__ bool join8(const float* part, int splits, int64_t stride, bool grouped, bool live, float (&v)[8]) {
   __shared__ float sum[3][64][9];
-  const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, group = grouped ? threadIdx.x >> 6 : 0, groups = grouped ? 4 : 1;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
   if (live)
 #pragma unroll 4
-    for (int s = group; s < splits; s += 4) {
+    for (int s = group; s < splits; s += groups) {
       float w[8];
       load8(part + s * stride, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
+  if (!grouped) return live;
   __syncthreads();
   if (group)
 #pragma unroll
@@ -559,13 +623,15 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
   const int np = (p.N + 7) & ~7, pieces = np / 8;
   const int64_t all = p.M * pieces;
-  for (int64_t base = (int64_t)blockIdx.x * 64; base < all; base += (int64_t)gridDim.x * 64) {
-    const int64_t id = base + (threadIdx.x & 63), m = id / pieces;
+  const bool grouped = p.splits > 4;
+  const int count = grouped ? 64 : 256;
+  for (int64_t base = (int64_t)blockIdx.x * count; base < all; base += (int64_t)gridDim.x * count) {
+    const int64_t id = base + (threadIdx.x & (count - 1)), m = id / pieces;
     const int n = (int)(id % pieces) * 8;
     const float* part = (const float*)p.part + m * p.ldpart + n;
     float v[8], u[8], h[8];
-    const bool mine = join8(part, p.splits, (GATE ? 2 : 1) * p.split_stride, id < all, v);
-    if constexpr (GATE) join8(part + p.split_stride, p.splits, 2 * p.split_stride, id < all, u);
+    const bool mine = join8(part, p.splits, (GATE ? 2 : 1) * p.split_stride, grouped, id < all, v);
+    if constexpr (GATE) join8(part + p.split_stride, p.splits, 2 * p.split_stride, grouped, id < all, u);
     if (!mine) continue;
     if constexpr (GATE) {
 #pragma unroll
@@ -608,15 +674,15 @@ struct GemmPlan { int tile, splits; size_t part_bytes; };
 // Tile and split of the k range: the least of an estimate in microseconds.  A product's time is that of its stages - alone on a CU, or two
 // workgroups to a CU where they fit (WIDE: two rounds) - but not less than the n side's bytes take, then for each round of workgroups
 // a start and the tile's results on their way (`bytes` per element of the tile), and for a split k range the joining launch.  The
-// constants are fitted to the measured times of every tile and split at 52 sizes of the block (6 to 65536 rows, widths 64 to 11008,
-// bf16 and fp32, all products of both passes): what it picks takes 2 % longer than the best on average, 42 % at worst (products of
-// 10 us), where always taking MID unsplit would take 50 % longer.  `outs`: products per n (2: both projections).
+// constants are fitted to the measured times of every tile and split at 48 sizes of the block (6 to 65536 rows, widths 64 to 11008,
+// bf16 and fp32, all products of both passes): what it picks takes 2 % longer than the best on average and 30 % at worst, where always
+// taking MID unsplit would take 66 % longer.  `outs`: products per n (2: both projections).
 inline GemmPlan gemm_plan(int64_t M, int N, int steps, int terms, int outs, int bytes, bool slim) {
   const int cus = 256;
-  constexpr double ALONE[TILES] = {1.8, 1.55, 0.6}, PAIR[TILES] = {5.1, 1.3, 0.9}, START[TILES] = {1.7, 1.9, 1.5};
+  constexpr double ALONE[TILES] = {1.6, 0.97, 0.54}, PAIR[TILES] = {4.0, 1.08, 0.8}, START[TILES] = {2.1, 1.7, 2.1};
   GemmPlan best = {TILE_MID, 1, 0};
   double cost = 1e300;
-  const double stream = (double)N * outs * steps * (terms > 1 ? 3 : 1) * GEMM_BK * 2 / 7.8e6;
+  const double stream = (double)N * outs * steps * (terms > 1 ? 3 : 1) * GEMM_BK * 2 / 4.4e6;
   for (int t = 0; t < TILES; ++t) {
     if (t == TILE_SLIM && !slim) continue;
     const int64_t tiles = ((M + TILE_M[t] - 1) / TILE_M[t]) * (((int64_t)N * outs + TILE_N[t] - 1) / TILE_N[t]);
@@ -627,8 +693,8 @@ inline GemmPlan gemm_plan(int64_t M, int N, int steps, int terms, int outs, int 
       const double alone = blocks <= cus / 2 ? 1.4 * ALONE[t] : ALONE[t];
       double c = per * terms * (full * PAIR[t] + (rest > cus ? PAIR[t] : rest ? alone : 0.0));
       if (c < stream) c = stream;
-      c += (double)((blocks + cus - 1) / cus) * (START[t] + TILE_M[t] * TILE_N[t] * (s > 1 ? 4 : bytes) / 18.0e3);
-      if (s > 1) c += 11.5 + (double)M * N * outs * 4 * s / 2.4e6;
+      c += (double)((blocks + cus - 1) / cus) * (START[t] + TILE_M[t] * TILE_N[t] * (s > 1 ? 4 : bytes) / 22.0e3);
+      if (s > 1) c += 9.0 + (double)M * N * outs * 4 * s / 2.3e6;
       if (c < cost) { cost = c; best.tile = t; best.splits = s; }
     }
   }
@@ -675,7 +741,7 @@ int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
     e = hipLaunchKernel(f, grid, dim3(tile == TILE_WIDE ? 512 : 256), args, bytes, st);
   }
   if (e == hipSuccess && a.splits > 1) {
-    const int64_t blocks = (a.M * ((a.N + 7) / 8) + 63) / 64;
+    const int64_t count = a.splits > 4 ? 64 : 256, blocks = (a.M * ((a.N + 7) / 8) + count - 1) / count;
     join_kernel<T, EPI><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
     e = hipGetLastError();
   }

@@ -7,19 +7,21 @@ what the kernels cannot read as it lies (a last dimension with a stride, rows of
 Outputs and workspaces come from torch's allocator, so the calls may be captured into a graph.  There is no CPU path."""
 import ctypes as C
 import math
+import struct
 
 import torch
 
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_POSITIONS = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
 
 
 def _dtype(t, name):
     if not torch.is_tensor(t):
         raise RuntimeError(f"{name} must be a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} must be on the GPU (it is on {t.device}). There is no CPU path.")
     if t.dtype not in _DTYPES:
         raise RuntimeError(f"{name} must be fp32, bfloat16 or half (got {t.dtype})")
@@ -27,6 +29,8 @@ def _dtype(t, name):
 
 
 def _like(t, x, name, dtypes=None):
+    if torch.is_tensor(t) and t.is_cuda and t.get_device() == x.get_device() and t.dtype in (dtypes or (x.dtype,)):
+        return t
     _dtype(t, name)
     if t.device != x.device:
         raise RuntimeError(f"{name} must be on {x.device} (got {t.device})")
@@ -39,7 +43,7 @@ def _vector(t, n, x, name, dtypes=None):
     if t is None:
         return None
     _like(t, x, name, dtypes)
-    if t.shape != (n,):
+    if t.dim() != 1 or t.shape[0] != n:
         raise RuntimeError(f"{name} must be [{n}] (got {tuple(t.shape)})")
     return t.contiguous()
 
@@ -74,7 +78,7 @@ def _ptr(t):
 def _call(t, fn, *args):
     """fn(*args, stream) on the tensor's device and its current stream; raises what the library reports."""
     index = t.get_device()
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -183,10 +187,26 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
 
 
 _Strides = C.c_int64 * 3
+_TENSOR = struct.Struct("@PP6qi4x")  # dm_rotary_tensor; packed by one call, as a structure built field by field costs more than the launch
 
 
-def _rotary_tensor(t, out):
-    return _lib.RotaryTensor(t.data_ptr(), out.data_ptr(), _Strides(*t.stride()[:3]), _Strides(*out.stride()[:3]), t.shape[2])
+def _turned(x, inplace):
+    """x as the kernel reads it, where the result goes, and both as dm_rotary_tensor."""
+    b, t, heads, d = x.shape
+    strides = x.stride()
+    if d > 1 and strides[3] != 1:
+        if inplace:
+            raise RuntimeError("in place needs contiguous head elements")
+        x = x.contiguous()
+        strides = x.stride()
+    if inplace:
+        if any(n > 1 and s == 0 for n, s in zip((b, t, heads), strides)):
+            raise RuntimeError("in place needs a tensor without expanded dimensions")
+        p = x.data_ptr()
+        return x, x, _lib.RotaryTensor.from_buffer_copy(_TENSOR.pack(p, p, *strides[:3], *strides[:3], heads))
+    out = _empty_like(x)
+    return x, out, _lib.RotaryTensor.from_buffer_copy(
+        _TENSOR.pack(x.data_ptr(), out.data_ptr(), *strides[:3], t * heads * d, heads * d, d, heads))
 
 
 def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inverse=False, inplace=False):
@@ -205,45 +225,38 @@ def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inver
             raise RuntimeError(f"k must be [{b}, {t}, heads, {d}] (got {tuple(k.shape)})")
     if layout not in ("half", "interleaved"):
         raise ValueError(f"Unknown rotary layout: {layout}")
-    if not torch.is_tensor(inv_freq) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device:
+    if not torch.is_tensor(inv_freq) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.get_device() != q.get_device():
         raise RuntimeError(f"inv_freq must be a float64 vector on {q.device} (rotary_frequencies makes one)")
-    rotary_dim = 2 * inv_freq.numel()
-    if rotary_dim > d:
-        raise RuntimeError(f"{inv_freq.numel()} pairs do not fit a head of {d} elements")
+    pairs = inv_freq.numel()
+    if 2 * pairs > d:
+        raise RuntimeError(f"{pairs} pairs do not fit a head of {d} elements")
     axes, strides = 1, None
     if positions is not None:
-        if positions.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8) or positions.device != q.device:
+        if not torch.is_tensor(positions) or positions.dtype not in _POSITIONS or positions.get_device() != q.get_device():
             raise RuntimeError(f"positions must be integers on {q.device}")
-        axes = positions.shape[0] if positions.dim() == 3 else 1
-        if positions.dim() not in (1, 2, 3) or axes < 1:
-            raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] (got {tuple(positions.shape)})")
-        if any(have not in (1, want) for have, want in zip(positions.shape[::-1], (t, b))):
-            raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] with B = {b}, T = {t} (got {tuple(positions.shape)})")
-        positions = positions.to(torch.int64)
-        if positions.shape != (axes, b, t):
-            positions = positions.expand(axes, b, t)
-        strides = _Strides(*positions.stride())
-    if inv_freq.numel() % axes:
-        raise RuntimeError(f"{inv_freq.numel()} pairs do not divide into {axes} axes")
-    args, outs = [], []
-    for x in (q, k):
-        if x is None:
-            args.append(None)
-            outs.append(None)
-            continue
-        if inplace:
-            if (d > 1 and x.stride(3) != 1) or any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-                raise RuntimeError("in place needs contiguous head elements and no expanded dimension")
-            out = x
-        else:
-            x = x if d == 1 or x.stride(3) == 1 else x.contiguous()
-            out = _empty_like(x)
-        args.append((x, _rotary_tensor(x, out)))
-        outs.append(out)
+        shape = positions.shape
+        dims = len(shape)
+        axes = shape[0] if dims == 3 else 1
+        if dims not in (1, 2, 3) or axes < 1:
+            raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] (got {tuple(shape)})")
+        if shape[-1] not in (1, t) or (dims > 1 and shape[-2] not in (1, b)):
+            raise RuntimeError(f"positions must be [T], [B, T] or [axes, B, T] with B = {b}, T = {t} (got {tuple(shape)})")
+        if positions.dtype != torch.int64:
+            positions = positions.to(torch.int64)
+        have = positions.stride()
+        strides = _Strides(have[0] if axes > 1 else 0, have[-2] if dims > 1 and shape[-2] > 1 else 0, have[-1] if shape[-1] > 1 else 0)
+    if pairs % axes:
+        raise RuntimeError(f"{pairs} pairs do not divide into {axes} axes")
+    if inplace and k is not None and k.data_ptr() == q.data_ptr() and q.numel():
+        raise RuntimeError("in place needs q and k that share no elements")
+    q, q_out, q_arg = _turned(q, inplace)
+    k_out = k_arg = None
+    if k is not None:
+        k, k_out, k_arg = _turned(k, inplace)
     inv_freq = inv_freq.contiguous()
-    _call(q, _lib.lib().dm_rotary, C.byref(args[0][1]), None if k is None else C.byref(args[1][1]), _ptr(positions), strides, axes,
-          inv_freq.data_ptr(), b, t, d, rotary_dim, layout == "interleaved", scale, bool(inverse), dt)
-    return tuple(outs)
+    _call(q, _lib.lib().dm_rotary, q_arg, k_arg, _ptr(positions), strides, axes, inv_freq.data_ptr(), b, t, d, 2 * pairs, layout == "interleaved",
+          scale, bool(inverse), dt)
+    return q_out, k_out
 
 
 # ------------------------------------------------------------------ gated feed-forward block
