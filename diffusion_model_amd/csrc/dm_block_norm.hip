@@ -10,181 +10,279 @@
 
 namespace dmb {
 
-// Sum over the TPR threads of a row: within a wave by shuffles, across the waves of a block through `red`.
+// Two sums over the TPR threads of a row: within a wave by shuffles, across the waves of a block through `red`, whose halves are used in
+// turn (`half`): one barrier, behind which nobody still reads the half that is written next.
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  if constexpr (TPR <= 64) {
-    return group_sum<TPR>(v);
-  } else {
+__device__ __forceinline__ void row_sums(float& a, float& b, float (*red)[2][TPR > 64 ? TPR / 64 : 1], int& half) {
+  constexpr int W = TPR < 64 ? TPR : 64;
+  a = group_sum<W>(a);
+  b = group_sum<W>(b);
+  if constexpr (TPR > 64) {
     constexpr int NW = TPR / 64;
-    v = group_sum<64>(v);
-    __syncthreads();  // the previous sum's readers are done with `red`
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) { red[half][0][threadIdx.x >> 6] = a; red[half][1][threadIdx.x >> 6] = b; }
     __syncthreads();
-    float s = 0.f;
+    a = b = 0.f;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) s += red[i];
-    return s;
+    for (int i = 0; i < NW; ++i) { a += red[half][0][i]; b += red[half][1][i]; }
+    half ^= 1;
   }
 }
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float (*red)[2][TPR > 64 ? TPR / 64 : 1], int& half) {
+  float none = 0.f;
+  row_sums<TPR>(v, none, red, half);
+  return v;
+}
 
-// TPR threads hold a row as NCH vectors of V elements each: C <= TPR * V * NCH, C % V == 0, rows V-aligned.
-template <typename T, typename P, int V, int TPR, int NCH>
+// V elements of a row, at any element boundary: the hardware takes such vectors (bf16, 16384 rows of odd width 1001: 16 us against 39 us
+// element by element).
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[V]; };
+
+// The piece of a row that a thread holds from column c on.  WHOLE (C a multiple of V): the piece lies inside the row or behind it.  Else the
+// last piece is moved back to end with the row: its first `skip` elements are a neighbour's too, which counts them in sums over the row;
+// both write the same values.  Behind the row all of it is skipped.
+template <int V, bool WHOLE>
+struct Place {
+  int at, skip;
+  bool in;
+  __device__ __forceinline__ Place(int c, int C) : at(WHOLE || c + V <= C ? c : C - V), skip(WHOLE ? 0 : c - at), in(c < C) {}
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, Piece<T, V>& r) const {
+    if (!WHOLE || in) {
+      r = *reinterpret_cast<const Piece<T, V>*>(row + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) r.v[j] = (T)0.f;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, const float (&v)[V]) const {
+    Piece<T, V> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r.v[j] = (T)v[j];
+    *reinterpret_cast<Piece<T, V>*>(row + at) = r;
+  }
+  __device__ __forceinline__ bool counts(int j) const { return WHOLE ? in : j >= skip; }
+};
+
+// TPR threads hold a row as NCH pieces each: C <= TPR * V * NCH.
+template <typename T, typename P, bool WHOLE, int TPR, int NCH>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 layer_norm_kernel(const T* __restrict__ x, int64_t xs, const P* __restrict__ w, const P* __restrict__ b, T* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t M, int C, float eps) {
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float red[2][2][TPR > 64 ? TPR / 64 : 1];
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;  // rows per block
   const int t = threadIdx.x % TPR;
+  int half = 0;
   for (int64_t base = (int64_t)blockIdx.x * RPB; base < M; base += (int64_t)gridDim.x * RPB) {
-  const int64_t row0 = base + threadIdx.x / TPR;
-  const bool live = row0 < M;
-  const int64_t row = live ? row0 : M - 1;  // surplus rows repeat the last one and store nothing
-  const T* xr = x + row * xs;
-  float v[NCH][V];
-  float s = 0.f;
+    const int64_t row0 = base + threadIdx.x / TPR;
+    const bool live = row0 < M;
+    const int64_t row = live ? row0 : M - 1;  // surplus rows repeat the last one and store nothing
+    const T* xr = x + row * xs;
+    float v[NCH][V];
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = (i * TPR + t) * V;
-    if (c < C) load_vec<T, V>(xr + c, v[i]);
+    for (int i = 0; i < NCH; ++i) {
+      const Place<V, WHOLE> at((i * TPR + t) * V, C);
+      Piece<T, V> r;
+      at.load(xr, r);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (c >= C) v[i][j] = 0.f;
-      s += v[i][j];
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = (float)r.v[j];
+        s += WHOLE || at.counts(j) ? v[i][j] : 0.f;
+      }
     }
-  }
-  const float mean = row_sum<TPR>(s, red) / C;
-  float q = 0.f;
+    const float mean = row_sum<TPR>(s, red, half) / C;
+    float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < NCH; ++i)
-    if ((i * TPR + t) * V < C)
+    for (int i = 0; i < NCH; ++i) {
+      const Place<V, WHOLE> at((i * TPR + t) * V, C);
+      if (at.in)
 #pragma unroll
-      for (int j = 0; j < V; ++j) { const float d = v[i][j] - mean; q += d * d; }
-  const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) / C + eps);
-  if (!live) continue;
-  T* yr = y + row * C;
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = (i * TPR + t) * V;
-    if (c >= C) continue;
-    float o[V], wv[V], bv[V];
-    if (w) load_vec<P, V>(w + c, wv);
-    if (b) load_vec<P, V>(b + c, bv);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      o[j] = (v[i][j] - mean) * rstd;
-      if (w) o[j] *= wv[j];
-      if (b) o[j] += bv[j];
+        for (int j = 0; j < V; ++j) {
+          const float d = v[i][j] - mean;
+          q += at.counts(j) ? d * d : 0.f;
+        }
     }
-    store_vec<T, V>(yr + c, o);
-  }
-  if (t == 0) {
-    if (mean_out) mean_out[row] = mean;
-    if (rstd_out) rstd_out[row] = rstd;
-  }
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red, half) / C + eps);
+    if (!live) continue;
+    T* yr = y + row * C;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const Place<V, WHOLE> at((i * TPR + t) * V, C);
+      if (!at.in) continue;
+      float o[V];
+      Piece<P, V> wv, bv;
+      if (w) at.load(w, wv);
+      if (b) at.load(b, bv);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        o[j] = (v[i][j] - mean) * rstd;
+        if (w) o[j] *= (float)wv.v[j];
+        if (b) o[j] += (float)bv.v[j];
+      }
+      at.store(yr, o);
+    }
+    if (t == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
+    }
   }
 }
 
-// Rows too wide for registers: three walks over the row (it stays in the caches), one block per row.
-template <typename T, typename P>
+// Rows too wide for registers (or narrower than a vector: V = 1): three walks over the row (it stays in the caches), one block per row.
+template <typename T, typename P, int V>
 __global__ void __launch_bounds__(1024)
 layer_norm_wide_kernel(const T* __restrict__ x, int64_t xs, const P* __restrict__ w, const P* __restrict__ b, T* __restrict__ y,
                        float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t M, int C, float eps) {
-  __shared__ float red[16];
+  __shared__ float red[2][2][16];
+  int half = 0;
   for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
-  const T* xr = x + row * xs;
-  float s = 0.f, q = 0.f;
-  for (int c = threadIdx.x; c < C; c += 1024) s += (float)xr[c];
-  const float mean = row_sum<1024>(s, red) / C;
-  for (int c = threadIdx.x; c < C; c += 1024) { const float d = (float)xr[c] - mean; q += d * d; }
-  const float rstd = 1.f / sqrtf(row_sum<1024>(q, red) / C + eps);
-  for (int c = threadIdx.x; c < C; c += 1024) {
-    float o = ((float)xr[c] - mean) * rstd;
-    if (w) o *= (float)w[c];
-    if (b) o += (float)b[c];
-    y[row * C + c] = (T)o;
-  }
-  if (threadIdx.x == 0) {
-    if (mean_out) mean_out[row] = mean;
-    if (rstd_out) rstd_out[row] = rstd;
-  }
+    const T* xr = x + row * xs;
+    float s = 0.f, q = 0.f;
+#pragma unroll 4
+    for (int c = threadIdx.x * V; c < C; c += 1024 * V) {
+      const Place<V, false> at(c, C);
+      Piece<T, V> v;
+      at.load(xr, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += at.counts(j) ? (float)v.v[j] : 0.f;
+    }
+    const float mean = row_sum<1024>(s, red, half) / C;
+#pragma unroll 4
+    for (int c = threadIdx.x * V; c < C; c += 1024 * V) {
+      const Place<V, false> at(c, C);
+      Piece<T, V> v;
+      at.load(xr, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = (float)v.v[j] - mean;
+        q += at.counts(j) ? d * d : 0.f;
+      }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red, half) / C + eps);
+#pragma unroll 2
+    for (int c = threadIdx.x * V; c < C; c += 1024 * V) {
+      const Place<V, false> at(c, C);
+      Piece<T, V> v;
+      Piece<P, V> wv, bv;
+      at.load(xr, v);
+      if (w) at.load(w, wv);
+      if (b) at.load(b, bv);
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        o[j] = ((float)v.v[j] - mean) * rstd;
+        if (w) o[j] *= (float)wv.v[j];
+        if (b) o[j] += (float)bv.v[j];
+      }
+      at.store(y + row * C, o);
+    }
+    if (threadIdx.x == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
+    }
   }
 }
 
-// dx, and the block's share of dw / db over the rows it walks (grid-stride): part[block][2][C].
-template <typename T, typename P, int V, int TPR, int NCH>
+// dx, and the block's share of dw / db over the rows it walks (grid-stride): part[block][2][C].  The next row's loads are under way while a
+// row is summed; rows stay in their own type in registers, so that the two rows and the two running sums of every column fit.
+// (Pieces are moved back at the end of every row: with a branch around each load, 8192 x 8192 bf16 take 151 us instead of 92.)
+template <typename T, typename P, int TPR, int NCH>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, const P* __restrict__ w,
                       const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, float* __restrict__ part,
                       int64_t M, int C) {
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  constexpr int V = 16 / sizeof(T), RPB = TPR < 256 ? 256 / TPR : 1;
+  constexpr bool AHEAD = NCH * V <= 16;  // (32 pairs of sums leave no registers for a second row)
+  __shared__ float red[2][2][TPR > 64 ? TPR / 64 : 1];
   const int t = threadIdx.x % TPR;
-  float aw[NCH][V], ab[NCH][V], wv[NCH][V];
+  int half = 0;
+  float aw[NCH][V], ab[NCH][V];
+  Piece<P, V> wv[NCH];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = (i * TPR + t) * V;
-    if (w && c < C) load_vec<P, V>(w + c, wv[i]);
+    const Place<V, false> at((i * TPR + t) * V, C);
+    if (w) at.load(w, wv[i]);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       aw[i][j] = ab[i][j] = 0.f;
-      if (!w || c >= C) wv[i][j] = 1.f;
+      if (!w) wv[i].v[j] = (P)1.f;
     }
   }
-  for (int64_t base = (int64_t)blockIdx.x * RPB; base < M; base += (int64_t)gridDim.x * RPB) {
-    const int64_t row0 = base + threadIdx.x / TPR;
-    const bool live = row0 < M;
-    const int64_t row = live ? row0 : M - 1;
-    const float mu = mean[row], rs = rstd[row];
-    float z[NCH][V], g[NCH][V];
+  struct Row { Piece<T, V> x[NCH], g[NCH]; float mu, rs; } cur, next;
+  auto load = [&](Row& r, int64_t base) __attribute__((always_inline)) {
+    int64_t row = base + threadIdx.x / TPR;
+    if (row >= M) row = M - 1;
+    r.mu = mean[row];
+    r.rs = rstd[row];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const Place<V, false> at((i * TPR + t) * V, C);
+      at.load(x + row * xs, r.x[i]);
+      at.load(dy + row * dys, r.g[i]);
+    }
+  };
+  const int64_t first = (int64_t)blockIdx.x * RPB, stride = (int64_t)gridDim.x * RPB;
+  load(cur, first);
+  for (int64_t base = first; base < M; base += stride) {
+    if (AHEAD) load(next, base + stride < M ? base + stride : base);
+    const int64_t row = base + threadIdx.x / TPR;
+    const bool live = row < M;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < C) {
-        load_vec<T, V>(x + row * xs + c, z[i]);
-        load_vec<T, V>(dy + row * dys + c, g[i]);
+      const Place<V, false> at((i * TPR + t) * V, C);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          z[i][j] = (z[i][j] - mu) * rs;
-          if (live) { aw[i][j] += g[i][j] * z[i][j]; ab[i][j] += g[i][j]; }
-          g[i][j] *= wv[i][j];
-          s1 += g[i][j];
-          s2 += g[i][j] * z[i][j];
-        }
+      for (int j = 0; j < V; ++j) {
+        const float z = ((float)cur.x[i].v[j] - cur.mu) * cur.rs, d = (float)cur.g[i].v[j];
+        if (live) { aw[i][j] += d * z; ab[i][j] += d; }
+        const float g = at.counts(j) ? d * (float)wv[i].v[j] : 0.f;
+        s1 += g;
+        s2 += at.counts(j) ? g * z : 0.f;
       }
     }
-    s1 = row_sum<TPR>(s1, red) / C;
-    s2 = row_sum<TPR>(s2, red) / C;
+    row_sums<TPR>(s1, s2, red, half);
+    s1 /= C;
+    s2 /= C;
     if (live)
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int c = (i * TPR + t) * V;
-        if (c >= C) continue;
+        const Place<V, false> at((i * TPR + t) * V, C);
+        if (!at.in) continue;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = rs * (g[i][j] - s1 - z[i][j] * s2);
-        store_vec<T, V>(dx + row * C + c, o);
+        for (int j = 0; j < V; ++j) {
+          const float z = ((float)cur.x[i].v[j] - cur.mu) * cur.rs, g = (float)cur.g[i].v[j] * (float)wv[i].v[j];
+          o[j] = cur.rs * (g - s1 - z * s2);
+        }
+        at.store(dx + row * C, o);
       }
+    if (AHEAD) cur = next;
+    else load(cur, base + stride < M ? base + stride : base);
   }
   if (!part) return;
   float* pw = part + (int64_t)blockIdx.x * 2 * C;
   if constexpr (RPB == 1) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c >= C) continue;
-#pragma unroll
-      for (int j = 0; j < V; ++j) { pw[c + j] = aw[i][j]; pw[C + c + j] = ab[i][j]; }
+      const Place<V, false> at((i * TPR + t) * V, C);
+      if (!at.in) continue;
+      at.store(pw, aw[i]);
+      at.store(pw + C, ab[i]);
     }
-  } else {  // the block's row groups are added in order through LDS, one vector column at a time
+  } else {  // the block's row groups are added in order through LDS, one piece column at a time
     __shared__ float sum[2][RPB][TPR][V];
     const int r = threadIdx.x / TPR;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
+      const Place<V, false> at((i * TPR + t) * V, C);
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < V; ++j) { sum[0][r][t][j] = aw[i][j]; sum[1][r][t][j] = ab[i][j]; }
+      for (int j = 0; j < V; ++j)
+        if (at.counts(j)) { sum[0][r][t][j - at.skip] = aw[i][j]; sum[1][r][t][j - at.skip] = ab[i][j]; }
       __syncthreads();
       for (int e = threadIdx.x; e < 2 * TPR * V; e += 256) {
         const int k = e / (TPR * V), o = e % (TPR * V), c = i * TPR * V + o;
@@ -197,141 +295,169 @@ layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict
   }
 }
 
-// Rows too wide for registers: dx alone (two walks over the row); dw / db by column_sums_kernel.
-template <typename T, typename P>
+// Rows too wide for registers (or narrower than a vector: V = 1): dx alone (two walks over the row), and the parameters' gradients by
+// columns.
+template <typename T, typename P, int V>
 __global__ void __launch_bounds__(1024)
 layer_norm_bwd_wide_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, const P* __restrict__ w,
                            const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, int64_t M, int C) {
-  __shared__ float red[16];
+  __shared__ float red[2][2][16];
+  int half = 0;
   for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
-  const float mu = mean[row], rs = rstd[row];
-  float s1 = 0.f, s2 = 0.f;
-  for (int c = threadIdx.x; c < C; c += 1024) {
-    const float g = (float)dy[row * dys + c] * (w ? (float)w[c] : 1.f), z = ((float)x[row * xs + c] - mu) * rs;
-    s1 += g;
-    s2 += g * z;
-  }
-  s1 = row_sum<1024>(s1, red) / C;
-  s2 = row_sum<1024>(s2, red) / C;
-  for (int c = threadIdx.x; c < C; c += 1024) {
-    const float g = (float)dy[row * dys + c] * (w ? (float)w[c] : 1.f), z = ((float)x[row * xs + c] - mu) * rs;
-    dx[row * C + c] = (T)(rs * (g - s1 - z * s2));
-  }
+    const float mu = mean[row], rs = rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+    auto piece = [&](const Place<V, false>& at, float (&z)[V], float (&g)[V]) __attribute__((always_inline)) {
+      Piece<T, V> xv, dv;
+      Piece<P, V> wv;
+      at.load(x + row * xs, xv);
+      at.load(dy + row * dys, dv);
+      if (w) at.load(w, wv);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        z[j] = ((float)xv.v[j] - mu) * rs;
+        g[j] = w ? (float)dv.v[j] * (float)wv.v[j] : (float)dv.v[j];
+      }
+    };
+#pragma unroll 2
+    for (int c = threadIdx.x * V; c < C; c += 1024 * V) {
+      const Place<V, false> at(c, C);
+      float z[V], g[V];
+      piece(at, z, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (at.counts(j)) { s1 += g[j]; s2 += g[j] * z[j]; }
+    }
+    row_sums<1024>(s1, s2, red, half);
+    s1 /= C;
+    s2 /= C;
+#pragma unroll 2
+    for (int c = threadIdx.x * V; c < C; c += 1024 * V) {
+      const Place<V, false> at(c, C);
+      float z[V], g[V];
+      piece(at, z, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[j] = rs * (g[j] - s1 - z[j] * s2);
+      at.store(dx + row * C, z);
+    }
   }
 }
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 layer_norm_bwd_wide_params_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs,
                                   const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part, int64_t M, int C) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * V;
   if (c >= C) return;
-  float aw = 0.f, ab = 0.f;
+  const Place<V, false> at(c, C);
+  float aw[V] = {}, ab[V] = {};
+#pragma unroll 4
   for (int64_t row = blockIdx.y; row < M; row += gridDim.y) {
-    const float g = (float)dy[row * dys + c];
-    aw += g * ((float)x[row * xs + c] - mean[row]) * rstd[row];
-    ab += g;
+    Piece<T, V> xv, dv;
+    at.load(x + row * xs, xv);
+    at.load(dy + row * dys, dv);
+    const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float g = (float)dv.v[j];
+      aw[j] += g * (((float)xv.v[j] - mu) * rs);
+      ab[j] += g;
+    }
   }
   float* pw = part + (int64_t)blockIdx.y * 2 * C;
-  pw[c] = aw;
-  pw[C + c] = ab;
+  at.store(pw, aw);
+  at.store(pw + C, ab);
 }
 
-constexpr int NORM_BWD_BLOCKS = 1024;
+// Blocks of the backward pass: four to a CU, but sixteen rows each where that leaves one to a CU, as each writes a row of sums for the
+// second launch to read (4096 x 16384 bf16: 1024 blocks' sums are two thirds of the tensors' bytes).
+inline int norm_bwd_blocks(int64_t M) { return (int)(M < 256 ? M : M < 256 * 16 ? 256 : M < 1024 * 16 ? M / 16 : 1024); }
 constexpr int64_t NORM_MAX_BLOCKS = 1 << 20;  // further rows are walked by the same blocks (a launch holds fewer than 2^32 threads)
 inline unsigned norm_grid(int64_t n) { return (unsigned)(n < NORM_MAX_BLOCKS ? n : NORM_MAX_BLOCKS); }
 
-struct NormShape { int V, TPR, NCH; };
+struct NormShape { int TPR, NCH; };
 
-// Vectors of 16 bytes where the width and every row allow it, else single elements.  A wave per row (a quarter of one for narrow rows)
-// while the row fits `most` vectors per lane, else a block of 256 or 1024 threads; {0,0,0}: the row does not fit registers.
-inline NormShape norm_shape(int C, int full, bool vec, int most, bool few_rows) {
-  NormShape s = {0, 0, 0};
-  s.V = vec ? full : 1;
-  const int64_t n = (C + s.V - 1) / s.V;  // vectors per row
+// A wave per row (a quarter of one for narrow rows) while the row fits `most` pieces per lane, else a block of 256, else a block of `wide`
+// threads with up to 32 elements each; {0, 0}: the row does not fit registers, or is no whole piece.
+inline NormShape norm_shape(int C, int V, int most, int wide) {
+  const int64_t n = (C + V - 1) / V;  // pieces per row
   auto up = [](int64_t v) { int p = 1; while (p < v) p *= 2; return p; };
-  if (n <= 16) { s.TPR = 16; s.NCH = 1; return s; }
-  if (n <= 64 * (few_rows ? 1 : most)) { s.TPR = 64; s.NCH = up((n + 63) / 64); return s; }
-  if (n <= 256 * most) { s.TPR = 256; s.NCH = up((n + 255) / 256); return s; }
-  if (n <= 1024 * most) { s.TPR = 1024; s.NCH = up((n + 1023) / 1024); return s; }
-  s.TPR = 0;
-  return s;
+  if (C < V) return {0, 0};
+  if (n <= 16) return {16, 1};
+  if (n <= 64 * most) return {64, up((n + 63) / 64)};
+  if (n <= 256 * most) return {256, up((n + 255) / 256)};
+  if (C <= 32 * wide) return {wide, up((n + wide - 1) / wide)};
+  return {0, 0};
 }
 
-template <typename T, typename P, int V, typename F>
+// f(TPR, NCH) of the shape (one of those that norm_shape gives in that direction)
+template <int V, bool FORWARD, typename F>
 int norm_dispatch(const NormShape& s, F&& f) {
-#define DM_NORM_CASE(tpr, nch) \
-  if (s.TPR == tpr && s.NCH == nch) return f(std::integral_constant<int, tpr>{}, std::integral_constant<int, nch>{});
+#define DM_NORM_CASE(tpr, nch)                                                                                                  \
+  if constexpr (FORWARD ? nch * V <= 32 && tpr != 512 : nch * V <= (tpr == 512 ? 32 : 16) && (tpr != 512 || nch * V > 8) && tpr != 1024) \
+    if (s.TPR == tpr && s.NCH == nch) return f(std::integral_constant<int, tpr>{}, std::integral_constant<int, nch>{});
   DM_NORM_CASE(16, 1) DM_NORM_CASE(64, 1) DM_NORM_CASE(64, 2) DM_NORM_CASE(64, 4) DM_NORM_CASE(256, 1) DM_NORM_CASE(256, 2)
-  DM_NORM_CASE(256, 4) DM_NORM_CASE(1024, 2) DM_NORM_CASE(1024, 4)
+  DM_NORM_CASE(256, 4) DM_NORM_CASE(512, 2) DM_NORM_CASE(512, 4) DM_NORM_CASE(512, 8) DM_NORM_CASE(1024, 1) DM_NORM_CASE(1024, 2)
+  DM_NORM_CASE(1024, 4) DM_NORM_CASE(1024, 8)
 #undef DM_NORM_CASE
-  return fail("layer norm: no kernel for %d threads x %d vectors", s.TPR, s.NCH);
-}
-
-template <typename T, typename P, int V>
-int norm_fwd_run(const NormShape& s, const T* x, int64_t xs, const P* w, const P* b, T* y, float* mean, float* rstd, int64_t M, int C,
-                 float eps, hipStream_t st) {
-  return norm_dispatch<T, P, V>(s, [&](auto tpr, auto nch) {
-    constexpr int TPR = decltype(tpr)::value, NCH = decltype(nch)::value, RPB = TPR < 256 ? 256 / TPR : 1;
-    layer_norm_kernel<T, P, V, TPR, NCH><<<dim3(norm_grid((M + RPB - 1) / RPB)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(
-        x, xs, w, b, y, mean, rstd, M, C, eps);
-    return launched("dm_layer_norm");
-  });
+  return fail("layer norm: no kernel for %d threads x %d pieces", s.TPR, s.NCH);
 }
 
 template <typename T, typename P>
-int norm_fwd(const void* x, int64_t xs, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t M, int C, float eps,
+int norm_fwd(const void* xp, int64_t xs, const void* wp, const void* bp, void* yp, float* mean, float* rstd, int64_t M, int C, float eps,
              hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = C % V == 0 && xs % V == 0 && aligned(x, 16) && aligned(y, 16) && (!w || aligned(w, V * sizeof(P))) &&
-                   (!b || aligned(b, V * sizeof(P)));
-  const NormShape s = norm_shape(C, V, vec, 4, M < 1024);
+  const T* x = (const T*)xp;
+  const P *w = (const P*)wp, *b = (const P*)bp;
+  T* y = (T*)yp;
+  const NormShape s = norm_shape(C, V, M < 1024 ? 1 : 4, 1024);  // (few rows: as many threads as there can be)
   if (!s.TPR) {
-    layer_norm_wide_kernel<T, P><<<dim3(norm_grid(M)), dim3(1024), 0, st>>>((const T*)x, xs, (const P*)w, (const P*)b, (T*)y, mean, rstd, M, C, eps);
+    const dim3 grid(norm_grid(M)), block(1024);
+    if (C < V) layer_norm_wide_kernel<T, P, 1><<<grid, block, 0, st>>>(x, xs, w, b, y, mean, rstd, M, C, eps);
+    else layer_norm_wide_kernel<T, P, V><<<grid, block, 0, st>>>(x, xs, w, b, y, mean, rstd, M, C, eps);
     return launched("dm_layer_norm");
   }
-  return s.V == V ? norm_fwd_run<T, P, V>(s, (const T*)x, xs, (const P*)w, (const P*)b, (T*)y, mean, rstd, M, C, eps, st)
-                  : norm_fwd_run<T, P, 1>(s, (const T*)x, xs, (const P*)w, (const P*)b, (T*)y, mean, rstd, M, C, eps, st);
-}
-
-template <typename T, typename P, int V>
-int norm_bwd_run(const NormShape& s, const T* dy, int64_t dys, const T* x, int64_t xs, const P* w, const float* mean, const float* rstd,
-                 T* dx, P* dw, P* db, float* part, int64_t M, int C, hipStream_t st) {
-  const bool params = dw || db;
-  int blocks = 0;
-  const int rc = norm_dispatch<T, P, V>(s, [&](auto tpr, auto nch) {
+  return norm_dispatch<V, true>(s, [&](auto tpr, auto nch) {
     constexpr int TPR = decltype(tpr)::value, NCH = decltype(nch)::value, RPB = TPR < 256 ? 256 / TPR : 1;
-    const int64_t need = (M + RPB - 1) / RPB;
-    blocks = (int)(need < NORM_BWD_BLOCKS ? need : NORM_BWD_BLOCKS);
-    layer_norm_bwd_kernel<T, P, V, TPR, NCH><<<dim3(blocks), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(
-        dy, dys, x, xs, w, mean, rstd, dx, params ? part : nullptr, M, C);
-    return launched("dm_layer_norm_backward");
+    const dim3 grid(norm_grid((M + RPB - 1) / RPB)), block(TPR < 256 ? 256 : TPR);
+    if (C % V == 0) layer_norm_kernel<T, P, true, TPR, NCH><<<grid, block, 0, st>>>(x, xs, w, b, y, mean, rstd, M, C, eps);
+    else layer_norm_kernel<T, P, false, TPR, NCH><<<grid, block, 0, st>>>(x, xs, w, b, y, mean, rstd, M, C, eps);
+    return launched("dm_layer_norm");
   });
-  if (rc || !params) return rc;
-  partial_rows_kernel<P><<<dim3((unsigned)((2 * (int64_t)C + 15) / 16)), dim3(256), 0, st>>>(part, blocks, C, dw, db);
-  return launched("dm_layer_norm_backward");
 }
 
 template <typename T, typename P>
-int norm_bwd(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, const float* mean, const float* rstd, void* dx,
-             void* dw, void* db, float* part, int64_t M, int C, hipStream_t st) {
+int norm_bwd(const void* dyp, int64_t dys, const void* xp, int64_t xs, const void* wp, const float* mean, const float* rstd, void* dxp,
+             void* dwp, void* dbp, float* part, int64_t M, int C, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = C % V == 0 && xs % V == 0 && dys % V == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) &&
-                   (!w || aligned(w, V * sizeof(P)));
-  const NormShape s = norm_shape(C, V, vec, 4, false);
+  const T *dy = (const T*)dyp, *x = (const T*)xp;
+  const P* w = (const P*)wp;
+  T* dx = (T*)dxp;
+  P *dw = (P*)dwp, *db = (P*)dbp;
+  const bool params = dw || db;
+  const NormShape s = norm_shape(C, V, 16 / V, 512);
+  int rc, rows = 0;  // of `part`
   if (!s.TPR) {
-    layer_norm_bwd_wide_kernel<T, P><<<dim3(norm_grid(M)), dim3(1024), 0, st>>>((const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd,
-                                                                              (T*)dx, M, C);
-    int rc = launched("dm_layer_norm_backward");
-    if (rc || !(dw || db)) return rc;
-    const int rows = (int)(M < 64 ? M : 64);
-    layer_norm_bwd_wide_params_kernel<T><<<dim3((unsigned)((C + 255) / 256), rows), dim3(256), 0, st>>>((const T*)dy, dys, (const T*)x, xs, mean,
-                                                                                             rstd, part, M, C);
-    if ((rc = launched("dm_layer_norm_backward"))) return rc;
-    partial_rows_kernel<P><<<dim3((unsigned)((2 * (int64_t)C + 15) / 16)), dim3(256), 0, st>>>(part, rows, C, (P*)dw, (P*)db);
-    return launched("dm_layer_norm_backward");
+    const dim3 grid(norm_grid(M)), block(1024);
+    if (C < V) layer_norm_bwd_wide_kernel<T, P, 1><<<grid, block, 0, st>>>(dy, dys, x, xs, w, mean, rstd, dx, M, C);
+    else layer_norm_bwd_wide_kernel<T, P, V><<<grid, block, 0, st>>>(dy, dys, x, xs, w, mean, rstd, dx, M, C);
+    rc = launched("dm_layer_norm_backward");
+    if (rc || !params) return rc;
+    rows = (int)(M < 256 ? M : 256);
+    if (C < V) layer_norm_bwd_wide_params_kernel<T, 1><<<dim3(1, rows), dim3(256), 0, st>>>(dy, dys, x, xs, mean, rstd, part, M, C);
+    else layer_norm_bwd_wide_params_kernel<T, V><<<dim3((C + 256 * V - 1) / (256 * V), rows), dim3(256), 0, st>>>(dy, dys, x, xs, mean, rstd, part, M, C);
+    rc = launched("dm_layer_norm_backward");
+  } else {
+    rc = norm_dispatch<V, false>(s, [&](auto tpr, auto nch) {
+      constexpr int TPR = decltype(tpr)::value, NCH = decltype(nch)::value, RPB = TPR < 256 ? 256 / TPR : 1;
+      const int64_t need = (M + RPB - 1) / RPB;
+      rows = (int)(need < norm_bwd_blocks(M) ? need : norm_bwd_blocks(M));
+      layer_norm_bwd_kernel<T, P, TPR, NCH><<<dim3(rows), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(dy, dys, x, xs, w, mean, rstd, dx,
+                                                                                              params ? part : nullptr, M, C);
+      return launched("dm_layer_norm_backward");
+    });
   }
-  return s.V == V ? norm_bwd_run<T, P, V>(s, (const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd, (T*)dx, (P*)dw, (P*)db, part, M, C, st)
-                  : norm_bwd_run<T, P, 1>(s, (const T*)dy, dys, (const T*)x, xs, (const P*)w, mean, rstd, (T*)dx, (P*)dw, (P*)db, part, M, C, st);
+  if (rc || !params) return rc;
+  partial_rows_kernel<P><<<dim3((unsigned)((2 * (int64_t)C + 15) / 16)), dim3(256), 0, st>>>(part, rows, C, dw, db);
+  return launched("dm_layer_norm_backward");
 }
 
 template <typename P>
@@ -377,7 +503,7 @@ int dm_layer_norm(const void* x_dev, int64_t x_stride, const void* weight_dev, c
 
 size_t dm_layer_norm_backward_workspace_bytes(int64_t M, int C) {
   if (M <= 0 || C < 1) return 0;
-  return (size_t)(M < dmb::NORM_BWD_BLOCKS ? M : dmb::NORM_BWD_BLOCKS) * 2 * (size_t)C * sizeof(float);
+  return (size_t)dmb::norm_bwd_blocks(M) * 2 * (size_t)C * sizeof(float);
 }
 
 int dm_layer_norm_backward(const void* dy_dev, int64_t dy_stride, const void* x_dev, int64_t x_stride, const void* weight_dev,

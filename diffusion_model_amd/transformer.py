@@ -48,17 +48,18 @@ def _vector(t, n, x, name, dtypes=None):
     return t.contiguous()
 
 
-def _rows(t):
-    """[..., C] as rows the kernels can read: (tensor, row stride in elements, number of rows)."""
+def _rows(t, pieces=True):
+    """[..., C] as rows the kernels can read: (tensor, row stride in elements, number of rows).  ``pieces``: rows of whole 16-byte pieces
+    start at multiples of 16 bytes."""
     c = t.shape[-1]
     if t.is_contiguous():
-        if t.data_ptr() % 16 == 0:
+        if not pieces or t.data_ptr() % 16 == 0:
             return t, c, t.numel() // c
         return t.clone(), c, t.numel() // c
     r = t.reshape(-1, c)
     m, whole = r.shape[0], 16 // t.element_size()
     if (c > 1 and r.stride(1) != 1) or (m > 1 and (r.stride(0) < c or r.stride(0) > 1 << 21)) or \
-            (c % whole == 0 and (r.data_ptr() % 16 or (m > 1 and r.stride(0) % whole))):
+            (pieces and c % whole == 0 and (r.data_ptr() % 16 or (m > 1 and r.stride(0) % whole))):
         r = r.clone(memory_format=torch.contiguous_format)
     return r, (r.stride(0) if m > 1 else c), m
 
@@ -109,7 +110,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     p = x if w is None and b is None else b if w is None else w
-    r, stride, m = _rows(x)
+    r, stride, m = _rows(x, False)
     y = _empty_like(x)
     mean = rstd = None
     if return_stats:
@@ -134,8 +135,8 @@ def layer_norm_backward(grad, x, weight, mean, rstd):
         if t.shape != x.shape[:-1]:
             raise RuntimeError(f"{name} must be {tuple(x.shape[:-1])} (got {tuple(t.shape)})")
     L = _lib.lib()
-    r, stride, m = _rows(x)
-    g, gstride, _ = _rows(grad)
+    r, stride, m = _rows(x, False)
+    g, gstride, _ = _rows(grad, False)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     dx = _empty_like(x)
     dw = db = ws = None

@@ -312,7 +312,7 @@ enum { DM_F32 = 0, DM_BF16 = 1, DM_F16 = 2 };
 enum { DM_ACT_SILU = 0, DM_ACT_GELU = 1 /* erf */, DM_ACT_GELU_TANH = 2, DM_ACT_RELU = 3, DM_ACT_SIGMOID = 4 };
 
 /* y[m,:] = (x[m,:] - mean) rstd weight + bias over rows of C elements, rstd = 1/sqrt(var + eps), var the biased variance.
- * x rows are x_stride elements apart.  weight, bias: [C] of x's type or fp32 (param_dtype), either may be NULL.
+ * x rows are x_stride elements apart, at any element boundary.  weight, bias: [C] of x's type or fp32 (param_dtype), either may be NULL.
  * mean_dev, rstd_dev: [M] fp32 for the backward pass, or NULL.  M == 0 does nothing. */
 int dm_layer_norm(const void* x_dev, int64_t x_stride, const void* weight_dev, const void* bias_dev, int param_dtype,
                   void* y_dev, float* mean_dev, float* rstd_dev, int64_t M, int C, float eps, int dtype, void* stream);
@@ -329,7 +329,7 @@ int dm_layer_norm_backward(const void* dy_dev, int64_t dy_stride, const void* x_
  * scaled by `scale`: elements (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`.  Elements from rotary_dim on are
  * copied.  positions int64 with strides (axis, image, token) in elements, or NULL for 0 .. T-1; with `axes` > 1 pair i takes
  * the axis i / (pairs / axes).  `inverse` turns back: the gradient of the forward call.  out == in (same strides) works in
- * place; otherwise the two may not overlap. */
+ * place (q and k may share no elements then); otherwise the two may not overlap. */
 typedef struct {
   const void* in;
   void* out;

@@ -501,3 +501,89 @@ def test_operators_on_two_streams_at_once():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+# ------------------------------------------------------------------ rows and sizes where a kernel's last piece, tile or step is not whole
+
+def _norm_bounds(x, w, b, dy, dt):
+    """(name, value, bound) of y, dx, dw, db; the bounds are those of test_layer_norm_forward_and_backward."""
+    y, z, _, rstd, gz, dx, dw, db = norm_oracle(x, w, b, 1e-5, dy)
+    e = 64 * 2.0 ** -24
+    xa = x.double().abs()
+    ez = e * ((xa + xa.mean(-1, keepdim=True)) * rstd[:, None] + 1 + z.abs())
+    span = rstd[:, None] * (gz.abs() + gz.abs().mean(-1, keepdim=True) + z.abs() * (gz * z).abs().mean(-1, keepdim=True))
+    drift = rstd[:, None] * (ez * (gz * z).abs().mean(-1, keepdim=True) + z.abs() * (gz.abs() * ez).mean(-1, keepdim=True))
+    ga = dy.double().abs()
+    tiny = 1e-7 * (dt == torch.float16)
+    return (("y", y, HALF[dt] * y.abs() + ez * w.double().abs() + e * b.double().abs() + tiny),
+            ("dx", dx, HALF[dt] * dx.abs() + 2 * e * span + 2 * drift + tiny),
+            ("dw", dw, HALF[w.dtype] * dw.abs() + (ga * (ez + e * z.abs())).sum(0) + tiny), ("db", db, HALF[w.dtype] * db.abs() + e * ga.sum(0) + tiny))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("width", [3, 4, 9, 15, 33, 127, 511, 1001, 1032, 4097, 5000, 12289, 16385, 32769])
+def test_layer_norm_rows_between_others(width, dtype):
+    """Rows of any width at any element of a wider array whose other elements are NaN, parameters off 16-byte boundaries: nothing beside a
+    row is read into its results, and a row behind the last one is not written."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(width + 1)
+    rows = 41 if width < 6000 else 6
+    x, dy = rand(g, rows, width, dtype=dt, scale=1.5, shift=0.5), rand(g, rows, width, dtype=dt)
+    w, b = rand(g, width, dtype=dt, scale=0.2, shift=1.0), rand(g, width, dtype=dt)
+    nan = float("nan")
+    flat = torch.full((rows + 1, width + 5), nan, dtype=dt, device=DEV)
+    gflat = torch.full((rows, width + 3), nan, dtype=dt, device=DEV)
+    wb = torch.full((2, width + 1), nan, dtype=dt, device=DEV)
+    xd, dyd, wd, bd = flat[:rows, 1:1 + width], gflat[:, 3:], wb[0, 1:], wb[1, :width]
+    for view, t in ((xd, x), (dyd, dy), (wd, w), (bd, b)):
+        view.copy_(t)
+    y, mu, rs = d.layer_norm(xd, wd, bd, return_stats=True)
+    got = (y, *d.layer_norm_backward(dyd, xd, wd, mu, rs))
+    for (name, want, tol), t in zip(_norm_bounds(x, w, b, dy, dt), got):
+        close(t, want, tol, f"{name} {rows}x{width}")
+    # the library's own entry point, into the middle of an array: what lies around the rows stays
+    out = torch.full((rows + 2, width), 7.0, dtype=dt, device=DEV)
+    code = {"fp32": 0, "bf16": 1, "fp16": 2}[dtype]
+    _lib.check(_lib.lib().dm_layer_norm(xd.data_ptr(), xd.stride(0), wd.data_ptr(), bd.data_ptr(), code, out[1].data_ptr(), None, None, rows, width,
+                                        1e-5, code, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out[1:-1], y) and (out[0] == 7).all() and (out[-1] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(5000, 72, 88, 40), (300, 1100, 1544, 1100), (9, 600, 1200, 600), (520, 136, 2056, 24), (2100, 24, 16, 8), (70, 4100, 24, 520)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_ffn_long_and_ragged_ranges(size, dtype):
+    """Long sums of no whole steps, whole or dealt among several workgroups, with every bias' gradient; bounds as in
+    test_gated_ffn_forward_and_backward."""
+    m, dd, f, n = size
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(m + n)
+    x, dy, w, b = ffn_case(g, m, dd, f, n, dt, True)
+    res, exact, rounded = ffn_oracle(x, dy, w, b, "silu")
+    xd, dyd, wd, bd = x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+    y, saved = d.gated_ffn(xd, *wd, *bd, save=True)
+    got = (y, *d.gated_ffn_backward(dyd, xd, *wd, saved, bias=True))
+    e = 2.0 ** -24 * (32 + max(dd, f, n, m) / 8)
+    for name, t in zip(("y", "dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down"), got):
+        close(t, res[name], HALF[dt] * res[name].abs() + e * exact[name] + (HALF[dt] * 1.01 * rounded[name] if dt != torch.float32 else 0), f"{name} {size}")
+
+
+def test_rotary_of_one_tensor_as_query_and_key():
+    g = torch.Generator().manual_seed(4)
+    x = rand(g, 1, 5, 3, 16).to(DEV)
+    inv = d.rotary_frequencies(16)[0].to(DEV)
+    q, k = d.apply_rotary(x, x, inv)
+    assert torch.equal(q, k) and torch.equal(q, d.apply_rotary(x, None, inv)[0])
+    with pytest.raises(RuntimeError, match="share no elements"):
+        d.apply_rotary(x, x, inv, inplace=True)
+
+
+def test_ffn_of_one_weight_for_both_projections():
+    """The same tensor twice among the inputs, and the gradient's tensor as the input itself."""
+    g = torch.Generator().manual_seed(6)
+    for rows in (3, 80):
+        x, w, wd = rand(g, rows, 32).to(DEV), rand(g, 48, 32, scale=0.2).to(DEV), rand(g, 32, 48, scale=0.2).to(DEV)
+        y, saved = d.gated_ffn(x, w, w, wd, save=True)
+        assert torch.equal(y, d.gated_ffn(x, w, w.clone(), wd))
+        a, b = d.gated_ffn_backward(x, x, w, w, wd, saved), d.gated_ffn_backward(x.clone(), x, w, w.clone(), wd, saved)
+        assert all(torch.equal(p, q) for p, q in zip(a[:4], b[:4]))
