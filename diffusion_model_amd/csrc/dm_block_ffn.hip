@@ -2,11 +2,15 @@
 //   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) u, y = h Wd^T + bd
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h, biases: column sums.
 // Both projections, the activation and the product are one kernel; so are dh, dg and du: for training the forward pass keeps u act'(g),
-// act(g) and h, three values where g and u would be two, so that none is rounded twice and nothing is computed again.  Two paths: up to SKINNY_ROWS rows (decode) the weights' bandwidth bounds the block and
-// every wave streams weight rows straight into matrix instructions; above that the tiled products of dm_block_gemm.hip.
-// Rounding: h, u act'(g), act(g), dg and du are kept in the tensors' type between the products (16-bit: the matrix pipe takes nothing wider), every
-// sum is fp32.  fp32 tensors are split into three bf16 terms and multiplied as six products (a1b1 a1b2 a2b1 a2b2 a1b3 a3b1; what is left
-// out is below 2^-25 of |a||b|).
+// act(g) and h, three values where g and u would be two, so that none is rounded twice and nothing is computed again.
+// Three paths.  Up to TOKEN_ROWS rows, and fp32 up to SKINNY_ROWS, the weights' bandwidth bounds the block, and every wave streams weight rows
+// straight into vector (gemv_kernel) or matrix (skinny_kernel) instructions; above that the tiled products of dm_block_gemm.hip, whose
+// smallest tile and split k range serve 16-bit decode batches.
+// Rounding: h, u act'(g), act(g), dg and du are kept in the tensors' type between the products.  The matrix pipe takes h, dg and du in
+// 16 bits and nothing wider; u act'(g) and act(g) are 16 bits for their bytes (32 would add 0.7 GB to a step of 8192 x 4096 x 11008, 3 % of
+// its time): a gradient has three roundings where results alone would have one, sqrt(3) of its error.  Every sum is fp32.
+// fp32 tensors are split into three bf16 terms and multiplied as six products (a1b1 a1b2 a2b1 a2b2 a1b3 a3b1; what is left out is below
+// 2^-25 of |a||b|): the fp32 matrix instructions have 1/16 of the bf16 ones' rate.
 #include <type_traits>
 
 #include "dm_block_gemm.hip"
@@ -17,34 +21,48 @@ constexpr int TOKEN_ROWS = 4;  // gemv_kernel
 constexpr int SKINNY_ROWS = 64;  // skinny_kernel, fp32
 
 // ---- operands that the products cannot read as they are: fp32 (three bf16 planes) and rows of no whole number of 16-byte pieces
-template <typename S, typename D, bool PLANES>
-__global__ void __launch_bounds__(256)
-pack_rows_kernel(const S* __restrict__ src, int64_t ld, D* __restrict__ dst, int64_t plane, int64_t rows, int cols, int pitch) {
-  const int pieces = pitch / 8;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < rows * pieces; id += (int64_t)gridDim.x * 256) {
-    const int64_t r = id / pieces;
-    const int c = (int)(id % pieces) * 8;
-    const S* s = src + r * ld + c;
-    S v[8];
-    if (sizeof(S) == 4 && c + 8 <= cols && ((uintptr_t)s & 15) == 0) {
-      const Vec<S, 4> a = *reinterpret_cast<const Vec<S, 4>*>(s), b = *reinterpret_cast<const Vec<S, 4>*>(s + 4);
+struct PackJob { const void* src; void* dst; int64_t ld, plane, rows, block0; int cols, pitch; };  // block0: the first of its blocks
+struct PackJobs { PackJob job[5]; int count; int64_t blocks; };
+constexpr int PACK_PIECES = 1024;  // of eight elements, per block
+
+// All matrices of a call in one launch: bound by memory, and by the launch where they are small.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const PackJobs jobs) {
+  constexpr bool PLANES = sizeof(T) == 4;
+  using D = typename std::conditional<PLANES, bf16, T>::type;
+  PackJob a = jobs.job[0];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { v[i] = a.v[i]; v[4 + i] = b.v[i]; }
+  for (int i = 1; i < 5; ++i)
+    if (i < jobs.count && blockIdx.x >= jobs.job[i].block0) a = jobs.job[i];
+  const int pieces = a.pitch / 8;
+  const int64_t piece0 = (blockIdx.x - a.block0) * PACK_PIECES, row0 = piece0 / pieces;
+  const unsigned rest = (unsigned)(piece0 - row0 * pieces);
+#pragma unroll
+  for (int k = 0; k < PACK_PIECES / 256; ++k) {
+    const unsigned id = rest + k * 256 + threadIdx.x;
+    const int64_t r = row0 + id / (unsigned)pieces;
+    const int c = (int)(id % (unsigned)pieces) * 8;
+    if (r >= a.rows) continue;
+    const T* s = (const T*)a.src + r * a.ld + c;
+    Piece<T, 8> v;
+    if (c + 8 <= a.cols) {
+      v = *reinterpret_cast<const Piece<T, 8>*>(s);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? s[i] : (S)0.f;
+      for (int i = 0; i < 8; ++i) v.v[i] = c + i < a.cols ? s[i] : (T)0.f;
     }
+    D* dst = (D*)a.dst + r * a.pitch + c;
     if constexpr (PLANES) {
       Vec<bf16, 8> o[3];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { bf16 t[3]; split3((float)v[i], t); o[0].v[i] = t[0]; o[1].v[i] = t[1]; o[2].v[i] = t[2]; }
+      for (int i = 0; i < 8; ++i) { bf16 t[3]; split3((float)v.v[i], t); o[0].v[i] = t[0]; o[1].v[i] = t[1]; o[2].v[i] = t[2]; }
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<bf16, 8>*>(dst + k * plane + r * pitch + c) = o[k];
+      for (int j = 0; j < 3; ++j) *reinterpret_cast<Vec<bf16, 8>*>(dst + j * a.plane) = o[j];
     } else {
       Vec<D, 8> o;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o.v[i] = (D)v[i];
-      *reinterpret_cast<Vec<D, 8>*>(dst + r * pitch + c) = o;
+      for (int i = 0; i < 8; ++i) o.v[i] = v.v[i];
+      *reinterpret_cast<Vec<D, 8>*>(dst) = o;
     }
   }
 }
@@ -78,7 +96,7 @@ __device__ __forceinline__ void finish_gate(const Streamed<T>& p, int n, int64_t
   }
 }
 
-// ---- up to TOKEN_ROWS rows: the weights' bandwidth.  A wave takes R rows of w (and of w2) and multiplies them with all of x in vector
+// ---- up to TOKEN_ROWS rows: the weights' bandwidth (one token through 4096 x 11008 bf16: 47 us, 5.8 TB/s of 270 MB; fp32 99 us).  A wave takes R rows of w (and of w2) and multiplies them with all of x in vector
 // instructions, a row's piece of 64 V elements per load; the KSPLIT waves that share rows split the k range and meet in LDS.
 template <int NV>  // v[i] summed over the wave; lane l < NV gets the i = l-th sum
 __device__ __forceinline__ float wave_sums(float (&v)[NV], int lane) {
@@ -99,10 +117,10 @@ __device__ __forceinline__ float wave_sums(float (&v)[NV], int lane) {
   return s;
 }
 
-template <typename T, int MR, bool GATE, int V, int KSPLIT>
+template <typename T, int MR, bool GATE, int KSPLIT>
 __global__ void __launch_bounds__(256)
 gemv_kernel(const Streamed<T> p) {
-  constexpr int R = 4, P = GATE ? 2 : 1, GROUPS = 4 / KSPLIT, NV = MR * R;
+  constexpr int V = 16 / sizeof(T), R = 4, P = GATE ? 2 : 1, GROUPS = 4 / KSPLIT, NV = MR * R;
   __shared__ float red[KSPLIT > 1 ? KSPLIT : 1][GROUPS][P][NV];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave / KSPLIT, part = wave % KSPLIT;
   const int n0 = (blockIdx.x * GROUPS + group) * R;
@@ -114,24 +132,28 @@ gemv_kernel(const Streamed<T> p) {
     if (GATE) rows[P - 1][r] = p.w2 + n * p.ldw;
   }
   float acc[P][NV] = {};
-#pragma unroll 2
-  for (int k = part * 64 * V + lane * V; k < p.K; k += KSPLIT * 64 * V) {
-    Vec<T, V> a[P][R], b[MR];
+  auto multiply = [&](int k, auto pieces) __attribute__((always_inline)) {  // a piece of every row from k on
+    constexpr int N = decltype(pieces)::value;
+    Piece<T, N> a[P][R], b[MR];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int q = 0; q < P; ++q) a[q][r] = *reinterpret_cast<const Vec<T, V>*>(rows[q][r] + k);
+      for (int q = 0; q < P; ++q) a[q][r] = *reinterpret_cast<const Piece<T, N>*>(rows[q][r] + k);
 #pragma unroll
-    for (int m = 0; m < MR; ++m) b[m] = *reinterpret_cast<const Vec<T, V>*>(p.x + (m < p.M ? m : p.M - 1) * p.xs + k);
+    for (int m = 0; m < MR; ++m) b[m] = *reinterpret_cast<const Piece<T, N>*>(p.x + (m < p.M ? m : p.M - 1) * p.xs + k);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int q = 0; q < P; ++q)
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
           for (int m = 0; m < MR; ++m) acc[q][m * R + r] = fmaf((float)a[q][r].v[i], (float)b[m].v[i], acc[q][m * R + r]);
-  }
+  };
+  const int whole = p.K / V * V;
+#pragma unroll 2
+  for (int k = part * 64 * V + lane * V; k < whole; k += KSPLIT * 64 * V) multiply(k, std::integral_constant<int, V>{});
+  if (part == 0 && lane < p.K - whole) multiply(whole + lane, std::integral_constant<int, 1>{});
   float s[P];
 #pragma unroll
   for (int q = 0; q < P; ++q) s[q] = wave_sums<NV>(acc[q], lane);
@@ -155,14 +177,14 @@ gemv_kernel(const Streamed<T> p) {
   else if (n < p.N) p.out[at] = (T)(s[0] + (p.bias ? (float)p.bias[n] : 0.f));
 }
 
-template <typename T, bool GATE, int V>
+template <typename T, bool GATE>
 int gemv_launch(const Streamed<T>& a, hipStream_t st) {
   const int groups = (int)(((int64_t)a.N + 7) / 8 * 8 + 3) / 4;  // of four rows, the padding of h among them
   int split = 1;  // sixteen waves for every CU, as long as each has a load of its own
-  while (split < 4 && groups * split < 4096 && a.K > split * 64 * V) split *= 2;
+  while (split < 4 && groups * split < 4096 && a.K > split * 64 * (int)(16 / sizeof(T))) split *= 2;
   auto run = [&](auto mr, auto ks) {
     constexpr int MR = decltype(mr)::value, KS = decltype(ks)::value;
-    gemv_kernel<T, MR, GATE, V, KS><<<dim3((groups + 4 / KS - 1) / (4 / KS)), dim3(256), 0, st>>>(a);
+    gemv_kernel<T, MR, GATE, KS><<<dim3((groups + 4 / KS - 1) / (4 / KS)), dim3(256), 0, st>>>(a);
   };
   auto rows = [&](auto ks) {
     if (a.M == 1) run(std::integral_constant<int, 1>{}, ks);
@@ -175,25 +197,24 @@ int gemv_launch(const Streamed<T>& a, hipStream_t st) {
   return launched("dm_gated_ffn");
 }
 
-// ---- fp32, up to SKINNY_ROWS rows
+// ---- fp32, up to SKINNY_ROWS rows (of 4 elements or more): 16 rows of 2048 x 5504 52 us (2.6 TB/s of 135 MB), 64 rows 112 us.  Tiles of
+// split operands would first write three planes of every weight.
 // Four instructions of four k each: instruction i takes element i of every lane's piece, on both sides.
-__device__ __forceinline__ f32x4 mfma_f32(const Vec<float, 4>& a, const Vec<float, 4>& b, f32x4 c) {
+__device__ __forceinline__ f32x4 mfma_f32(const Piece<float, 4>& a, const Piece<float, 4>& b, f32x4 c) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
   return c;
 }
 
-__device__ __forceinline__ Vec<float, 4> load_piece(const float* row, int k, int K, bool vec) {
-  Vec<float, 4> r;
-  if (vec) {
-    if (k < K) return *reinterpret_cast<const Vec<float, 4>*>(row + k);
+// Elements k .. k + 3 of a row of K >= 4; the row's last ones are a load moved back to end with the row, of which what lies before k counts
+// as zero (`behind`, once the load has arrived): both sides of a product place them alike.
+__device__ __forceinline__ Piece<float, 4> load_piece(const float* row, int k, int K) {
+  return *reinterpret_cast<const Piece<float, 4>*>(row + (k + 4 <= K ? k : K - 4));
+}
+__device__ __forceinline__ Piece<float, 4> behind(Piece<float, 4> v, int k, int K) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = 0.f;
-    return r;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r.v[i] = k + i < K ? row[k + i] : 0.f;
-  return r;
+  for (int i = 0; i < 4; ++i) v.v[i] = k + 4 <= K || K - 4 + i >= k ? v.v[i] : 0.f;
+  return v;
 }
 
 constexpr int SKINNY_WAVES = 8;
@@ -201,7 +222,7 @@ constexpr int SKINNY_WAVES = 8;
 // out[m, n] for 16 n per block: the waves deal the k range among themselves in chunks, and their sums meet in LDS.  A chunk is U pieces
 // of every row (U * 64 bytes on end), and the next chunk is on its way while one is multiplied.  Blocks begin at different chunks: in
 // step they would all ask for the same columns of rows a power of two apart, which lie on few of the memory's channels.
-template <int MT, bool GATE, bool VEC>
+template <int MT, bool GATE>
 __global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const Streamed<float> p) {
   constexpr int V = 4, STEP = 4 * V, P = GATE ? 2 : 1;
   constexpr int U = MT == 4 ? 2 : 4;
@@ -218,30 +239,36 @@ __global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const Streame
     xr[t] = p.x + (m < p.M ? m : p.M - 1) * p.xs;
   }
   f32x4 acc[P][MT] = {};
-  struct Chunk { Vec<float, V> a[P][U], b[U][MT]; } one, two;
+  struct Chunk { Piece<float, V> a[P][U], b[U][MT]; int k; } one, two;  // k: of its first piece
   const int chunks = (p.K + U * STEP - 1) / (U * STEP), turn = (int)(blockIdx.x * 7u % (unsigned)chunks);
   auto load = [&](Chunk& c, int at) __attribute__((always_inline)) {
     if (at >= chunks) return;
     at += turn;
     if (at >= chunks) at -= chunks;
-    const int k0 = at * U * STEP + (lane >> 4) * V;
+    c.k = at * U * STEP;
+    const int k0 = c.k + (lane >> 4) * V;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      c.a[0][i] = load_piece(w1r, k0 + i * STEP, p.K, VEC);
-      if (GATE) c.a[P - 1][i] = load_piece(w2r, k0 + i * STEP, p.K, VEC);
+      c.a[0][i] = load_piece(w1r, k0 + i * STEP, p.K);
+      if (GATE) c.a[P - 1][i] = load_piece(w2r, k0 + i * STEP, p.K);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) c.b[i][t] = load_piece(xr[t], k0 + i * STEP, p.K, VEC);
+      for (int t = 0; t < MT; ++t) c.b[i][t] = load_piece(xr[t], k0 + i * STEP, p.K);
   };
   auto multiply = [&](const Chunk& c) __attribute__((always_inline)) {
+    const bool last = c.k + U * STEP > p.K;
 #pragma unroll
-    for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i) {
+      const int k = c.k + (lane >> 4) * V + i * STEP;
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) {
+        const Piece<float, V> b = last ? behind(c.b[i][t], k, p.K) : c.b[i][t];
 #pragma unroll
-        for (int q = 0; q < P; ++q) acc[q][t] = mfma_f32(c.a[q][i], c.b[i][t], acc[q][t]);
+        for (int q = 0; q < P; ++q) acc[q][t] = mfma_f32(last ? behind(c.a[q][i], k, p.K) : c.a[q][i], b, acc[q][t]);
+      }
+    }
   };
   int at = wave;
   load(one, at);
@@ -278,22 +305,20 @@ __global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const Streame
   }
 }
 
-template <bool GATE, bool VEC>
+template <bool GATE>
 int skinny_launch(const Streamed<float>& a, hipStream_t st) {
   const dim3 grid((a.N + 15) / 16), block(SKINNY_WAVES * 64);
-  if (a.M <= 16) skinny_kernel<1, GATE, VEC><<<grid, block, 0, st>>>(a);
-  else if (a.M <= 32) skinny_kernel<2, GATE, VEC><<<grid, block, 0, st>>>(a);
-  else skinny_kernel<4, GATE, VEC><<<grid, block, 0, st>>>(a);
+  if (a.M <= 16) skinny_kernel<1, GATE><<<grid, block, 0, st>>>(a);
+  else if (a.M <= 32) skinny_kernel<2, GATE><<<grid, block, 0, st>>>(a);
+  else skinny_kernel<4, GATE><<<grid, block, 0, st>>>(a);
   return launched("dm_gated_ffn");
 }
 
 template <typename T, bool GATE>
 int streamed(const Streamed<T>& a, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const bool whole = a.K % V == 0;  // (rows start at multiples of 16 bytes then: ffn_check_matrix)
   if constexpr (std::is_same<T, float>::value)
-    if (a.M > TOKEN_ROWS) return whole ? skinny_launch<GATE, true>(a, st) : skinny_launch<GATE, false>(a, st);
-  return whole ? gemv_launch<T, GATE, V>(a, st) : gemv_launch<T, GATE, 1>(a, st);
+    if (a.M > TOKEN_ROWS) return skinny_launch<GATE>(a, st);
+  return gemv_launch<T, GATE>(a, st);
 }
 
 // ---- workspace
@@ -313,31 +338,25 @@ struct Operand { const void* p; int64_t ld, plane; };
 struct FfnSizes { int64_t M; int D, F, N, dtype; };
 
 template <typename T>
-int pack_launch(const void* src, int64_t ld, void* dst, int64_t plane, int64_t rows, int cols, hipStream_t st) {
-  const int pitch = (int)round_up(cols, 8);
-  const int64_t blocks = (rows * (pitch / 8) + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
-  if constexpr (std::is_same<T, float>::value)
-    pack_rows_kernel<float, bf16, true><<<grid, dim3(256), 0, st>>>((const float*)src, ld, (bf16*)dst, plane, rows, cols, pitch);
-  else
-    pack_rows_kernel<T, T, false><<<grid, dim3(256), 0, st>>>((const T*)src, ld, (T*)dst, plane, rows, cols, pitch);
+int pack_launch(const PackJobs& jobs, hipStream_t st) {
+  if (!jobs.count) return 0;
+  if (jobs.blocks > (1LL << 24)) return fail("gated feed-forward block: operands of %lld elements to pack", (long long)jobs.blocks * PACK_PIECES * 8);
+  pack_rows_kernel<T><<<dim3((unsigned)jobs.blocks), dim3(256), 0, st>>>(jobs);
   return launched("gated feed-forward block");
 }
 
-// Takes room for the packed form of a [rows][cols] matrix where the products cannot read it as it lies, and (launch) fills it.
+// Takes room for the packed form of a [rows][cols] matrix where the products cannot read it as it lies; `needed`: it is to be packed.
 template <typename T>
-int prepare_operand(Operand& o, const void* src, int64_t ld, int64_t rows, int cols, Carver& ws, bool launch, hipStream_t st) {
+Operand prepare_operand(PackJobs& jobs, const void* src, int64_t ld, int64_t rows, int cols, Carver& ws, bool needed = true) {
   constexpr bool F32 = std::is_same<T, float>::value;
-  if (!F32 && cols % 8 == 0) {
-    o = {src, ld, 0};
-    return 0;
-  }
+  if (!F32 && cols % 8 == 0) return {src, ld, 0};
   const int64_t pitch = round_up(cols, 8);
-  o.ld = pitch;
-  o.plane = rows * pitch;
   void* p = ws.take((size_t)(F32 ? 3 : 1) * rows * pitch * 2);
-  o.p = p;
-  return launch ? pack_launch<T>(src, ld, p, o.plane, rows, cols, st) : 0;
+  if (needed) {
+    jobs.job[jobs.count++] = {src, p, ld, rows * pitch, rows, jobs.blocks, cols, (int)pitch};
+    jobs.blocks += (rows * (pitch / 8) + PACK_PIECES - 1) / PACK_PIECES;
+  }
+  return {p, pitch, rows * pitch};
 }
 template <typename T>
 Operand take_operand(int64_t rows, int cols, Carver& ws) {
@@ -418,7 +437,7 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   constexpr bool F32 = std::is_same<T, float>::value;
   const int64_t Fp = pad8(z.F);
   const Saved<T> kept(saved, z.M, z.F);
-  if (z.M <= TOKEN_ROWS || (F32 && z.M <= SKINNY_ROWS)) {
+  if (z.M <= TOKEN_ROWS || (F32 && z.M <= SKINNY_ROWS && z.D >= 4 && z.F >= 4)) {
     T* h = saved && !F32 ? (T*)kept.h.p : (T*)ws.take((size_t)z.M * Fp * sizeof(T));
     if (!run) return 0;
     const int M = (int)z.M;
@@ -428,18 +447,17 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
     const Streamed<T> down = {h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, M, z.N, z.F, act};
     return streamed<T, false>(down, st);
   }
-  Operand x, wg, wu, wd, h;
-  int rc = prepare_operand<T>(x, in.x, in.xs, z.M, z.D, ws, run, st);
-  if (!rc) rc = prepare_operand<T>(wg, in.wg, z.D, z.F, z.D, ws, run, st);
-  if (!rc) rc = prepare_operand<T>(wu, in.wu, z.D, z.F, z.D, ws, run, st);
-  if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
-  if (rc) return rc;
-  h = saved ? kept.h : take_operand<T>(z.M, z.F, ws);
+  PackJobs jobs = {};
+  const Operand x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws), wg = prepare_operand<T>(jobs, in.wg, z.D, z.F, z.D, ws),
+                wu = prepare_operand<T>(jobs, in.wu, z.D, z.F, z.D, ws), wd = prepare_operand<T>(jobs, in.wd, z.F, z.N, z.F, ws);
+  const Operand h = saved ? kept.h : take_operand<T>(z.M, z.F, ws);
   const int terms = F32 ? 6 : 1;
   const size_t part_bytes = gemm_plan(z.M, z.N, iters_of(z.F), terms, 1, sizeof(T), true).part_bytes;
   const GemmPlan gate = gemm_plan(z.M, z.F, iters_of(z.D), terms, 2, F32 ? 7 : 3, true);
   void* part = ws.take(gate.part_bytes > part_bytes ? gate.part_bytes : part_bytes);  // used by one product after the other
   if (!run) return 0;
+  int rc = pack_launch<T>(jobs, st);
+  if (rc) return rc;
 
   GemmArgs g = {};
   add_terms<T>(g, x, wg);
@@ -465,13 +483,10 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
                  hipStream_t st) {
   const int64_t Fp = pad8(z.F);
   const int terms = std::is_same<T, float>::value ? 6 : 1;
-  Operand x, wg, wu, wd, y;
-  int rc = prepare_operand<T>(y, dy, dys, z.M, z.N, ws, run, st);
-  if (!rc) rc = prepare_operand<T>(wd, in.wd, z.F, z.N, z.F, ws, run, st);
-  if (!rc) rc = prepare_operand<T>(x, in.x, in.xs, z.M, z.D, ws, run && (gr.dwg || gr.dwu), st);
-  if (!rc) rc = prepare_operand<T>(wg, in.wg, z.D, z.F, z.D, ws, run && gr.dx, st);
-  if (!rc) rc = prepare_operand<T>(wu, in.wu, z.D, z.F, z.D, ws, run && gr.dx, st);
-  if (rc) return rc;
+  PackJobs jobs = {};
+  const Operand y = prepare_operand<T>(jobs, dy, dys, z.M, z.N, ws), wd = prepare_operand<T>(jobs, in.wd, z.F, z.N, z.F, ws),
+                x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws, gr.dwg || gr.dwu),
+                wg = prepare_operand<T>(jobs, in.wg, z.D, z.F, z.D, ws, gr.dx), wu = prepare_operand<T>(jobs, in.wu, z.D, z.F, z.D, ws, gr.dx);
   const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws);
   const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
   size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F), terms * 2, 1, sizeof(T), true).part_bytes;
@@ -480,6 +495,8 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
   void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
   if (!run) return 0;
+  int rc = pack_launch<T>(jobs, st);
+  if (rc) return rc;
 
   GemmArgs a = {};  // dh, and from it dg and du
   add_terms<T>(a, y, wd);

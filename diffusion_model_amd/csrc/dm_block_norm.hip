@@ -34,12 +34,7 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[2][TPR > 64 ? TPR
   return v;
 }
 
-// V elements of a row, at any element boundary: the hardware takes such vectors (bf16, 16384 rows of odd width 1001: 16 us against 39 us
-// element by element).
-template <typename T, int V>
-struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[V]; };
-
-// The piece of a row that a thread holds from column c on.  WHOLE (C a multiple of V): the piece lies inside the row or behind it.  Else the
+// The Piece of a row that a thread holds from column c on.  WHOLE (C a multiple of V): the piece lies inside the row or behind it.  Else the
 // last piece is moved back to end with the row: its first `skip` elements are a neighbour's too, which counts them in sums over the row;
 // both write the same values.  Behind the row all of it is skipped.
 template <int V, bool WHOLE>

@@ -342,9 +342,9 @@ int dm_rotary(const dm_rotary_tensor* q, const dm_rotary_tensor* k, const int64_
 
 /* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down: x [M][D] rows x_stride apart, w_gate and w_up [F][D],
  * w_down [N][F], y [M][N], biases [F], [F], [N] or NULL, all of one type.  saved_dev: NULL, or dm_gated_ffn_saved_bytes for the
- * backward pass.  Between its products the block keeps the tensors' type: 16-bit types round h, and for the
- * backward pass u act'(g), act(g), dg and du, there.  fp32 operands
- * are multiplied as three bf16 terms each above 64 rows (an infinite operand gives NaN there, where fp32 would give an infinity).
+ * backward pass.  Between its products the block keeps the tensors' type: 16-bit types round h, and for the backward pass
+ * u act'(g), act(g), dg and du, there.  fp32 operands are multiplied as three bf16 terms each, but for forward passes of few rows
+ * (an infinite operand gives NaN there, where fp32 would give an infinity).
  * Rows of whole 16-byte pieces must start at multiples of 16 bytes. */
 size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype);
 size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype, int save); /* save: with saved_dev */

@@ -587,3 +587,22 @@ def test_ffn_of_one_weight_for_both_projections():
         assert torch.equal(y, d.gated_ffn(x, w, w.clone(), wd))
         a, b = d.gated_ffn_backward(x, x, w, w, wd, saved), d.gated_ffn_backward(x.clone(), x, w, w.clone(), wd, saved)
         assert all(torch.equal(p, q) for p, q in zip(a[:4], b[:4]))
+
+
+@pytest.mark.parametrize("size", [(6, 5, 7, 3), (20, 3, 40, 5), (20, 40, 3, 5), (37, 515, 130, 129), (64, 63, 33, 1), (2, 2, 2, 2), (4, 517, 1031, 9)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_ffn_few_fp32_rows_of_odd_widths(size):
+    """Rows whose last piece is moved back, and rows of less than a piece; inputs between NaN.  Bounds as in
+    test_gated_ffn_forward_and_backward."""
+    m, dd, f, n = size
+    g = torch.Generator().manual_seed(m * dd)
+    x, dy, w, b = ffn_case(g, m, dd, f, n, torch.float32, True)
+    res, exact, _ = ffn_oracle(x, dy, w, b, "gelu")
+    wide = torch.full((m, dd + 3), float("nan"), device=DEV)
+    wide[:, 2:2 + dd] = x.to(DEV)
+    xd, dyd, wd, bd = wide[:, 2:2 + dd], dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+    y, saved = d.gated_ffn(xd, *wd, *bd, activation="gelu", save=True)
+    got = (y, *d.gated_ffn_backward(dyd, xd, *wd, saved, activation="gelu", bias=True))
+    e = 2.0 ** -24 * (32 + max(size) / 8)
+    for name, t in zip(("y", "dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down"), got):
+        close(t, res[name], 2.0 ** -24 * res[name].abs() + e * exact[name], f"{name} {size}")
