@@ -4,6 +4,8 @@
 // registers, no cancellation) follow from there, and the result is written once.  All sums are fp32.  The parameters'
 // gradients are summed per workgroup over the rows it walks, written as partial rows and added in a fixed order by a second
 // launch: no atomics, the same bits every time.
+// Measured, tensors' bytes per time (a large copy: 4.7 TB/s, what the caches hold faster): forward 262144 x 256 fp32 100 us (5.4 TB/s),
+// forward and backward 32768 x 4096 bf16 287 us (4.7), backward 8192 x 8192 bf16 92 us (4.4), 4096 x 8191 bf16 46 us (4.4).
 #include <type_traits>
 
 #include "dm_block_common.h"
