@@ -396,17 +396,18 @@ inline int planned(GemmArgs& g, const GemmPlan& plan, void* part) {
   g.splits = plan.splits;
   g.part = part;
   g.ldpart = round_up(g.N, 8);
-  g.split_stride = g.M * g.ldpart;
+  g.split_stride = (g.pair ? 2 * g.M : g.M) * g.ldpart;
   return plan.tile;
 }
 
-// out[M][N] = A B (+ bias); sums: the sum of A over k (both operands KS).
+// out[M][N] = A B (+ bias); sums: the sum of A over k (both operands KS).  g.pair: of two A, with g.out2 and g.sums2.
 template <typename T, bool AKS, bool BKS>
 int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part, hipStream_t st) {
-  const int tile = planned(g, gemm_plan(g.M, g.N, g.iters, g.segments, 1, sizeof(T), !AKS), part);
+  const int tile = planned(g, gemm_plan(g.pair ? 2 * g.M : g.M, g.N, g.iters, g.segments, 1, sizeof(T), !AKS), part);
   g.out = out;
   g.bias = bias;
   g.sums = sums;
+  if (g.pair) g.out.vec = out.vec && g.out2.vec;
   g.sum_part = (float*)part + g.splits * g.split_stride;
   g.sum_segments = std::is_same<T, float>::value ? 1 << 0 | 1 << 2 | 1 << 4 : 1;  // add_terms: each plane of A once
   return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, tile, st);
@@ -487,11 +488,13 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   const Operand y = prepare_operand<T>(jobs, dy, dys, z.M, z.N, ws), wd = prepare_operand<T>(jobs, in.wd, z.F, z.N, z.F, ws),
                 x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws, gr.dwg || gr.dwu),
                 wg = prepare_operand<T>(jobs, in.wg, z.D, z.F, z.D, ws, gr.dx), wu = prepare_operand<T>(jobs, in.wu, z.D, z.F, z.D, ws, gr.dx);
-  const Operand dg = take_operand<T>(z.M, z.F, ws), du = take_operand<T>(z.M, z.F, ws);
+  // dg and du side by side, so that one product gives both projections' gradients: twice the tiles of a launch, one launch less
+  const Operand dg = take_operand<T>(z.M, 2 * (int)Fp, ws), du = {(char*)dg.p + 2 * Fp, dg.ld, dg.plane};
   const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
   size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F), terms * 2, 1, sizeof(T), true).part_bytes;
   const GemmPlan dact = gemm_plan(z.M, z.F, iters_of(z.N), terms, 1, terms > 1 ? 20 : 8, true);
-  const size_t more[] = {dact.part_bytes, gemm_plan(z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes, gemm_plan(z.N, z.F, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes};
+  const size_t more[] = {dact.part_bytes, gemm_plan(2LL * z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes,
+                         gemm_plan(z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes, gemm_plan(z.N, z.F, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes};
   for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
   void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
   if (!run) return 0;
@@ -514,14 +517,23 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
     if ((rc = product<T, false, true>(g, result<T>(gr.dx, z.D), nullptr, nullptr, part, st))) return rc;
   }
   // (the sum of dg^T, du^T, dy^T over the rows of the batch is the bias' gradient)
-  auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out, void* bias) {
+  auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out, void* bias, void* out2 = nullptr, void* bias2 = nullptr) {
     GemmArgs g = {};
     add_terms<T>(g, l, r);
     g.M = rows; g.N = cols; g.K = (int)z.M; g.iters = iters_of(z.M);
+    if (out2) {
+      g.pair = 2 * Fp;
+      g.out2 = result<T>(out2, cols);
+      g.sums2 = bias2;
+    }
     return product<T, true, true>(g, result<T>(out, cols), nullptr, bias, part, st);
   };
-  if (gr.dwg && (rc = weight(dg, x, z.F, z.D, gr.dwg, gr.dbg))) return rc;
-  if (gr.dwu && (rc = weight(du, x, z.F, z.D, gr.dwu, gr.dbu))) return rc;
+  if (gr.dwg && gr.dwu) {
+    if ((rc = weight(dg, x, z.F, z.D, gr.dwg, gr.dbg, gr.dwu, gr.dbu))) return rc;
+  } else {
+    if (gr.dwg && (rc = weight(dg, x, z.F, z.D, gr.dwg, gr.dbg))) return rc;
+    if (gr.dwu && (rc = weight(du, x, z.F, z.D, gr.dwu, gr.dbu))) return rc;
+  }
   if (gr.dwd && (rc = weight(y, kept.h, z.N, z.F, gr.dwd, gr.dbd))) return rc;
   return 0;
 }

@@ -178,7 +178,7 @@ struct GemmArgs {
   int64_t M;
   int N, K;                           // N: of one projection for EPI_GATE.  K: true length; a KC row is zero from there to the end of its piece
   int tiles_m, tiles_n, splits;
-  Out out, out2, out3;                // STORE: out.  GATE: out = h, and for the backward pass (null: not kept) out2 = u act'(g), out3 = act(g).
+  Out out, out2, out3;                // STORE: out (out2: see `pair`).  GATE: out = h, and for the backward pass (null: not kept) out2 = u act'(g), out3 = act(g).
                                       // DACT: out = dg, out2 = du
   const void *bias, *bias2;           // of the result's type; GATE: of the operands'
   const void *ug, *ag;                // DACT: u act'(g) and act(g), rows of ldg
@@ -189,6 +189,8 @@ struct GemmArgs {
   void* sums;                         // STORE with both operands KS: sum over k of A[m, k] over the segments of sum_segments, of the result's type,
   float* sum_part;                    // or null; splits > 1: their parts, M apart
   int sum_segments;
+  int64_t pair;                       // STORE with both operands KS: 0, or two products of one B in one launch: the second A lies `pair` bytes
+  void* sums2;                        // behind the first, its result in out2.p, its sums in sums2; their partial rows follow the first's
 };
 
 // Where a stage keeps a piece of 16 bytes.  KS (one LDS row per k, R columns): piece c of row k lies at c ^ ks_key(k), so that the 32
@@ -305,8 +307,9 @@ gemm_kernel(const GemmArgs p) {
   const int band = 8 * p.tiles_n;
   const int first = tile / band * 8;
   const int rows = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
-  const int tm = first + tile % band % rows, tn = tile % band / rows;
-  const int64_t m0 = (int64_t)tm * BM;
+  const int tm = __builtin_amdgcn_readfirstlane(first + tile % band % rows), tn = __builtin_amdgcn_readfirstlane(tile % band / rows);
+  const bool other = SUMS && p.pair && tm >= p.tiles_m / 2;  // of the second of a pair
+  const int64_t m0 = (int64_t)(other ? tm - p.tiles_m / 2 : tm) * BM;
   const int n0 = tn * (GATE ? BN / 2 : BN);
 
   // The block's range: k steps, and every term of the product in each.
@@ -330,7 +333,7 @@ gemm_kernel(const GemmArgs p) {
   auto group_end = [&](int from) __attribute__((always_inline)) { return from >= whole ? step1 : from + group < whole ? from + group : whole; };
   int seg = 0, step = step0, group0 = step0, group1 = group_end(step0);  // of the next stage to be asked for
   bool moved = false;
-  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2 - LDS_BIAS, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2 - LDS_BIAS;
+  const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2 + (other ? p.pair : 0) - LDS_BIAS, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2 - LDS_BIAS;
   constexpr int LOADS = sa.PASSES + sb.PASSES;
   // (kept in registers: a scalar load among the products would wait for every LDS read under way)
   int segments = p.segments, k_end = p.K, sum_segments = p.sum_segments;
@@ -462,7 +465,8 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
       for (int x = 0; x < XS; ++x) asum[x] = mfma16(ones, fragment<BM, AKS>(st, lane, wm * MI + wn * XS + x, s), asum[x], T());
   };
-  const bool sums = SUMS && p.sums && tn == 0;
+  void* const sums_out = SUMS ? other ? p.sums2 : p.sums : nullptr;
+  const bool sums = sums_out && tn == 0;
   if (turns) {
     uint32_t cur = 0;
     bool sum = false, next[GEMM_STAGES];  // do the stage at hand, and those asked for, count for the sums of A
@@ -502,6 +506,8 @@ gemm_kernel(const GemmArgs p) {
   constexpr int ROWS = WM * 32, PITCH = BN * 4 + 16, COLS = GATE ? BN / 2 : BN, PIECES = COLS / 8, TASKS = ROWS * PIECES / (NW * 64);
   const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces (with zeros: rows of B out of range are zero)
   static_assert(NW * 64 % PIECES == 0, "a thread keeps its columns");
+  Out out = p.out;
+  if (other) out.p = p.out2.p;
   float b1[8], b2[8];
   if constexpr (!DACT) {
     const int n = n0 + threadIdx.x % PIECES * 8;
@@ -538,8 +544,8 @@ gemm_kernel(const GemmArgs p) {
         const int64_t m = m0 + row / 32 * (MI * 16) + i * 32 + row % 32;
         if (m >= p.M || n >= p.N) continue;
         const float v = *(const DM_LDS float*)(buf + row * PITCH + id % BN * 4);
-        if (p.out.f32) ((float*)p.out.p)[m * p.out.ld + n] = v + bias_at<float>(p.bias, n, p.N);
-        else ((T*)p.out.p)[m * p.out.ld + n] = (T)(v + bias_at<T>(p.bias, n, p.N));
+        if (out.f32) ((float*)out.p)[m * out.ld + n] = v + bias_at<float>(p.bias, n, p.N);
+        else ((T*)out.p)[m * out.ld + n] = (T)(v + bias_at<T>(p.bias, n, p.N));
       }
       continue;
     }
@@ -554,7 +560,7 @@ gemm_kernel(const GemmArgs p) {
       from_lds(at, v);
       if constexpr (GATE) from_lds(at + 128, u);
       if (p.splits > 1) {  // joined by a second launch
-        float* part = (float*)p.part + blockIdx.y * (GATE ? 2 : 1) * p.split_stride + m * p.ldpart + n;
+        float* part = (float*)p.part + blockIdx.y * (GATE ? 2 : 1) * p.split_stride + (other ? p.M + m : m) * p.ldpart + n;
         store_f32(part, v);
         if constexpr (GATE) store_f32(part + p.split_stride, u);
         continue;
@@ -573,8 +579,8 @@ gemm_kernel(const GemmArgs p) {
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += b1[e];
-        if (p.out.f32) store8<T, OUT_F32>(p.out, m, n, p.N, v);
-        else store8<T, OUT_16>(p.out, m, n, p.N, v);
+        if (out.f32) store8<T, OUT_F32>(out, m, n, p.N, v);
+        else store8<T, OUT_16>(out, m, n, p.N, v);
       }
     }
   }
@@ -583,10 +589,10 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
       for (int x = 0; x < XS; ++x) {
         const int64_t m = m0 + (wm * MI + wn * XS + x) * 16 + lane;
-        if (!p.sums || tn || lane >= 16 || m >= p.M) continue;
-        if (p.splits > 1) p.sum_part[blockIdx.y * p.M + m] = asum[x][0];
-        else if (p.out.f32) ((float*)p.sums)[m] = asum[x][0];
-        else ((T*)p.sums)[m] = (T)asum[x][0];
+        if (!sums || lane >= 16 || m >= p.M) continue;
+        if (p.splits > 1) p.sum_part[(blockIdx.y * (p.pair ? 2 : 1) + other) * p.M + m] = asum[x][0];
+        else if (out.f32) ((float*)sums_out)[m] = asum[x][0];
+        else ((T*)sums_out)[m] = (T)asum[x][0];
       }
     }
   }
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
   using Kept = typename std::conditional<F32, float, T>::type;
   constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
   const int np = (p.N + 7) & ~7, pieces = np / 8;
-  const int64_t all = p.M * pieces;
+  const int64_t rows = EPI == EPI_STORE && p.pair ? 2 * p.M : p.M, all = rows * pieces;
   const bool grouped = p.splits > 4;
   const int count = grouped ? 64 : 256;
   for (int64_t base = (int64_t)blockIdx.x * count; base < all; base += (int64_t)gridDim.x * count) {
@@ -648,8 +654,10 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
     } else if constexpr (EPI == EPI_STORE) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
-      if (p.out.f32) store8<T, OUT_F32>(p.out, m, n, p.N, v);
-      else store8<T, OUT_16>(p.out, m, n, p.N, v);
+      Out o = p.out;
+      if (m >= p.M) o.p = p.out2.p;
+      if (o.f32) store8<T, OUT_F32>(o, m >= p.M ? m - p.M : m, n, p.N, v);
+      else store8<T, OUT_16>(o, m >= p.M ? m - p.M : m, n, p.N, v);
     } else {
       float ag[8];
       load8((const Kept*)p.ug + m * p.ldg + n, u);
@@ -660,13 +668,15 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
       store8<T, BETWEEN>(p.out2, m, n, np, h);
     }
   }
-  if (EPI == EPI_STORE && p.sums)
-    for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < p.M; m += (int64_t)gridDim.x * 256) {
+  if (EPI == EPI_STORE && (p.sums || p.sums2))
+    for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < rows; m += (int64_t)gridDim.x * 256) {
+      void* const out = m >= p.M ? p.sums2 : p.sums;
+      if (!out) continue;
       float s = 0.f;
 #pragma unroll 16
-      for (int i = 0; i < p.splits; ++i) s += p.sum_part[i * p.M + m];
-      if (p.out.f32) ((float*)p.sums)[m] = s;
-      else ((T*)p.sums)[m] = (T)s;
+      for (int i = 0; i < p.splits; ++i) s += p.sum_part[i * rows + m];
+      if (p.out.f32) ((float*)out)[m >= p.M ? m - p.M : m] = s;
+      else ((T*)out)[m >= p.M ? m - p.M : m] = (T)s;
     }
 }
 
@@ -723,7 +733,7 @@ template <typename T, bool AKS, bool BKS, int EPI>
 int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, SLIM = !AKS;
   const int bm = TILE_M[tile], bn = TILE_N[tile];
-  a.tiles_m = (int)((a.M + bm - 1) / bm);
+  a.tiles_m = (int)((a.M + bm - 1) / bm) * (a.pair ? 2 : 1);
   a.tiles_n = GATE ? (a.N + bn / 2 - 1) / (bn / 2) : (a.N + bn - 1) / bn;
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > (1 << 22)) return fail("gated feed-forward block: %lld output tiles in one product", (long long)tiles);
@@ -747,7 +757,7 @@ int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
     e = hipLaunchKernel(f, grid, dim3(tile == TILE_WIDE ? 512 : 256), args, bytes, st);
   }
   if (e == hipSuccess && a.splits > 1) {
-    const int64_t count = a.splits > 4 ? 64 : 256, blocks = (a.M * ((a.N + 7) / 8) + count - 1) / count;
+    const int64_t count = a.splits > 4 ? 64 : 256, blocks = (a.M * (a.pair ? 2 : 1) * ((a.N + 7) / 8) + count - 1) / count;
     join_kernel<T, EPI><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
     e = hipGetLastError();
   }

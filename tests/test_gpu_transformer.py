@@ -606,3 +606,32 @@ def test_gated_ffn_few_fp32_rows_of_odd_widths(size):
     e = 2.0 ** -24 * (32 + max(size) / 8)
     for name, t in zip(("y", "dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down"), got):
         close(t, res[name], 2.0 ** -24 * res[name].abs() + e * exact[name], f"{name} {size}")
+
+
+@pytest.mark.parametrize("size", [(90, 40, 56, 24), (90, 33, 57, 21), (1500, 64, 300, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_ffn_backward_of_some_gradients(size):
+    """The library's entry point asked for one projection's gradient, or one bias of two: what both together give, to fp32 rounding; what
+    was not asked for is not written."""
+    m, dd, f, n = size
+    g = torch.Generator().manual_seed(m + dd)
+    x, dy, w, b = ffn_case(g, m, dd, f, n, torch.float32, True)
+    xd, dyd, wd, bd = x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+    _, saved = d.gated_ffn(xd, *wd, *bd, save=True)
+    full = dict(zip(("dx", "dwg", "dwu", "dwd", "dbg", "dbu", "dbd"), d.gated_ffn_backward(dyd, xd, *wd, saved, bias=True)))
+    exact = ffn_oracle(x, dy, w, b, "silu")[1]
+    bound = {"dx": "dx", "dwg": "dw_gate", "dwu": "dw_up", "dwd": "dw_down", "dbg": "db_gate", "dbu": "db_up", "dbd": "db_down"}
+    L = _lib.lib()
+    nbytes = L.dm_gated_ffn_backward_workspace_bytes(m, dd, f, n, 0)
+    e = 2 * 2.0 ** -24 * (32 + max(size) / 8)  # both sides within the bound of test_gated_ffn_forward_and_backward
+    for asked in (("dwg",), ("dwu", "dbu"), ("dwg", "dwu", "dbu"), ("dwg", "dwu", "dbg"), ("dx", "dwd"), ("dwd", "dbd"), ("dwg", "dbg", "dwd")):
+        out = {k: torch.full_like(t, 3.0) for k, t in full.items()}
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+        p = {k: t.data_ptr() if k in asked else None for k, t in out.items()}
+        _lib.check(L.dm_gated_ffn_backward(dyd.data_ptr(), n, xd.data_ptr(), dd, wd[0].data_ptr(), wd[1].data_ptr(), wd[2].data_ptr(), saved.data_ptr(),
+                                           p["dx"], p["dwg"], p["dwu"], p["dwd"], p["dbg"], p["dbu"], p["dbd"], m, dd, f, n, 0, 0, ws.data_ptr(), nbytes,
+                                           torch.cuda.current_stream().cuda_stream))
+        for k, t in out.items():
+            if k in asked:
+                close(t, full[k].cpu().double(), 2.0 ** -23 * full[k].cpu().double().abs() + e * exact[bound[k]], f"{k} of {asked}")
+            else:
+                assert (t == 3).all(), (k, asked)
