@@ -15,7 +15,7 @@
 // Bound by the matrix pipe and what is issued beside it: a SIMD's time is nearly the sum of its waves' products and other instructions, so
 // everything else in a step is kept short and lies between the products.  Measured, bf16, 8192 rows of width 4096, hidden 11008: both
 // projections with their gate 1.18 ms (1.25 PFLOP/s), down 0.55 ms (1.35), dh with dg and du 0.76 ms, dx 1.12 ms (1.32), a weight's gradient
-// 0.63 ms (1.18; 688 tiles in three rounds of 256); the library's products of these shapes reach 1.03 to 1.60.
+// 0.63 ms (1.18; 688 tiles in three rounds of 256 CUs); the library's products of these shapes reach 1.03 to 1.60.
 #ifndef DM_BLOCK_GEMM_HIP
 #define DM_BLOCK_GEMM_HIP
 #include <atomic>

@@ -215,7 +215,8 @@ def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inver
     position * inv_freq; returns (q, k).  ``inv_freq`` (float64 [rotary_dim / 2], on the GPU) says how much of the head turns;
     the rest is copied.  ``positions``: integers [T], [B, T], or [axes, B, T] (pair i takes axis i // (pairs / axes)), None for
     0..T-1; angles are formed in 64 bits.  ``layout``: "half" pairs element i with i + rotary_dim/2, "interleaved" 2i with 2i + 1.
-    ``inverse`` turns back: applied to gradients it is the backward pass.  ``inplace`` writes into q and k themselves."""
+    ``inverse`` turns back: applied to gradients it is the backward pass.  ``inplace`` writes into q and k
+    themselves, which must share no elements then."""
     dt = _dtype(q, "q")
     if q.dim() != 4 or q.shape[3] < 1:
         raise RuntimeError(f"q must be [B, T, heads, head_dim] (got {tuple(q.shape)})")
@@ -248,7 +249,7 @@ def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inver
         strides = _Strides(have[0] if axes > 1 else 0, have[-2] if dims > 1 and shape[-2] > 1 else 0, have[-1] if shape[-1] > 1 else 0)
     if pairs % axes:
         raise RuntimeError(f"{pairs} pairs do not divide into {axes} axes")
-    if inplace and k is not None and k.data_ptr() == q.data_ptr() and q.numel():
+    if inplace and k is not None and k.data_ptr() == q.data_ptr() and q.numel() and k.numel():
         raise RuntimeError("in place needs q and k that share no elements")
     q, q_out, q_arg = _turned(q, inplace)
     k_out = k_arg = None
@@ -282,7 +283,8 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     """(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down, with weights as nn.Linear holds them: w_gate and w_up
     [hidden, width], w_down [out, hidden].  All tensors are of one type.  ``activation``: silu, gelu (erf), gelu_tanh, relu, sigmoid.
     ``save``: (y, saved), with ``saved`` (opaque) for ``gated_ffn_backward``.  16-bit types round the hidden values to that type
-    between the matrix products; fp32 keeps fp32 accuracy."""
+    between the matrix products; fp32 keeps fp32 accuracy (an infinite
+    operand may give NaN where fp32 would give an infinity)."""
     dt, d, f, n, w_gate, w_up, w_down = _ffn_check(x, w_gate, w_up, w_down, activation)
     b_gate, b_up, b_down = _vector(b_gate, f, x, "b_gate"), _vector(b_up, f, x, "b_up"), _vector(b_down, n, x, "b_down")
     L = _lib.lib()
