@@ -172,7 +172,7 @@ extern "C" int dm_rotary(const dm_rotary_tensor* q, const dm_rotary_tensor* k, c
     if (B * T > 0 && (!t->in || !t->out)) return fail("dm_rotary: null argument");
     a.in[w] = t->in; a.out[w] = t->out; a.heads[w] = t->heads;
     for (int i = 0; i < 3; ++i) { a.is[w][i] = t->in_stride[i]; a.os[w][i] = t->out_stride[i]; }
-    if (t->in == t->out) {
+    if (t->in == t->out && B * T > 0) {
       for (int i = 0; i < 3; ++i)
         if (t->in_stride[i] != t->out_stride[i]) return fail("dm_rotary: in place needs the input's strides");
     } else {

@@ -635,3 +635,27 @@ def test_gated_ffn_backward_of_some_gradients(size):
                 close(t, full[k].cpu().double(), 2.0 ** -23 * full[k].cpu().double().abs() + e * exact[bound[k]], f"{k} of {asked}")
             else:
                 assert (t == 3).all(), (k, asked)
+
+
+def test_operators_on_nothing():
+    """Batches, tokens and heads of no elements, one vector without a leading dimension, gradients and weights as views."""
+    inv = d.rotary_frequencies(8)[0].to(DEV)
+    for shape in ((2, 0, 3, 8), (0, 5, 3, 8), (2, 3, 0, 8)):
+        x = torch.empty(shape, device=DEV)
+        for inplace in (False, True):
+            q, k = d.apply_rotary(x, x.clone(), inv, torch.zeros(shape[:2], dtype=torch.int32, device=DEV), inplace=inplace)
+            assert q.shape == k.shape == shape
+    g = torch.Generator().manual_seed(9)
+    w, wd = rand(g, 4, 8).to(DEV), rand(g, 8, 4).to(DEV)
+    for shape in ((3, 0, 8), (8,)):
+        x = rand(g, *shape).to(DEV)
+        n, mu, rs = d.layer_norm(x, return_stats=True)
+        y, saved = d.gated_ffn(x, w, w, wd, save=True)
+        assert n.shape == y.shape == shape and mu.shape == shape[:-1]
+        assert d.layer_norm_backward(y, x, None, mu, rs)[0].shape == shape and d.gated_ffn_backward(y, x, w, w, wd, saved)[0].shape == shape
+    x = rand(g, 70, 16, dtype=torch.bfloat16).to(DEV)
+    ws = [rand(g, 16, 24).to(DEV, torch.bfloat16).t(), rand(g, 24, 32).to(DEV, torch.bfloat16)[:, ::2], rand(g, 16, 24).to(DEV, torch.bfloat16)]
+    dy = torch.ones(1, 1, device=DEV, dtype=torch.bfloat16).expand(70, 16)
+    saved = d.gated_ffn(x, *ws, save=True)[1]
+    a, b = d.gated_ffn_backward(dy, x, *ws, saved), d.gated_ffn_backward(dy.contiguous(), x, *[t.contiguous() for t in ws], saved)
+    assert all(torch.equal(p, q) for p, q in zip(a[:4], b[:4]))
