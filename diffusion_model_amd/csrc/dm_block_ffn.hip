@@ -321,6 +321,63 @@ int streamed(const Streamed<T>& a, hipStream_t st) {
   return gemv_launch<T, GATE>(a, st);
 }
 
+// ---- fp32 backward, up to SKINNY_ROWS rows: part[split][m][n] = sum over the split's k of A[m][k] B[k][n], B's rows in memory.  A thread takes
+// four columns of sixteen rows and walks k; A's part lies in LDS.  Bound by B's bytes, where tiles of split operands would first write three
+// planes of it; the parts are joined like those of a tile's split range.
+constexpr int COLUMN_ROWS = 16, COLUMN_K = 128;  // k per split, at most
+struct Columns { const float* a; const bf16* planes; int64_t lda, plane; const float* b; int64_t ldb; float* part; int64_t split_stride, ldpart; int M, N, K, per; };
+__global__ void __launch_bounds__(256) column_kernel(const Columns p) {
+  __shared__ float a[COLUMN_K][COLUMN_ROWS];
+  const int m0 = blockIdx.z * COLUMN_ROWS, k0 = blockIdx.y * p.per, count = p.K - k0 < p.per ? p.K - k0 : p.per;
+  for (int e = threadIdx.x; e < count * COLUMN_ROWS; e += 256) {
+    const int m = m0 + e / count, k = e % count;
+    float v = 0.f;
+    if (m < p.M) {
+      const int64_t at = m * p.lda + k0 + k;
+      v = p.a ? p.a[at] : ((float)p.planes[2 * p.plane + at] + (float)p.planes[p.plane + at]) + (float)p.planes[at];
+    }
+    a[k][e / count] = v;
+  }
+  __syncthreads();
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n >= p.N) return;
+  const int at = n + 4 <= p.N ? n : p.N - 4;  // (the last piece is moved back; both write the same values)
+  float acc[COLUMN_ROWS][4] = {};
+  const float* b = p.b + (int64_t)k0 * p.ldb + at;
+#pragma unroll 8
+  for (int k = 0; k < count; ++k) {
+    const Piece<float, 4> v = *reinterpret_cast<const Piece<float, 4>*>(b + k * p.ldb);
+#pragma unroll
+    for (int m = 0; m < COLUMN_ROWS; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[m][j] = fmaf(a[k][m], v.v[j], acc[m][j]);
+  }
+  float* part = p.part + blockIdx.y * p.split_stride + at;
+#pragma unroll
+  for (int m = 0; m < COLUMN_ROWS; ++m)
+    if (m0 + m < p.M) {
+      Piece<float, 4> r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.v[j] = acc[m][j];
+      float* row = part + (m0 + m) * p.ldpart;
+      *reinterpret_cast<Piece<float, 4>*>(row) = r;
+      if (n + 4 >= p.N)  // the padding of a row holds zeros
+        for (int c = p.N - at; at + c < p.ldpart; ++c) row[c] = 0.f;
+    }
+}
+// k per split: a thousand workgroups where the range gives them, 16 k or more each
+inline int column_per(int64_t M, int N, int K) {
+  const int blocks = (int)((N + 1023) / 1024 * ((M + COLUMN_ROWS - 1) / COLUMN_ROWS));
+  int per = (int)((int64_t)K * blocks / 1024);
+  return per < 16 ? 16 : per > COLUMN_K ? COLUMN_K : per;
+}
+inline int column_splits(int64_t M, int N, int K) { return (K + column_per(M, N, K) - 1) / column_per(M, N, K); }
+inline int column_launch(Columns a, hipStream_t st) {
+  a.per = column_per(a.M, a.N, a.K);
+  column_kernel<<<dim3((a.N + 1023) / 1024, column_splits(a.M, a.N, a.K), (a.M + COLUMN_ROWS - 1) / COLUMN_ROWS), dim3(256), 0, st>>>(a);
+  return launched("dm_gated_ffn_backward");
+}
+
 // ---- workspace
 struct Carver {
   char* base;
@@ -484,10 +541,15 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
                  hipStream_t st) {
   const int64_t Fp = pad8(z.F);
   const int terms = std::is_same<T, float>::value ? 6 : 1;
+  const bool few = std::is_same<T, float>::value && z.M <= SKINNY_ROWS && z.D >= 4 && z.F >= 4;  // column_kernel
   PackJobs jobs = {};
-  const Operand y = prepare_operand<T>(jobs, dy, dys, z.M, z.N, ws), wd = prepare_operand<T>(jobs, in.wd, z.F, z.N, z.F, ws),
-                x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws, gr.dwg || gr.dwu),
-                wg = prepare_operand<T>(jobs, in.wg, z.D, z.F, z.D, ws, gr.dx), wu = prepare_operand<T>(jobs, in.wu, z.D, z.F, z.D, ws, gr.dx);
+  const Operand y = prepare_operand<T>(jobs, dy, dys, z.M, z.N, ws), x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws, gr.dwg || gr.dwu);
+  Operand wd = {}, wg = {}, wu = {};
+  if (!few) {
+    wd = prepare_operand<T>(jobs, in.wd, z.F, z.N, z.F, ws);
+    wg = prepare_operand<T>(jobs, in.wg, z.D, z.F, z.D, ws, gr.dx);
+    wu = prepare_operand<T>(jobs, in.wu, z.D, z.F, z.D, ws, gr.dx);
+  }
   // dg and du side by side, so that one product gives both projections' gradients: twice the tiles of a launch, one launch less
   const Operand dg = take_operand<T>(z.M, 2 * (int)Fp, ws), du = {(char*)dg.p + 2 * Fp, dg.ld, dg.plane};
   const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
@@ -496,6 +558,10 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   const size_t more[] = {dact.part_bytes, gemm_plan(2LL * z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes,
                          gemm_plan(z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes, gemm_plan(z.N, z.F, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes};
   for (size_t b : more) part_bytes = b > part_bytes ? b : part_bytes;
+  if (few) {
+    const size_t columns[] = {(size_t)column_splits(z.M, z.F, z.N) * z.M * Fp * 4, (size_t)2 * column_splits(z.M, z.D, z.F) * z.M * pad8(z.D) * 4};
+    for (size_t b : columns) part_bytes = b > part_bytes ? b : part_bytes;
+  }
   void* part = ws.take(part_bytes);  // used by one product after the other, in stream order
   if (!run) return 0;
   int rc = pack_launch<T>(jobs, st);
@@ -507,14 +573,32 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   a.out = between<T>(dg); a.out2 = between<T>(du);
   a.ug = kept.ug; a.ag = kept.ag; a.ldg = Fp;
   const int tile = planned(a, dact, part);
-  if ((rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, tile, st))) return rc;
+  if constexpr (std::is_same<T, float>::value)
+    if (few) {
+      a.splits = column_splits(z.M, z.F, z.N);
+      if ((rc = column_launch({(const float*)dy, nullptr, dys, 0, (const float*)in.wd, z.F, (float*)part, a.split_stride, a.ldpart, (int)z.M, z.F, z.N, 0}, st)))
+        return rc;
+      if ((rc = join_launch<bf16, EPI_DACT_F32>(a, st))) return rc;
+    }
+  if (!few && (rc = gemm_launch<Mat<T>, false, true, std::is_same<T, float>::value ? EPI_DACT_F32 : EPI_DACT>(a, tile, st))) return rc;
 
   if (gr.dx) {
     GemmArgs g = {};
     add_terms<T>(g, dg, wg);
     add_terms<T>(g, du, wu, true);
     g.M = z.M; g.N = z.D; g.K = z.F; g.iters = iters_of(z.F);
-    if ((rc = product<T, false, true>(g, result<T>(gr.dx, z.D), nullptr, nullptr, part, st))) return rc;
+    if constexpr (std::is_same<T, float>::value)
+      if (few) {
+        const int half = column_splits(z.M, z.D, z.F);
+        planned(g, {TILE_MID, 2 * half, 0}, part);
+        g.out = result<T>(gr.dx, z.D);
+        for (int i = 0; i < 2 && !rc; ++i)
+          rc = column_launch({nullptr, (const bf16*)(i ? du.p : dg.p), dg.ld, dg.plane, (const float*)(i ? in.wu : in.wg), z.D,
+                              (float*)part + i * half * g.split_stride, g.split_stride, g.ldpart, (int)z.M, z.D, z.F, 0}, st);
+        if (!rc) rc = join_launch<bf16, EPI_STORE>(g, st);
+        if (rc) return rc;
+      }
+    if (!few && (rc = product<T, false, true>(g, result<T>(gr.dx, z.D), nullptr, nullptr, part, st))) return rc;
   }
   // (the sum of dg^T, du^T, dy^T over the rows of the batch is the bias' gradient)
   auto weight = [&](const Operand& l, const Operand& r, int rows, int cols, void* out, void* bias, void* out2 = nullptr, void* bias2 = nullptr) {

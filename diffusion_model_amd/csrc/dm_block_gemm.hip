@@ -729,6 +729,13 @@ inline hipError_t allow_lds(const void* f, int bytes, std::atomic<uint64_t>& don
   return e;
 }
 
+template <typename T, int EPI>
+int join_launch(const GemmArgs& a, hipStream_t st) {
+  const int64_t count = a.splits > 4 ? 64 : 256, blocks = (a.M * (a.pair ? 2 : 1) * ((a.N + 7) / 8) + count - 1) / count;
+  join_kernel<T, EPI><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
+  return launched("gated feed-forward block");
+}
+
 template <typename T, bool AKS, bool BKS, int EPI>
 int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, SLIM = !AKS;
@@ -756,11 +763,7 @@ int gemm_launch(GemmArgs a, int tile, hipStream_t st) {
     void* args[] = {&a};
     e = hipLaunchKernel(f, grid, dim3(tile == TILE_WIDE ? 512 : 256), args, bytes, st);
   }
-  if (e == hipSuccess && a.splits > 1) {
-    const int64_t count = a.splits > 4 ? 64 : 256, blocks = (a.M * (a.pair ? 2 : 1) * ((a.N + 7) / 8) + count - 1) / count;
-    join_kernel<T, EPI><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st>>>(a);
-    e = hipGetLastError();
-  }
+  if (e == hipSuccess && a.splits > 1) return join_launch<T, EPI>(a, st);
   return e == hipSuccess ? 0 : fail("gated feed-forward block: launch failed: %s", hipGetErrorString(e));
 }
 
