@@ -64,6 +64,7 @@ _SIGS = {
     "dm_layer_norm_backward_workspace_bytes": (_sz, [_l, _i]),
     "dm_layer_norm_backward": (_i, [_vp, _l, _vp, _l, _vp, _i, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _vp, _sz, _vp]),
     "dm_rotary": (_i, [C.POINTER(RotaryTensor), C.POINTER(RotaryTensor), _vp, C.POINTER(_l), _i, _vp, _l, _l, _i, _i, _i, _f, _i, _i, _vp]),
+    "dm_debug_ffn_plan": (_i, [_i, _i]),
     "dm_gated_ffn_saved_bytes": (_sz, [_l, _i, _i]),
     "dm_gated_ffn_workspace_bytes": (_sz, [_l, _i, _i, _i, _i, _i]),
     "dm_gated_ffn": (_i, [_vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
@@ -72,7 +73,7 @@ _SIGS = {
                                    _sz, _vp]),
 }
 EXPORTS = tuple(_SIGS)
-ABI_VERSION = 5  # include/dm_sampler.h: DM_ABI_VERSION
+ABI_VERSION = 6  # include/dm_sampler.h: DM_ABI_VERSION
 CHUNK_FN = C.CFUNCTYPE(_vp, _vp, _i, _i)  # dm_chunk_fn
 
 

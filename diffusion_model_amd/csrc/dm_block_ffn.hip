@@ -661,6 +661,14 @@ __global__ void fill_zero_bytes_kernel(uint32_t* p, int64_t words, uint16_t* tai
 
 extern "C" {
 
+int dm_debug_ffn_plan(int tile, int splits) {
+  using namespace dmb;
+  if (tile < -1 || tile >= TILES || splits < 1 || splits > 64) return fail("dm_debug_ffn_plan: tile %d (-1 to 2), %d parts (1 to 64)", tile, splits);
+  forced_tile = tile;
+  forced_splits = splits;
+  return 0;
+}
+
 size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype) {
   using namespace dmb;
   if (M <= 0 || F < 1 || !dtype_ok(dtype)) return 0;

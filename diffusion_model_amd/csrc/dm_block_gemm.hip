@@ -686,6 +686,12 @@ enum { TILE_WIDE, TILE_MID, TILE_SLIM, TILES };
 constexpr int TILE_M[TILES] = {256, 128, 64}, TILE_N[TILES] = {256, 128, 128}, TILE_PER_CU[TILES] = {1, 2, 2};
 
 struct GemmPlan { int tile, splits; size_t part_bytes; };
+inline size_t gemm_part_bytes(int64_t M, int N, int outs, int splits) {
+  return splits > 1 ? (size_t)splits * outs * M * (round_up(N, 8) + 1) * 4 : 0;  // products, and sums of A
+}
+
+// Tests run every product with every tile: dm_debug_ffn_plan, of the calling thread.
+inline thread_local int forced_tile = -1, forced_splits = 1;
 
 // Tile and split of the k range: the least of an estimate in microseconds.  A product's time is that of its stages - alone on a CU, or two
 // workgroups to a CU where they fit (WIDE: two rounds) - but not less than the n side's bytes take, then for each round of workgroups
@@ -694,6 +700,13 @@ struct GemmPlan { int tile, splits; size_t part_bytes; };
 // bf16 and fp32, all products of both passes): what it picks takes 2 % longer than the best on average and 30 % at worst, where always
 // taking MID unsplit would take 66 % longer.  `outs`: products per n (2: both projections).
 inline GemmPlan gemm_plan(int64_t M, int N, int steps, int terms, int outs, int bytes, bool slim) {
+  if (forced_tile >= 0) {
+    GemmPlan forced = {forced_tile == TILE_SLIM && !slim ? (int)TILE_MID : forced_tile, 1, 0};
+    const int per = split_steps(steps, forced_splits);
+    forced.splits = (steps + per - 1) / per;
+    forced.part_bytes = gemm_part_bytes(M, N, outs, forced.splits);
+    return forced;
+  }
   const int cus = 256;
   constexpr double ALONE[TILES] = {1.6, 0.97, 0.54}, PAIR[TILES] = {4.0, 1.08, 0.8}, START[TILES] = {2.1, 1.7, 2.1};
   GemmPlan best = {TILE_MID, 1, 0};
@@ -714,7 +727,7 @@ inline GemmPlan gemm_plan(int64_t M, int N, int steps, int terms, int outs, int 
       if (c < cost) { cost = c; best.tile = t; best.splits = s; }
     }
   }
-  if (best.splits > 1) best.part_bytes = (size_t)best.splits * outs * M * (round_up(N, 8) + 1) * 4;  // products, and sums of A
+  best.part_bytes = gemm_part_bytes(M, N, outs, best.splits);
   return best;
 }
 

@@ -42,8 +42,9 @@ const char* dm_last_error(void);
  * 3: dm_sample_chunked, the fused low-resolution kernel class, the any-geometry kernel classes;
  * 4: dm_sample's workspace holds one carve per parallel sub-batch chain (dm_sample_workspace_bytes grew for large batches),
  *    dm_sample_branches, dm_stream_create / dm_stream_destroy;
- * 5: the transformer-block operators dm_layer_norm*, dm_rotary, dm_gated_ffn*; nothing of version 4 changed). */
-#define DM_ABI_VERSION 5
+ * 5: the transformer-block operators dm_layer_norm*, dm_rotary, dm_gated_ffn*; nothing of version 4 changed;
+ * 6: dm_debug_ffn_plan; nothing of version 5 changed). */
+#define DM_ABI_VERSION 6
 int dm_version(void);
 /* sha256 over the compiler flags and sources this library was built from (__graft_entry__.build_key); "unkeyed" for a
  * hand build.  build() compares it with the tree it runs in, so a library built with other flags is not reused. */
@@ -359,6 +360,10 @@ int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_d
                           void* dw_up_dev, void* dw_down_dev, void* db_gate_dev, void* db_up_dev, void* db_down_dev, int64_t M,
                           int D, int F, int N, int activation, int dtype, void* workspace_dev, size_t workspace_bytes,
                           void* stream);
+/* Test hook, for the calling thread: the tiled products of the gated block run with this tile (0: 256 x 256, 1: 128 x 128,
+ * 2: 64 x 128 where a product has it, 128 x 128 elsewhere) and k ranges of `splits` parts (1 to 64; fewer where the range is shorter)
+ * instead of what the sizes would choose; tile -1: as the sizes choose.  Workspace sizes follow. */
+int dm_debug_ffn_plan(int tile, int splits);
 
 #ifdef __cplusplus
 }

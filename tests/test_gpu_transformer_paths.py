@@ -1,0 +1,167 @@
+"""Transformer-block operators (GPU): every tile and split of the gated block's products, layer norms of many rows, rotary calls whose
+threads walk several heads; against the formulas in 64 bits (oracles and bounds of test_gpu_transformer.py)."""
+import pytest
+import torch
+
+import diffusion_model_amd as d
+from diffusion_model_amd import _lib
+from test_gpu_transformer import DEV, DTYPES, HALF, _norm_bounds, close, ffn_case, ffn_oracle, norm_oracle, rand, rotary_oracle
+
+pytestmark = pytest.mark.gpu
+NAMES = ("y", "dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down")
+TILES = {"256x256": 0, "128x128": 1, "64x128": 2}
+
+
+class plan:
+    """The tiled products of the block with one tile and k ranges of `splits` parts."""
+
+    def __init__(self, tile, splits):
+        self.args = TILES[tile], splits
+
+    def __enter__(self):
+        _lib.check(_lib.lib().dm_debug_ffn_plan(*self.args))
+
+    def __exit__(self, *_):
+        _lib.check(_lib.lib().dm_debug_ffn_plan(-1, 1))
+
+
+def step(x, dy, w, b, act):
+    y, saved = d.gated_ffn(x, *w, *b, activation=act, save=True)
+    return (y, *d.gated_ffn_backward(dy, x, *w, saved, activation=act, bias=True))
+
+
+def ffn_bounds(x, dy, w, b, act, dt):
+    """(name, value, bound).  fp32 sums of K terms: at most K/8 + 32 half steps of the absolute sums.  16-bit types round h, u act'(g),
+    act(g), dg and du, each by half a step, before they are multiplied: two roundings of dg and du, one of h."""
+    res, exact, _ = ffn_oracle(x, dy, w, b, act)
+    m, dd = x.shape
+    f, n = w[0].shape[0], w[2].shape[0]
+    e = 2.0 ** -24 * (32 + max(dd, f, n, m) / 8)
+    X, DY, (wg, wu, wd) = x.double(), dy.double(), [t.double() for t in w]
+    bg, bu, _ = [0.0 if t is None else t.double() for t in b]
+    g, u = X @ wg.T + bg, X @ wu.T + bu
+    a, da = {"relu": lambda v: (v.clamp_min(0), (v > 0).double()), "silu": lambda v: (v * torch.sigmoid(v), torch.sigmoid(v) * (1 + v * torch.sigmoid(-v)))}[act](g)
+    dh = DY @ wd
+    h, dg, du = a * u, dh * u * da, dh * a
+    half = HALF[dt] if dt != torch.float32 else 0.0
+    hr, dgr, dur = half * h.abs(), 2 * half * dg.abs(), 2 * half * du.abs()
+    if act == "relu":  # at the kink an error of g decides between the two slopes
+        near = g.abs() <= e * (X.abs() @ wg.abs().T + abs(bg))
+        dgr = dgr + near * (dh * u).abs()
+    rounded = {"y": hr @ wd.abs().T, "dx": dgr @ wg.abs() + dur @ wu.abs(), "dw_gate": dgr.T @ X.abs(), "dw_up": dur.T @ X.abs(),
+               "dw_down": DY.abs().T @ hr, "db_gate": dgr.sum(0), "db_up": dur.sum(0), "db_down": torch.zeros(n, dtype=torch.float64)}
+    tiny = 1e-6 if dt == torch.float16 else 0.0  # of fp16 values below its normal range, half a step of 2^-24 each
+    return [(k, res[k], HALF[dt] * res[k].abs() + e * exact[k] + 1.01 * rounded[k] + tiny) for k in NAMES]
+
+
+# rows, width, hidden, out: several tiles of every size with a rest, in whole 16-byte pieces and off them; long sums over the rows, the
+# width and the hidden values
+SIZES = [(700, 264, 312, 280), (613, 259, 301, 277), (2100, 136, 152, 136), (300, 1304, 328, 520)]
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("tile", list(TILES))
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_every_tile_and_split(size, dtype, tile, splits):
+    m, dd, f, n = size
+    dt = DTYPES[dtype]
+    act = "relu" if (m + splits) % 2 else "silu"
+    g = torch.Generator().manual_seed(m + f)
+    x, dy, w, b = ffn_case(g, m, dd, f, n, dt, True)
+    args = x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+    with plan(tile, splits):
+        got = step(*args, act)
+        again = step(*args, act)
+    for (name, want, tol), t, t2 in zip(ffn_bounds(x, dy, w, b, act, dt), got, again):
+        close(t, want, tol, f"{name} {size} {dtype} {act} {tile} in {splits}")
+        assert torch.equal(t, t2), name
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [2, 40, 150])
+def test_relu_of_16_bit_rows(rows, dtype):
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(rows)
+    x, dy, w, b = ffn_case(g, rows, 72, 120, 56, dt, True)
+    got = step(x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b], "relu")
+    for (name, want, tol), t in zip(ffn_bounds(x, dy, w, b, "relu", dt), got):
+        close(t, want, tol, f"{name} {rows} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_strided_rows_of_every_path(dtype):
+    """Rows inside wider arrays give the bits of contiguous ones: few rows and many, x and the output's gradient."""
+    dt = DTYPES[dtype]
+    for rows in (2, 20, 64, 300):
+        g = torch.Generator().manual_seed(rows)
+        x, dy, w, b = ffn_case(g, rows, 48, 72, 40, dt, True)
+        w, b = [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+        want = step(x.to(DEV), dy.to(DEV), w, b, "silu")
+        for off in (0, 3, 8):
+            wide = torch.full((rows, 64), float("nan"), dtype=dt, device=DEV)
+            pad = torch.full((rows, 56), float("nan"), dtype=dt, device=DEV)
+            wide[:, off:off + 48], pad[:, off:off + 40] = x.to(DEV), dy.to(DEV)
+            for name, p, q in zip(NAMES, want, step(wide[:, off:off + 48], pad[:, off:off + 40], w, b, "silu")):
+                assert torch.equal(p, q), (rows, off, name)
+
+
+# ------------------------------------------------------------------ layer norm, many rows
+
+# shapes of the kernels in every type: 16, 64, 256, 512 and 1024 threads a row, one to eight pieces each, whole pieces and not
+MANY = [(5003, 100), (4101, 250), (3001, 300), (3007, 520), (5000, 1000), (1100, 1030), (2101, 1504), (1029, 2050), (1301, 4095), (1025, 4096),
+        (1100, 6001), (1061, 12289)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,width", MANY, ids=lambda v: str(v))
+def test_layer_norm_of_many_rows(rows, width, dtype):
+    """Every block walks several rows in the backward pass, and the forward pass takes its kernels for many rows.  Bounds as in
+    test_layer_norm_forward_and_backward; a column's sum has at most rows / 256 + 4 + 16 + 16 additions on end."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(rows + width)
+    x, dy = rand(g, rows, width, dtype=dt, scale=1.5, shift=0.5), rand(g, rows, width, dtype=dt)
+    w, b = rand(g, width, dtype=dt, scale=0.2, shift=1.0), rand(g, width, dtype=dt)
+    xd, dyd, wd = x.to(DEV), dy.to(DEV), w.to(DEV)
+    y, mu, rs = d.layer_norm(xd, wd, b.to(DEV), return_stats=True)
+    got = (y, *d.layer_norm_backward(dyd, xd, wd, mu, rs))
+    for (name, want, tol), t in zip(_norm_bounds(x, w, b, dy, dt), got):
+        close(t, want, tol, f"{name} {rows}x{width}")
+    _, _, mean, rstd = norm_oracle(x, w, b, 1e-5)
+    xa = x.double().abs().mean(-1)
+    e = 64 * 2.0 ** -24
+    em = e * xa * rstd
+    close(mu, mean, e * xa, "mean")
+    close(rs, rstd, rstd * (e + em + em * em), "rstd")
+
+
+# ------------------------------------------------------------------ rotary: several heads per thread
+
+# (tokens, heads, kv_heads, head_dim, rotary_dim): a thread walks 2, 4 or 8 heads; head counts that no group divides, groups that hold
+# the last query heads and the first key heads; one element at a time (33 and 9 pairs) and whole vectors
+WALKS = [(1400, 9, 2, 66, 66), (2700, 9, 2, 66, 66), (4100, 9, 2, 66, 66), (8000, 5, 1, 66, 66), (4000, 5, 1, 66, 66), (8200, 9, 2, 64, 64),
+         (16500, 9, 2, 64, 48), (3300, 13, 6, 40, 18)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("walk", WALKS, ids=lambda s: "x".join(map(str, s)))
+def test_rotary_of_several_heads_per_thread(walk, layout, dtype):
+    t, h, hk, dd, rd = walk
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(t + h)
+    qkv = rand(g, 1, t, (h + 2 * hk) * dd, dtype=dt)
+    inv, _ = d.rotary_frequencies(rd)
+    pos = torch.randint(0, 10 ** 6, (1, t), generator=g)
+    qd = qkv.to(DEV)
+    views = lambda a: (a[..., :h * dd].unflatten(-1, (h, dd)), a[..., h * dd:(h + hk) * dd].unflatten(-1, (hk, dd)))  # noqa: E731
+    got = d.apply_rotary(*views(qd), inv.to(DEV), pos.to(DEV), layout=layout, scale=1.1)
+    e = 6 * 2.0 ** -24 + 4 * 10 ** 6 * 2.0 ** -52  # as in test_rotary
+    for x, y in zip(views(qkv), got):
+        want, mag = rotary_oracle(x, inv, pos[None], layout, 1.1, False)
+        close(y, want, HALF[dt] * want.abs() + e * mag, f"{walk}")
+        assert torch.equal(y[..., rd:].cpu(), x[..., rd:])
+    d.apply_rotary(*views(qd), inv.to(DEV), pos.to(DEV), layout=layout, scale=1.1, inplace=True)
+    for x, y in zip(views(qd), got):
+        assert torch.equal(x, y)
+    assert torch.equal(qd[..., (h + hk) * dd:].cpu(), qkv[..., (h + hk) * dd:])
