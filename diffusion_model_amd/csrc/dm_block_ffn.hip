@@ -423,12 +423,17 @@ Operand take_operand(int64_t rows, int cols, Carver& ws) {
   return o;
 }
 
-// The product terms of two operands (`second`: of two more, of the same shape): one, or the six of split fp32.
+// The product terms of two operands (`second`: of two more, of the same shape): one, or the six of split fp32, those with a leading plane on
+// both sides last.
 template <typename T>
 void add_terms(GemmArgs& g, const Operand& a, const Operand& b, bool second = false) {
-  auto add = [&](uint64_t i, uint64_t j) { g.terms |= (i | j << 2 | (second ? 16 : 0)) << 5 * g.segments++; };
-  add(0, 0);
-  if (std::is_same<T, float>::value) { add(0, 1); add(1, 0); add(0, 2); add(2, 0); add(1, 1); }  // (no two plane tiles new at once but the first)
+  g.terms = 0;
+  g.segments = 0;
+  auto add = [&](uint64_t i, uint64_t j, int s) { g.terms |= (i | j << 2 | (s ? 16 : 0)) << 5 * g.segments++; };
+  if (std::is_same<T, float>::value)
+    for (int s = 0; s <= second; ++s) { add(2, 0, s); add(1, 0, s); add(1, 1, s); add(0, 1, s); add(0, 2, s); }  // (one plane tile new at once)
+  g.early = g.segments;
+  for (int s = 0; s <= second; ++s) add(0, 0, s);
   g.a[second] = a.p;
   g.b[second] = b.p;
   g.lda = a.ld;
@@ -466,7 +471,7 @@ int product(GemmArgs g, const Out& out, const void* bias, void* sums, void* part
   g.sums = sums;
   if (g.pair) g.out.vec = out.vec && g.out2.vec;
   g.sum_part = (float*)part + g.splits * g.split_stride;
-  g.sum_segments = std::is_same<T, float>::value ? 1 << 0 | 1 << 2 | 1 << 4 : 1;  // add_terms: each plane of A once
+  g.sum_segments = std::is_same<T, float>::value ? 1 << 0 | 1 << 1 | 1 << 5 : 1;  // add_terms: each plane of A once
   return gemm_launch<Mat<T>, AKS, BKS, EPI_STORE>(g, tile, st);
 }
 

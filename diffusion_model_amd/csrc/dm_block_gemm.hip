@@ -166,7 +166,10 @@ __device__ __forceinline__ void from_lds(const char DM_LDS* p, float (&v)[8]) {
 }
 
 constexpr int LDS_BIAS = 3 * 1024;  // see load_to_lds
-constexpr uint32_t UNBOUNDED = 0x80000000u, OUTSIDE = 0x80000000u;  // bytes of a buffer; an offset outside of every one
+constexpr uint32_t UNBOUNDED = 0x80000000u;  // bytes of a buffer
+// Offsets outside of every buffer (one inside is below 2^30): of a row or column that the tensor does not have; and, as a bit of an offset,
+// of k behind a step of fewer k.
+constexpr uint32_t OUTSIDE = 0xC0000000u, BEHIND = 0x80000000u;
 enum { EPI_STORE, EPI_GATE, EPI_GATE_F32, EPI_DACT, EPI_DACT_F32 };  // _F32: of split fp32 operands
 
 struct GemmArgs {
@@ -174,6 +177,7 @@ struct GemmArgs {
   int64_t plane_a, plane_b;           // bytes from one plane of an operand to the next
   uint64_t terms;                     // five bits per product term: plane of a, plane of b (two bits each), which of the two a and b
   int segments, iters;                // number of terms, k steps of GEMM_BK
+  int early;                          // the first terms that are taken over the whole range before the others are
   int64_t lda, ldb;                   // elements
   int64_t M;
   int N, K;                           // N: of one projection for EPI_GATE.  K: true length; a KC row is zero from there to the end of its piece
@@ -328,11 +332,15 @@ gemm_kernel(const GemmArgs p) {
   // keep their order, and so does the one with a step of fewer k: that step comes last.)
   const int shift = per % 8 && p.splits > 1 ? 0 : (tm + 2 * tn) & (p.segments > 1 && !(AKS && p.splits > 1) ? 3 : 7);
   const int whole = p.K / GEMM_BK < step1 ? p.K / GEMM_BK : step1;
-  // A term takes a group of steps, then the next term takes the same group (the last step, if it has fewer k, is one by itself).
+  // A term takes a group of steps, then the next term takes the same group (the last step, if it has fewer k, is one by itself).  The
+  // `early` terms, of split fp32 the small ones, go through the whole range first: an instruction's sum is as exact as the largest of what it adds,
+  // so small terms that met the main one's sum would lose as much in each instruction as the main term does (step of 65536 x 256 x 1024, relative
+  // to 64 bits: 0.7 to 2.4e-6 so and 1.6 to 3.4e-7 this way; 2180 and 2215 us, as the main term's planes are fetched once more).
   const int group = p.segments > 1 ? AKS && p.splits > 1 ? 1 : 4 : p.iters;
   auto group_end = [&](int from) __attribute__((always_inline)) { return from >= whole ? step1 : from + group < whole ? from + group : whole; };
   int seg = 0, step = step0, group0 = step0, group1 = group_end(step0);  // of the next stage to be asked for
-  bool moved = false;
+  int seg0 = 0, seg1 = p.early ? p.early : p.segments;                   // terms that take turns now
+  bool moved = false, again = false;
   const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2 + (other ? p.pair : 0) - LDS_BIAS, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2 - LDS_BIAS;
   constexpr int LOADS = sa.PASSES + sb.PASSES;
   // (kept in registers: a scalar load among the products would wait for every LDS read under way)
@@ -363,18 +371,28 @@ gemm_kernel(const GemmArgs p) {
   struct Request { i32x4 a, b, b2; uint32_t at, a_bytes, b_bytes; bool sum; };
   auto request = [&](Request& r, int piece, int turn) __attribute__((always_inline)) {
     if (piece == 0) {
+      if (again) {  // (not where `again` is set: loads of the step before follow there)
+        asm volatile("");
+        again = false;
+#pragma unroll
+        for (int j = 0; j < sa.PASSES; ++j)
+          if (!AKS && sa.off[j] < OUTSIDE) sa.off[j] &= ~BEHIND;
+#pragma unroll
+        for (int j = 0; j < sb.PASSES; ++j)
+          if (!BKS && sb.off[j] < OUTSIDE) sb.off[j] &= ~BEHIND;
+      }
       uint32_t at = (step | 7) < whole ? step ^ shift : step, a_bytes = UNBOUNDED, b_bytes = UNBOUNDED;
       const int left = turn < turns ? k_end - (int)at * GEMM_BK : 0;
-      if (left < GEMM_BK) {  // the last step, of a k range of no whole steps (behind it come only its own terms), or behind the range
+      if (left < GEMM_BK) {  // the last step, of a k range of no whole steps (behind it come its own terms, or the range again), or behind the range
         asm volatile("");    // (a branch: every step would pay for the selection)
         a_bytes = !left ? 0 : AKS ? left * lda2 + LDS_BIAS : UNBOUNDED;  // rows of a KS tile end with the k range
         b_bytes = !left ? 0 : BKS ? left * ldb2 + LDS_BIAS : UNBOUNDED;
 #pragma unroll
         for (int j = 0; j < sa.PASSES; ++j)
-          if (!AKS && sa.k_of(wave, lane, j) >= left) sa.off[j] = OUTSIDE;
+          if (!AKS && sa.k_of(wave, lane, j) >= left) sa.off[j] |= BEHIND;
 #pragma unroll
         for (int j = 0; j < sb.PASSES; ++j)
-          if (!BKS && sb.k_of(wave, lane, j) >= left) sb.off[j] = OUTSIDE;
+          if (!BKS && sb.k_of(wave, lane, j) >= left) sb.off[j] |= BEHIND;
       }
       r.sum = SUMS && turn < turns && (sum_segments >> seg & 1);
       pin(at), pin(a_bytes), pin(b_bytes);
@@ -394,9 +412,15 @@ gemm_kernel(const GemmArgs p) {
       ++step;
       moved = segments != 1 && step == group1;
       if (moved) {
-        if (++seg == segments) {
-          seg = 0;
+        if (++seg == seg1) {
           group0 = group1;
+          if (group0 >= step1 && seg1 < segments) {  // the range again, with the other terms
+            seg0 = seg1;
+            seg1 = segments;
+            group0 = step0;
+            again = true;
+          }
+          seg = seg0;
           group1 = group_end(group0);
         }
         step = group0;

@@ -165,3 +165,27 @@ def test_rotary_of_several_heads_per_thread(walk, layout, dtype):
     for x, y in zip(views(qd), got):
         assert torch.equal(x, y)
     assert torch.equal(qd[..., (h + hk) * dd:].cpu(), qkv[..., (h + hk) * dd:])
+
+
+@pytest.mark.parametrize("size", [(40000, 256, 320, 256), (3000, 700, 1500, 700)], ids=lambda s: "x".join(map(str, s)))
+def test_fp32_steps_are_as_exact_as_fp32_products(size):
+    """Every result's error against 64 bits, over its elements, beside that of the same formula in fp32 products and sums: twice it at most.
+    (Errors of one sign in dh would add up in the bias' gradients over the rows.)"""
+    m, dd, f, n = size
+    g = torch.Generator(device=DEV).manual_seed(5)
+    mk = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    x, dy, w = mk(m, dd), mk(m, n), [mk(f, dd) * dd ** -0.5, mk(f, dd) * dd ** -0.5, mk(n, f) * f ** -0.5]
+    b = [0.1 * mk(f), 0.1 * mk(f), 0.1 * mk(n)]
+    got = step(x, dy, w, b, "silu")
+
+    def formula(t):
+        X, DY, wg, wu, wd, bg, bu, bd = [v.to(t) for v in (x, dy, *w, *b)]
+        gate, up = X @ wg.T + bg, X @ wu.T + bu
+        s = torch.sigmoid(gate)
+        h, dh = gate * s * up, DY @ wd
+        dg, du = dh * up * s * (1 + gate * torch.sigmoid(-gate)), dh * gate * s
+        return h @ wd.T + bd, dg @ wg + du @ wu, dg.T @ X, du.T @ X, DY.T @ h, dg.sum(0), du.sum(0), DY.sum(0)
+    for name, t, plain, want in zip(NAMES, got, formula(torch.float32), formula(torch.float64)):
+        err, ref = ((v.double() - want).norm() / want.norm() for v in (t, plain))
+        print(size, name, "%.2e %.2e" % (err, ref))
+        assert err <= 2 * ref, (name, err, ref)
