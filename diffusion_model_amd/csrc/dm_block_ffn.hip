@@ -708,6 +708,7 @@ int dm_gated_ffn(const void* x_dev, int64_t x_stride, const void* w_gate_dev, co
   const FfnSizes z = {M, D, F, N, dtype};
   if (const int rc = ffn_check(who, z, activation)) return rc;
   if (M == 0) return 0;
+  if (M == 1) x_stride = D;  // (rows of a product's second operand end where the stride says)
   if (ffn_check_matrix(who, "x", x_dev, x_stride, M, D, dtype) || ffn_check_matrix(who, "w_gate", w_gate_dev, D, F, D, dtype) ||
       ffn_check_matrix(who, "w_up", w_up_dev, D, F, D, dtype) || ffn_check_matrix(who, "w_down", w_down_dev, F, N, F, dtype))
     return 1;
@@ -742,6 +743,7 @@ int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_d
     }
     return 0;
   }
+  if (M == 1) { dy_stride = N; x_stride = D; }  // (rows of a product's second operand end where the stride says)
   if (ffn_check_matrix(who, "dy", dy_dev, dy_stride, M, N, dtype) || ffn_check_matrix(who, "x", x_dev, x_stride, M, D, dtype) ||
       ffn_check_matrix(who, "w_gate", w_gate_dev, D, F, D, dtype) || ffn_check_matrix(who, "w_up", w_up_dev, D, F, D, dtype) ||
       ffn_check_matrix(who, "w_down", w_down_dev, F, N, F, dtype))

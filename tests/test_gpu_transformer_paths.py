@@ -189,3 +189,29 @@ def test_fp32_steps_are_as_exact_as_fp32_products(size):
         err, ref = ((v.double() - want).norm() / want.norm() for v in (t, plain))
         print(size, name, "%.2e %.2e" % (err, ref))
         assert err <= 2 * ref, (name, err, ref)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_one_row_has_any_stride(dtype):
+    """The library's entry points with one row: the distance to a next row, which is not there, does not matter."""
+    dt, code = DTYPES[dtype], {"fp32": 0, "bf16": 1}[dtype]
+    g = torch.Generator().manual_seed(2)
+    x, dy, w, _ = ffn_case(g, 1, 64, 136, 72, dt, False)
+    xd, dyd, wd = x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w]
+    y, saved = d.gated_ffn(xd, *wd, save=True)
+    want = d.gated_ffn_backward(dyd, xd, *wd, saved, bias=True)
+    L = _lib.lib()
+    nbytes = L.dm_gated_ffn_backward_workspace_bytes(1, 64, 136, 72, code)
+    fbytes = L.dm_gated_ffn_workspace_bytes(1, 64, 136, 72, code, 0)
+    stream = torch.cuda.current_stream().cuda_stream
+    for stride in (0, 8, 1, 1 << 22):
+        got = [torch.full_like(t, 3.0) for t in want]
+        ws = torch.empty(nbytes + fbytes, dtype=torch.uint8, device=DEV)
+        _lib.check(L.dm_gated_ffn_backward(dyd.data_ptr(), stride, xd.data_ptr(), stride, *(t.data_ptr() for t in wd), saved.data_ptr(),
+                                           *(t.data_ptr() for t in got), 1, 64, 136, 72, 0, code, ws.data_ptr(), nbytes, stream))
+        for name, p, q in zip(NAMES[1:], got, want):
+            assert torch.equal(p, q), (stride, name)
+        out = torch.full_like(y, 3.0)
+        _lib.check(L.dm_gated_ffn(xd.data_ptr(), stride, *(t.data_ptr() for t in wd), None, None, None, out.data_ptr(), None, 1, 64, 136, 72, 0, code,
+                                  ws.data_ptr(), fbytes, stream))
+        assert torch.equal(out, y), stride
