@@ -90,6 +90,13 @@ __device__ __forceinline__ void store8(const Out& o, int64_t m, int n, int N, co
   }
 }
 
+// Columns behind a row's end hold zeros whatever the row holds: the product of an infinite element with the zeros out there is NaN.
+__device__ __forceinline__ void zero_behind(int n, int N, float (&v)[8]) {
+  if (n + 8 > N)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = n + e < N ? v[e] : 0.f;
+}
+
 // ---- activations: value and slope in fp32, all but the erf form by way of s(z) = 1 / (1 + exp(-z)); tanh's by 1 + tanh(y) = 2 s(2 y).
 // Results that are rounded to 16 bits take the hardware's exp2 and reciprocal (relative error below 2^-20 for |z| < 16).
 template <bool FAST>
@@ -528,8 +535,9 @@ gemm_kernel(const GemmArgs p) {
   // eight columns, neighbouring lanes next to each other: written straight from the accumulators, rows a power of two apart crowd
   // on few of the L2's channels (41 us of a 256 x 256 tile's time, measured at a row of 8 KB).
   constexpr int ROWS = WM * 32, PITCH = BN * 4 + 16, COLS = GATE ? BN / 2 : BN, PIECES = COLS / 8, TASKS = ROWS * PIECES / (NW * 64);
-  const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces (with zeros: rows of B out of range are zero)
+  const int np = (p.N + 7) & ~7;  // intermediate results are padded to whole pieces of zeros
   static_assert(NW * 64 % PIECES == 0, "a thread keeps its columns");
+  const bool ragged = n0 + COLS > p.N;
   Out out = p.out;
   if (other) out.p = p.out2.p;
   float b1[8], b2[8];
@@ -593,11 +601,13 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) { v[e] += b1[e]; u[e] += b2[e]; }
         gate_values<!F32>(p.act, v, u, h);
+        if (ragged) zero_behind(n, p.N, h), zero_behind(n, p.N, u), zero_behind(n, p.N, v);
         store8<T, BETWEEN>(p.out, m, n, np, h);
         if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
       } else if constexpr (DACT) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) { u[e] = v[e] * (float)ug[t].v[e]; h[e] = v[e] * (float)ag[t].v[e]; }
+        if (ragged) zero_behind(n, p.N, u), zero_behind(n, p.N, h);
         store8<T, BETWEEN>(p.out, m, n, np, u);
         store8<T, BETWEEN>(p.out2, m, n, np, h);
       } else {
@@ -673,6 +683,7 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) { v[e] += bias_at<Kept>(p.bias, n + e, p.N); u[e] += bias_at<Kept>(p.bias2, n + e, p.N); }
       gate_values<!F32>(p.act, v, u, h);
+      zero_behind(n, p.N, h), zero_behind(n, p.N, u), zero_behind(n, p.N, v);
       store8<T, BETWEEN>(p.out, m, n, np, h);
       if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
     } else if constexpr (EPI == EPI_STORE) {
@@ -688,6 +699,7 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
       load8((const Kept*)p.ag + m * p.ldg + n, ag);
 #pragma unroll
       for (int e = 0; e < 8; ++e) { u[e] *= v[e]; h[e] = ag[e] * v[e]; }
+      zero_behind(n, p.N, u), zero_behind(n, p.N, h);
       store8<T, BETWEEN>(p.out, m, n, np, u);
       store8<T, BETWEEN>(p.out2, m, n, np, h);
     }

@@ -215,3 +215,28 @@ def test_one_row_has_any_stride(dtype):
         _lib.check(L.dm_gated_ffn(xd.data_ptr(), stride, *(t.data_ptr() for t in wd), None, None, None, out.data_ptr(), None, 1, 64, 136, 72, 0, code,
                                   ws.data_ptr(), fbytes, stream))
         assert torch.equal(out, y), stride
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("rows", [3, 70])
+def test_infinities_of_odd_widths_stay_infinities(rows, splits, dtype):
+    """16-bit rows whose hidden width is no whole number of pieces: an infinite element among positive numbers gives infinities, not NaN."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(1)
+    pos = lambda *s: (torch.rand(*s, generator=g) * 0.1 + 0.1).to(dt).to(DEV)  # noqa: E731
+    dd, f, n = 400, 205, 403
+    x, dy, w = pos(rows, dd), pos(rows, n), [pos(f, dd), pos(f, dd), pos(n, f)]
+    w[2] = w[2] * 0.1
+    clean = d.gated_ffn(x, *w, activation="relu")
+    xi, dyi = x.clone(), dy.clone()
+    xi[1, 5], dyi[2, 7] = float("inf"), float("inf")
+    keep = torch.arange(rows, device=DEV)
+    with plan("128x128", splits):
+        y = d.gated_ffn(xi, *w, activation="relu")
+        assert (y[1] == float("inf")).all() and torch.equal(y[keep != 1], d.gated_ffn(x, *w, activation="relu")[keep != 1]) and clean.isfinite().all()
+        _, saved = d.gated_ffn(x, *w, activation="relu", save=True)
+        dx, dwg, dwu, dwd = d.gated_ffn_backward(dyi, x, *w, saved, activation="relu")[:4]
+    assert (dx[2] == float("inf")).all() and dx[keep != 2].isfinite().all()
+    assert (dwg == float("inf")).all() and (dwu == float("inf")).all()
+    assert (dwd[7] == float("inf")).all() and dwd[:7].isfinite().all()
