@@ -347,7 +347,8 @@ gemm_kernel(const GemmArgs p) {
   auto group_end = [&](int from) __attribute__((always_inline)) { return from >= whole ? step1 : from + group < whole ? from + group : whole; };
   int seg = 0, step = step0, group0 = step0, group1 = group_end(step0);  // of the next stage to be asked for
   int seg0 = 0, seg1 = p.early ? p.early : p.segments;                   // terms that take turns now
-  bool moved = false, again = false;
+  bool moved = false;
+  int look = GEMM_BK;  // k left at a step: fewer are looked at closer
   const int64_t a0 = (AKS ? m0 : m0 * p.lda) * 2 + (other ? p.pair : 0) - LDS_BIAS, b0 = (BKS ? (int64_t)n0 : (int64_t)n0 * p.ldb) * 2 - LDS_BIAS;
   constexpr int LOADS = sa.PASSES + sb.PASSES;
   // (kept in registers: a scalar load among the products would wait for every LDS read under way)
@@ -378,28 +379,29 @@ gemm_kernel(const GemmArgs p) {
   struct Request { i32x4 a, b, b2; uint32_t at, a_bytes, b_bytes; bool sum; };
   auto request = [&](Request& r, int piece, int turn) __attribute__((always_inline)) {
     if (piece == 0) {
-      if (again) {  // (not where `again` is set: loads of the step before follow there)
-        asm volatile("");
-        again = false;
-#pragma unroll
-        for (int j = 0; j < sa.PASSES; ++j)
-          if (!AKS && sa.off[j] < OUTSIDE) sa.off[j] &= ~BEHIND;
-#pragma unroll
-        for (int j = 0; j < sb.PASSES; ++j)
-          if (!BKS && sb.off[j] < OUTSIDE) sb.off[j] &= ~BEHIND;
-      }
       uint32_t at = (step | 7) < whole ? step ^ shift : step, a_bytes = UNBOUNDED, b_bytes = UNBOUNDED;
       const int left = turn < turns ? k_end - (int)at * GEMM_BK : 0;
-      if (left < GEMM_BK) {  // the last step, of a k range of no whole steps (behind it come its own terms, or the range again), or behind the range
-        asm volatile("");    // (a branch: every step would pay for the selection)
-        a_bytes = !left ? 0 : AKS ? left * lda2 + LDS_BIAS : UNBOUNDED;  // rows of a KS tile end with the k range
-        b_bytes = !left ? 0 : BKS ? left * ldb2 + LDS_BIAS : UNBOUNDED;
+      if (left < look) {   // the last step, of a k range of no whole steps (behind it come its own terms, or the range again), or behind the range
+        asm volatile("");  // (a branch: every step would pay for the selection)
+        if (look > GEMM_BK) {  // the first step of the range taken again (not where that is found: loads of the step before follow there)
+          look = GEMM_BK;
 #pragma unroll
-        for (int j = 0; j < sa.PASSES; ++j)
-          if (!AKS && sa.k_of(wave, lane, j) >= left) sa.off[j] |= BEHIND;
+          for (int j = 0; j < sa.PASSES; ++j)
+            if (!AKS && sa.off[j] < OUTSIDE) sa.off[j] &= ~BEHIND;
 #pragma unroll
-        for (int j = 0; j < sb.PASSES; ++j)
-          if (!BKS && sb.k_of(wave, lane, j) >= left) sb.off[j] |= BEHIND;
+          for (int j = 0; j < sb.PASSES; ++j)
+            if (!BKS && sb.off[j] < OUTSIDE) sb.off[j] &= ~BEHIND;
+        }
+        if (left < GEMM_BK) {
+          a_bytes = !left ? 0 : AKS ? left * lda2 + LDS_BIAS : UNBOUNDED;  // rows of a KS tile end with the k range
+          b_bytes = !left ? 0 : BKS ? left * ldb2 + LDS_BIAS : UNBOUNDED;
+#pragma unroll
+          for (int j = 0; j < sa.PASSES; ++j)
+            if (!AKS && sa.k_of(wave, lane, j) >= left) sa.off[j] |= BEHIND;
+#pragma unroll
+          for (int j = 0; j < sb.PASSES; ++j)
+            if (!BKS && sb.k_of(wave, lane, j) >= left) sb.off[j] |= BEHIND;
+        }
       }
       r.sum = SUMS && turn < turns && (sum_segments >> seg & 1);
       pin(at), pin(a_bytes), pin(b_bytes);
@@ -425,7 +427,7 @@ gemm_kernel(const GemmArgs p) {
             seg0 = seg1;
             seg1 = segments;
             group0 = step0;
-            again = true;
+            look = 0x7fffffff;
           }
           seg = seg0;
           group1 = group_end(group0);
