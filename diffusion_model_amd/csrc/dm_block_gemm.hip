@@ -99,13 +99,17 @@ __device__ __forceinline__ void zero_behind(int n, int N, float (&v)[8]) {
 
 // ---- activations: value and slope in fp32, all but the erf form by way of s(z) = 1 / (1 + exp(-z)); tanh's by 1 + tanh(y) = 2 s(2 y).
 // Results that are rounded to 16 bits take the hardware's exp2 and reciprocal (relative error below 2^-20 for |z| < 16).
+// `rest`: 1 - s(z), where s is near 1 as exp(-z) s: the difference would hold none of its bits (z = 17) or too few (z = 9 for a slope of fp16).
 template <bool FAST>
-__device__ __forceinline__ float sigmoid(float z) {
-  if (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
-  return 1.f / (1.f + expf(-z));
+__device__ __forceinline__ float sigmoid(float z, float& rest) {
+  const float e = FAST ? __builtin_amdgcn_exp2f(z * -1.44269504f) : expf(-z);
+  const float s = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+  rest = s < 0.5f ? 1.f - s : e * s;
+  return s;
 }
 template <int ACT, bool FAST>
 __device__ __forceinline__ void activation(float v, float& value, float& slope) {
+  float rest;
   if constexpr (ACT == DM_ACT_RELU) {
     value = v > 0.f ? v : (v != v ? v : 0.f);
     slope = v > 0.f ? 1.f : 0.f;
@@ -114,13 +118,13 @@ __device__ __forceinline__ void activation(float v, float& value, float& slope) 
     value = v * cdf;
     slope = cdf + v * expf(-0.5f * v * v) * 0.39894228f;
   } else if constexpr (ACT == DM_ACT_GELU_TANH) {
-    const float s = sigmoid<FAST>(1.5957691f * (v + 0.044715f * v * v * v));
+    const float s = sigmoid<FAST>(1.5957691f * (v + 0.044715f * v * v * v), rest);
     value = v * s;
-    slope = s + v * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * v * v);
+    slope = s + v * s * rest * 1.5957691f * (1.f + 0.134145f * v * v);
   } else {
-    const float s = sigmoid<FAST>(v);
+    const float s = sigmoid<FAST>(v, rest);
     value = ACT == DM_ACT_SIGMOID ? s : v * s;
-    slope = ACT == DM_ACT_SIGMOID ? s * (1.f - s) : s * (1.f + v * (1.f - s));
+    slope = ACT == DM_ACT_SIGMOID ? s * rest : s * (1.f + v * rest);
   }
 }
 // f(constant) for the activation at run time

@@ -240,3 +240,27 @@ def test_infinities_of_odd_widths_stay_infinities(rows, splits, dtype):
     assert (dx[2] == float("inf")).all() and dx[keep != 2].isfinite().all()
     assert (dwg == float("inf")).all() and (dwu == float("inf")).all()
     assert (dwd[7] == float("inf")).all() and dwd[:7].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows", [3, 30, 150])
+def test_sigmoid_slope_of_large_gates(rows, dtype):
+    """s (1 - s) where 1 - s is far below s: relative to the slope itself."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(rows)
+    x, dy, w, b = ffn_case(g, rows, 8, 40, 24, dt, True)
+    b[0] = torch.linspace(9.0, 14.0 if dt != torch.float16 else 10.5, 40).to(dt)
+    b[1] = torch.full((40,), 64.0).to(dt)
+    w[0] = w[0] * 0.125
+    got = step(x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b], "sigmoid")
+    X, DY, (wg, wu, wd) = x.double(), dy.double(), [t.double() for t in w]
+    gate, up = X @ wg.T + b[0].double(), X @ wu.T + b[1].double()
+    dh = DY @ wd
+    dg = dh * up * torch.sigmoid(gate) * torch.sigmoid(-gate)
+    # g is of order 14 and a sum of 9 terms: 9 half steps of 16 move the slope by 2^-17; the exponential and the reciprocal of 16-bit types
+    # 2^-18, half a step of u and of dh (24 terms of their absolute sum); then two roundings of 16-bit types
+    rel = 2.0 ** -16 + (2 * HALF[dt] if dt != torch.float32 else 0.0)
+    err = rel * dg.abs() + 32 * 2.0 ** -24 * (DY.abs() @ wd.abs()) * (dg / dh).abs()
+    tiny = 2.0 ** -25 * (2 + dh.abs()) if dt == torch.float16 else 0.0  # half a step of fp16 numbers below the normal ones, of u act'(g) and dg
+    close(got[5], dg.sum(0), HALF[dt] * dg.sum(0).abs() + (err + tiny).sum(0) + (2.0 ** -25 if dt == torch.float16 else 0.0), "db_gate")
+    close(got[2], dg.T @ X, HALF[dt] * (dg.T @ X).abs() + (err + tiny).T @ X.abs() + (2.0 ** -25 if dt == torch.float16 else 0.0), "dw_gate")
