@@ -120,7 +120,7 @@ __device__ __forceinline__ void activation(float v, float& value, float& slope) 
   } else if constexpr (ACT == DM_ACT_GELU_TANH) {
     const float s = sigmoid<FAST>(1.5957691f * (v + 0.044715f * v * v * v), rest);
     value = v * s;
-    slope = s + v * s * rest * 1.5957691f * (1.f + 0.134145f * v * v);
+    slope = s + v * s * rest * 1.5957691f * (1.f + 0.134145f * fminf(v * v, 1e30f));  // (rest or s is 0 long before: not 0 times infinity)
   } else {
     const float s = sigmoid<FAST>(v, rest);
     value = ACT == DM_ACT_SIGMOID ? s : v * s;

@@ -264,3 +264,26 @@ def test_sigmoid_slope_of_large_gates(rows, dtype):
     tiny = 2.0 ** -25 * (2 + dh.abs()) if dt == torch.float16 else 0.0  # half a step of fp16 numbers below the normal ones, of u act'(g) and dg
     close(got[5], dg.sum(0), HALF[dt] * dg.sum(0).abs() + (err + tiny).sum(0) + (2.0 ** -25 if dt == torch.float16 else 0.0), "db_gate")
     close(got[2], dg.T @ X, HALF[dt] * (dg.T @ X).abs() + (err + tiny).T @ X.abs() + (2.0 ** -25 if dt == torch.float16 else 0.0), "dw_gate")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", "sigmoid"])
+@pytest.mark.parametrize("rows", [2, 30, 150])
+def test_slopes_of_huge_gates(rows, act, dtype):
+    """Gates of 1e6 to 1e20 either way: act(g) is g or 0 (sigmoid: 1 or 0), the slope 1 or 0 (sigmoid: 0)."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(rows)
+    x, dy, w, b = ffn_case(g, rows, 16, 24, 8, dt, True)
+    size = torch.tensor([1e6, -1e6, 1e10, -1e10, 1e13, -1e13, 1e15, -1e15, 1e18, -1e18, 1e20, -1e20]).to(dt)
+    b[0] = size.repeat(2)
+    w[2] = (w[2].float() * (1e-12 if act != "sigmoid" else 1.0)).to(dt)
+    got = step(x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b], act)
+    up = x.double() @ w[1].double().T + b[1].double()
+    ua = x.double().abs() @ w[1].double().abs().T + b[1].double().abs()
+    dh, dha = dy.double() @ w[2].double(), dy.double().abs() @ w[2].double().abs()
+    slope = (b[0] > 0).double() if act != "sigmoid" else torch.zeros(24, dtype=torch.float64)
+    dg, bound = dh * up * slope, (dha * ua * slope)
+    # two roundings of 16-bit types, 32 half steps for the two sums; the sum over the rows
+    err = (32 * 2.0 ** -24 + (2 * HALF[dt] if dt != torch.float32 else 0.0)) * bound
+    close(got[5], dg.sum(0), HALF[dt] * dg.sum(0).abs() + err.sum(0) + rows * 2.0 ** -24 * bound.sum(0), "db_gate")
+    assert all(t.isfinite().all() for t in got)
