@@ -121,15 +121,17 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     return (y, mean, rstd) if return_stats else y
 
 
-def layer_norm_backward(grad, x, weight, mean, rstd):
+def layer_norm_backward(grad, x, weight, mean, rstd, bias=None):
     """(dx, dweight, dbias) from the output's gradient and what ``layer_norm(..., return_stats=True)`` returned.  The parameters'
-    gradients are None where ``weight`` is None, otherwise of its type, summed over all rows in a fixed order."""
+    gradients are of their type, summed over all rows in a fixed order: both where there is a ``weight``, dbias alone where only
+    the forward call's ``bias`` is given, otherwise None."""
     dt = _dtype(x, "x")
     _like(grad, x, "grad")
     if x.dim() < 1 or x.shape[-1] < 1 or grad.shape != x.shape:
         raise RuntimeError(f"grad must have x's shape {tuple(x.shape)} (got {tuple(grad.shape)})")
     c = x.shape[-1]
     w = _vector(weight, c, x, "weight", (x.dtype, torch.float32))
+    b = _vector(bias, c, x, "bias", (x.dtype, torch.float32) if w is None else (w.dtype,))
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         _like(t, x, name, (torch.float32,))
         if t.shape != x.shape[:-1]:
@@ -141,11 +143,12 @@ def layer_norm_backward(grad, x, weight, mean, rstd):
     dx = _empty_like(x)
     dw = db = ws = None
     nbytes = 0
-    if w is not None:
-        dw, db = torch.empty_like(w), torch.empty_like(w)
+    p = b if w is None else w
+    if p is not None:
+        dw, db = None if w is None else torch.empty_like(w), torch.empty_like(p)
         nbytes = L.dm_layer_norm_backward_workspace_bytes(m, c)
         ws = _workspace(x, nbytes)
-    _call(x, L.dm_layer_norm_backward, g.data_ptr(), gstride, r.data_ptr(), stride, _ptr(w), dt if w is None else _DTYPES[w.dtype],
+    _call(x, L.dm_layer_norm_backward, g.data_ptr(), gstride, r.data_ptr(), stride, _ptr(w), dt if p is None else _DTYPES[p.dtype],
           mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), m, c, dt, _ptr(ws), nbytes)
     return dx, dw, db
 

@@ -287,3 +287,21 @@ def test_slopes_of_huge_gates(rows, act, dtype):
     err = (32 * 2.0 ** -24 + (2 * HALF[dt] if dt != torch.float32 else 0.0)) * bound
     close(got[5], dg.sum(0), HALF[dt] * dg.sum(0).abs() + err.sum(0) + rows * 2.0 ** -24 * bound.sum(0), "db_gate")
     assert all(t.isfinite().all() for t in got)
+
+
+@pytest.mark.parametrize("dtype,ptype", [("fp32", "fp32"), ("bf16", "bf16"), ("fp16", "fp32")])
+def test_layer_norm_backward_of_a_bias_without_weight(dtype, ptype):
+    dt, pt = DTYPES[dtype], DTYPES[ptype]
+    g = torch.Generator().manual_seed(3)
+    for rows, width in ((37, 100), (300, 1001), (0, 24), (5, 3), (2, 40000)):
+        x, dy, b = rand(g, rows, width, dtype=dt), rand(g, rows, width, dtype=dt), rand(g, width, dtype=pt)
+        _, mu, rs = d.layer_norm(x.to(DEV), None, b.to(DEV), return_stats=True)
+        dx, dw, db = d.layer_norm_backward(dy.to(DEV), x.to(DEV), None, mu, rs, bias=b.to(DEV))
+        assert dw is None and db.dtype == pt and db.shape == (width,)
+        want = dy.double().sum(0)
+        close(db, want, HALF[pt] * want.abs() + 64 * 2.0 ** -24 * dy.double().abs().sum(0), "db")
+        assert torch.equal(dx, d.layer_norm_backward(dy.to(DEV), x.to(DEV), None, mu, rs)[0])
+        w = torch.ones(width, dtype=pt, device=DEV)
+        assert torch.equal(d.layer_norm_backward(dy.to(DEV), x.to(DEV), w, mu, rs, bias=b.to(DEV))[2], db)
+    with pytest.raises(RuntimeError, match="bias"):
+        d.layer_norm_backward(dy.to(DEV), x.to(DEV), None, mu, rs, bias=b.to(DEV)[:-1])
