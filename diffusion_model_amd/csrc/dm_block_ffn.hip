@@ -6,8 +6,8 @@
 // Three paths.  Up to TOKEN_ROWS rows, and fp32 up to SKINNY_ROWS, the weights' bandwidth bounds the block, and every wave streams weight rows
 // straight into vector (gemv_kernel) or matrix (skinny_kernel) instructions; above that the tiled products of dm_block_gemm.hip, whose
 // smallest tile and split k range serve 16-bit decode batches.
-// Rounding: h, u act'(g), act(g), dg and du are kept in the tensors' type between the products.  The matrix pipe takes h, dg and du in
-// 16 bits and nothing wider; u act'(g) and act(g) are 16 bits for their bytes (32 would add 0.7 GB to a step of 8192 x 4096 x 11008, 3 % of
+// Rounding: h, u act'(g), act(g), dg and du are kept in the tensors' type between the products (but h of one or two rows in fp32: EXACT_ROWS).  The
+// matrix pipe takes h, dg and du in 16 bits and nothing wider; u act'(g) and act(g) are 16 bits for their bytes (32 would add 0.7 GB to a step of 8192 x 4096 x 11008, 3 % of
 // its time): a gradient has three roundings where results alone would have one, sqrt(3) of its error.  Every sum is fp32.
 // fp32 tensors are split into three bf16 terms and multiplied as six products (a1b1 a1b2 a2b1 a2b2 a1b3 a3b1; what is left out is below
 // 2^-25 of |a||b|): the fp32 matrix instructions have 1/16 of the bf16 ones' rate.
@@ -18,6 +18,9 @@
 namespace dmb {
 
 constexpr int TOKEN_ROWS = 4;  // gemv_kernel
+// ... which keeps h in 32 bits up to so many rows of 16-bit tensors.  Every wave reads all of h: 4096 x 11008 bf16 takes 46.9 us of one row with h in 16
+// bits and 47.4 with 32, 48.9 and 49.7 of two, but 51.7 and 59.9 of four.
+constexpr int EXACT_ROWS = 2;
 constexpr int SKINNY_ROWS = 64;  // skinny_kernel, fp32
 
 // ---- operands that the products cannot read as they are: fp32 (three bf16 planes) and rows of no whole number of 16-byte pieces
@@ -67,14 +70,17 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const PackJobs jobs) {
   }
 }
 
-template <typename T>
-struct Streamed {  // arguments of gemv_kernel and skinny_kernel
-  const T *x; int64_t xs; const T *w, *w2; int64_t ldw; const T *bias, *bias2; T* out; int64_t ldo; T *ug, *ag; bf16* planes; int M, N, K, act;
+// Arguments of gemv_kernel and skinny_kernel: weights of type T, x of X, results of O.  What a backward pass needs of h is written beside it, as
+// elements of the weights' type (`kept`) or planes.
+template <typename T, typename X, typename O>
+struct Streamed {
+  const X* x; int64_t xs; const T *w, *w2; int64_t ldw; const T *bias, *bias2; O* out; int64_t ldo; T *ug, *ag, *kept; bf16* planes; int M, N, K, act;
 };
+using StreamedF32 = Streamed<float, float, float>;
 
 // h, and what the backward pass needs, of one element from its two sums; the padding of a row holds zeros.
-template <typename T>
-__device__ __forceinline__ void finish_gate(const Streamed<T>& p, int n, int64_t at, float g, float u) {
+template <typename T, typename X, typename O>
+__device__ __forceinline__ void finish_gate(const Streamed<T, X, O>& p, int n, int64_t at, float g, float u) {
   if (n >= ((p.N + 7) & ~7)) return;
   float h = 0.f, ag = 0.f;
   if (n < p.N) {
@@ -87,7 +93,8 @@ __device__ __forceinline__ void finish_gate(const Streamed<T>& p, int n, int64_t
   } else {
     u = 0.f;
   }
-  p.out[at] = (T)h;
+  p.out[at] = (O)h;
+  if (p.kept) p.kept[at] = (T)h;
   if (p.ug) { p.ug[at] = (T)u; p.ag[at] = (T)ag; }
   if (p.planes) {
     bf16 t[3];
@@ -117,9 +124,9 @@ __device__ __forceinline__ float wave_sums(float (&v)[NV], int lane) {
   return s;
 }
 
-template <typename T, int MR, bool GATE, int KSPLIT>
+template <typename T, typename X, typename O, int MR, bool GATE, int KSPLIT>
 __global__ void __launch_bounds__(256)
-gemv_kernel(const Streamed<T> p) {
+gemv_kernel(const Streamed<T, X, O> p) {
   constexpr int V = 16 / sizeof(T), R = 4, P = GATE ? 2 : 1, GROUPS = 4 / KSPLIT, NV = MR * R;
   __shared__ float red[KSPLIT > 1 ? KSPLIT : 1][GROUPS][P][NV];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave / KSPLIT, part = wave % KSPLIT;
@@ -134,13 +141,14 @@ gemv_kernel(const Streamed<T> p) {
   float acc[P][NV] = {};
   auto multiply = [&](int k, auto pieces) __attribute__((always_inline)) {  // a piece of every row from k on
     constexpr int N = decltype(pieces)::value;
-    Piece<T, N> a[P][R], b[MR];
+    Piece<T, N> a[P][R];
+    Piece<X, N> b[MR];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int q = 0; q < P; ++q) a[q][r] = *reinterpret_cast<const Piece<T, N>*>(rows[q][r] + k);
 #pragma unroll
-    for (int m = 0; m < MR; ++m) b[m] = *reinterpret_cast<const Piece<T, N>*>(p.x + (m < p.M ? m : p.M - 1) * p.xs + k);
+    for (int m = 0; m < MR; ++m) b[m] = *reinterpret_cast<const Piece<X, N>*>(p.x + (m < p.M ? m : p.M - 1) * p.xs + k);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -174,22 +182,22 @@ gemv_kernel(const Streamed<T> p) {
   if (lane >= NV || m >= p.M) return;
   const int64_t at = (int64_t)m * p.ldo + n;
   if constexpr (GATE) finish_gate(p, n, at, s[0], s[P - 1]);
-  else if (n < p.N) p.out[at] = (T)(s[0] + (p.bias ? (float)p.bias[n] : 0.f));
+  else if (n < p.N) p.out[at] = (O)(s[0] + (p.bias ? (float)p.bias[n] : 0.f));
 }
 
-template <typename T, bool GATE>
-int gemv_launch(const Streamed<T>& a, hipStream_t st) {
+template <bool GATE, typename T, typename X, typename O>
+int gemv_launch(const Streamed<T, X, O>& a, hipStream_t st) {
   const int groups = (int)(((int64_t)a.N + 7) / 8 * 8 + 3) / 4;  // of four rows, the padding of h among them
   int split = 1;  // sixteen waves for every CU, as long as each has a load of its own
   while (split < 4 && groups * split < 4096 && a.K > split * 64 * (int)(16 / sizeof(T))) split *= 2;
   auto run = [&](auto mr, auto ks) {
     constexpr int MR = decltype(mr)::value, KS = decltype(ks)::value;
-    gemv_kernel<T, MR, GATE, KS><<<dim3((groups + 4 / KS - 1) / (4 / KS)), dim3(256), 0, st>>>(a);
+    gemv_kernel<T, X, O, MR, GATE, KS><<<dim3((groups + 4 / KS - 1) / (4 / KS)), dim3(256), 0, st>>>(a);
   };
   auto rows = [&](auto ks) {
     if (a.M == 1) run(std::integral_constant<int, 1>{}, ks);
     else if (a.M == 2) run(std::integral_constant<int, 2>{}, ks);
-    else run(std::integral_constant<int, 4>{}, ks);
+    else if constexpr (sizeof(X) == sizeof(O) || sizeof(T) == 4) run(std::integral_constant<int, 4>{}, ks);  // (EXACT_ROWS)
   };
   if (split == 1) rows(std::integral_constant<int, 1>{});
   else if (split == 2) rows(std::integral_constant<int, 2>{});
@@ -223,7 +231,7 @@ constexpr int SKINNY_WAVES = 8;
 // of every row (U * 64 bytes on end), and the next chunk is on its way while one is multiplied.  Blocks begin at different chunks: in
 // step they would all ask for the same columns of rows a power of two apart, which lie on few of the memory's channels.
 template <int MT, bool GATE>
-__global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const Streamed<float> p) {
+__global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const StreamedF32 p) {
   constexpr int V = 4, STEP = 4 * V, P = GATE ? 2 : 1;
   constexpr int U = MT == 4 ? 2 : 4;
   __shared__ f32x4 red[SKINNY_WAVES][P][MT][64];
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(SKINNY_WAVES * 64) skinny_kernel(const Streame
 }
 
 template <bool GATE>
-int skinny_launch(const Streamed<float>& a, hipStream_t st) {
+int skinny_launch(const StreamedF32& a, hipStream_t st) {
   const dim3 grid((a.N + 15) / 16), block(SKINNY_WAVES * 64);
   if (a.M <= 16) skinny_kernel<1, GATE><<<grid, block, 0, st>>>(a);
   else if (a.M <= 32) skinny_kernel<2, GATE><<<grid, block, 0, st>>>(a);
@@ -314,11 +322,11 @@ int skinny_launch(const Streamed<float>& a, hipStream_t st) {
   return launched("dm_gated_ffn");
 }
 
-template <typename T, bool GATE>
-int streamed(const Streamed<T>& a, hipStream_t st) {
+template <bool GATE, typename T, typename X, typename O>
+int streamed(const Streamed<T, X, O>& a, hipStream_t st) {
   if constexpr (std::is_same<T, float>::value)
     if (a.M > TOKEN_ROWS) return skinny_launch<GATE>(a, st);
-  return gemv_launch<T, GATE>(a, st);
+  return gemv_launch<GATE>(a, st);
 }
 
 // ---- fp32 backward, up to SKINNY_ROWS rows: part[split][m][n] = sum over the split's k of A[m][k] B[k][n], B's rows in memory.  A thread takes
@@ -501,14 +509,19 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   const int64_t Fp = pad8(z.F);
   const Saved<T> kept(saved, z.M, z.F);
   if (z.M <= TOKEN_ROWS || (F32 && z.M <= SKINNY_ROWS && z.D >= 4 && z.F >= 4)) {
-    T* h = saved && !F32 ? (T*)kept.h.p : (T*)ws.take((size_t)z.M * Fp * sizeof(T));
-    if (!run) return 0;
     const int M = (int)z.M;
-    const Streamed<T> gate = {(const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp, kept.ug, kept.ag,
-                              saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act};
-    if (const int rc = streamed<T, true>(gate, st)) return rc;
-    const Streamed<T> down = {h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, M, z.N, z.F, act};
-    return streamed<T, false>(down, st);
+    auto both = [&](auto type) {  // of h
+      using H = decltype(type);
+      H* h = (H*)ws.take((size_t)z.M * Fp * sizeof(H));
+      if (!run) return 0;
+      const Streamed<T, T, H> gate = {(const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp,
+                                      kept.ug, kept.ag, saved && !F32 ? (T*)kept.h.p : nullptr, saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act};
+      if (const int rc = streamed<true>(gate, st)) return rc;
+      const Streamed<T, H, T> down = {h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, nullptr,
+                                      M, z.N, z.F, act};
+      return streamed<false>(down, st);
+    };
+    return z.M <= EXACT_ROWS ? both(float()) : both(T());
   }
   PackJobs jobs = {};
   const Operand x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws), wg = prepare_operand<T>(jobs, in.wg, z.D, z.F, z.D, ws),

@@ -305,3 +305,20 @@ def test_layer_norm_backward_of_a_bias_without_weight(dtype, ptype):
         assert torch.equal(d.layer_norm_backward(dy.to(DEV), x.to(DEV), w, mu, rs, bias=b.to(DEV))[2], db)
     with pytest.raises(RuntimeError, match="bias"):
         d.layer_norm_backward(dy.to(DEV), x.to(DEV), None, mu, rs, bias=b.to(DEV)[:-1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("size", [(512, 1400, 264), (72, 33, 17)], ids=lambda s: "x".join(map(str, s)))
+def test_single_tokens_round_once(size, rows, dtype):
+    """Of one or two rows nothing but the result is rounded to 16 bits, with or without what a backward pass needs."""
+    dt = DTYPES[dtype]
+    dd, f, n = size
+    g = torch.Generator().manual_seed(rows + f)
+    x, dy, w, b = ffn_case(g, rows, dd, f, n, dt, True)
+    res, exact, _ = ffn_oracle(x, dy, w, b, "gelu")
+    xd, w, b = x.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+    y = d.gated_ffn(xd, *w, *b, activation="gelu")
+    e = 2.0 ** -24 * (32 + max(dd, f, n) / 8)
+    close(y, res["y"], HALF[dt] * res["y"].abs() + e * exact["y"] + (2.0 ** -25 if dt == torch.float16 else 0.0), "y")
+    assert torch.equal(y, d.gated_ffn(xd, *w, *b, activation="gelu", save=True)[0])
