@@ -250,7 +250,7 @@ __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t off0, uint32_t 
   asm volatile(
       "s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %2, 0 offen offset:%4 lds\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:%5 lds" ::"v"(off0),
       "v"(off1), "s"(rsrc), "s"(lds), "n"(FIRST), "n"(FIRST + 1024)
-      : "memory");
+      : "memory", "m0");
 }
 // (addresses have 48 bits: no stride)
 __device__ __forceinline__ i32x4 buffer_of(uint64_t u, uint32_t bytes) {
