@@ -159,7 +159,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     """(inv_freq, scale) for ``apply_rotary``: inv_freq[i] = base^(-2i / d), float64, with d = rotary_dim / axes (each axis has
     the whole range).  To stretch positions trained up to ``original_length`` by ``factor``: "linear" divides all frequencies;
     "ntk" raises the base so that the slowest pair is divided by ``factor``; "yarn" divides the pairs that turn less than once over
-    the trained length, keeps those that turn more than 32 times, blends between, and scales by 0.1 ln(factor) + 1."""
+    the trained length, keeps those that turn more than 32 times, blends between (linearly in the pair, from the last whole pair before the
+    one that turns 32 times to the first one behind that which turns once, which may lie behind the slowest pair), and scales by 0.1 ln(factor) + 1."""
     if axes < 1 or rotary_dim < 0 or rotary_dim % (2 * axes):
         raise ValueError(f"rotary_dim {rotary_dim} must be a multiple of {2 * axes} (pairs on {axes} axes)")
     if base <= 0 or factor <= 0:
@@ -181,7 +182,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
         def pair_that_turns(n):
             return span * math.log(original_length / (n * 2 * math.pi)) / math.log(base)
         low = max(math.floor(pair_that_turns(32)), 0)
-        high = min(math.ceil(pair_that_turns(1)), span - 1)
+        high = min(math.ceil(pair_that_turns(1)), 2 * span - 1)
         ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
         inv = inv / factor * ramp + inv * (1 - ramp)
         scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0

@@ -147,3 +147,23 @@ def test_rotary_frequencies():
                 dict(rotary_dim=8, factor=0.0), dict(rotary_dim=8, scaling="cubic"), dict(rotary_dim=8, scaling="yarn", factor=2.0)):
         with pytest.raises(ValueError):
             d.rotary_frequencies(**bad)
+
+
+@pytest.mark.parametrize("dim,base,length,factor", [(128, 10000.0, 131072, 4.0), (128, 10000.0, 65536, 4.0), (8, 10000.0, 8192, 16.0),
+                                                     (64, 500.0, 100000, 8.0), (128, 10000.0, 4096, 8.0), (128, 10000.0, 10 ** 11, 2.0)])
+def test_yarn_blends_every_pair_that_turns_more_than_once(dim, base, length, factor):
+    """A pair is divided whole only from where pairs turn less than once over the trained length, also where that lies behind the last one."""
+    pairs = dim // 2
+    inv, _ = d.rotary_frequencies(dim, base=base)
+    yarn, _ = d.rotary_frequencies(dim, base=base, scaling="yarn", factor=factor, original_length=length)
+    turns = inv * length / (2 * math.pi)
+
+    def pair(n):  # base^(-i / pairs) length = 2 pi n
+        return pairs * math.log(length / (2 * math.pi * n)) / math.log(base)
+    first, last = max(math.floor(pair(32)), 0), min(math.ceil(pair(1)), dim - 1)
+    for i in range(pairs):
+        part = min(max((i - first) / (last - first), 0.0), 1.0) if last > first else 0.0
+        want = inv[i].item() * ((1 - part) + part / factor)
+        assert abs(yarn[i].item() - want) <= 4e-16 * want, (i, turns[i].item())
+        if turns[i] > 1:
+            assert yarn[i] > inv[i] / factor * (1 + 1e-12), i
