@@ -329,7 +329,7 @@ int streamed(const Streamed<T, X, O>& a, hipStream_t st) {
   return gemv_launch<GATE>(a, st);
 }
 
-// ---- fp32 backward, up to SKINNY_ROWS rows: part[split][m][n] = sum over the split's k of A[m][k] B[k][n], B's rows in memory.  A thread takes
+// ---- fp32 backward of few rows (columns_fit): part[split][m][n] = sum over the split's k of A[m][k] B[k][n], B's rows in memory.  A thread takes
 // four columns of sixteen rows and walks k; A's part lies in LDS.  Bound by B's bytes, where tiles of split operands would first write three
 // planes of it; the parts are joined like those of a tile's split range.
 constexpr int COLUMN_ROWS = 16, COLUMN_K = 128;  // k per split, at most
@@ -401,6 +401,16 @@ struct Carver {
 struct Operand { const void* p; int64_t ld, plane; };
 
 struct FfnSizes { int64_t M; int D, F, N, dtype; };
+
+// fp32 backward passes by column_kernel: where splitting the weights into planes costs more than multiplying in vector instructions, so for
+// large weights and few rows.  Measured, backward pass in us with it and with tiles of planes, weights of ... elements each:
+// 1M (512 x 2048) 62 and 55 of one row; 4.4M (1918 x 2281) 104 and 114 of one, 123 and 116 of 16; 7.6M (1456 x 5223) 112 and 154 of one, 163 and 162
+// of 32; 11M (2048 x 5504) 184 and 208 of 17, 223 and 215 of 48; 45M (4096 x 11008) 416 and 742 of one, 605 and 777 of 48, 822 and 791 of 64.
+inline bool columns_fit(const FfnSizes& z) {
+  if (z.D < 4 || z.F < 4 || z.M > SKINNY_ROWS) return false;  // its pieces; the rows that its tests reach
+  if (forced_tile >= 0) return forced_tile == FORCED_COLUMNS;
+  return z.M <= 48 && z.M << 18 <= (int64_t)z.F * (2LL * z.D + z.N) / 3 - (1 << 21);
+}
 
 template <typename T>
 int pack_launch(const PackJobs& jobs, hipStream_t st) {
@@ -559,7 +569,7 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
                  hipStream_t st) {
   const int64_t Fp = pad8(z.F);
   const int terms = std::is_same<T, float>::value ? 6 : 1;
-  const bool few = std::is_same<T, float>::value && z.M <= SKINNY_ROWS && z.D >= 4 && z.F >= 4;  // column_kernel
+  const bool few = std::is_same<T, float>::value && columns_fit(z);
   PackJobs jobs = {};
   const Operand y = prepare_operand<T>(jobs, dy, dys, z.M, z.N, ws), x = prepare_operand<T>(jobs, in.x, in.xs, z.M, z.D, ws, gr.dwg || gr.dwu);
   Operand wd = {}, wg = {}, wu = {};
@@ -681,7 +691,7 @@ extern "C" {
 
 int dm_debug_ffn_plan(int tile, int splits) {
   using namespace dmb;
-  if (tile < -1 || tile >= TILES || splits < 1 || splits > 64) return fail("dm_debug_ffn_plan: tile %d (-1 to 2), %d parts (1 to 64)", tile, splits);
+  if (tile < -1 || tile > FORCED_COLUMNS || splits < 1 || splits > 64) return fail("dm_debug_ffn_plan: tile %d (-1 to 3), %d parts (1 to 64)", tile, splits);
   forced_tile = tile;
   forced_splits = splits;
   return 0;

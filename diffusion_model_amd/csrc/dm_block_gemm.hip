@@ -732,7 +732,8 @@ inline size_t gemm_part_bytes(int64_t M, int N, int outs, int splits) {
   return splits > 1 ? (size_t)splits * outs * M * (round_up(N, 8) + 1) * 4 : 0;  // products, and sums of A
 }
 
-// Tests run every product with every tile: dm_debug_ffn_plan, of the calling thread.
+// Tests run every product with every tile: dm_debug_ffn_plan, of the calling thread.  FORCED_COLUMNS: column_kernel wherever it can.
+constexpr int FORCED_COLUMNS = TILES;
 inline thread_local int forced_tile = -1, forced_splits = 1;
 
 // Tile and split of the k range: the least of an estimate in microseconds.  A product's time is that of its stages - alone on a CU, or two
@@ -742,7 +743,7 @@ inline thread_local int forced_tile = -1, forced_splits = 1;
 // bf16 and fp32, all products of both passes): what it picks takes 2 % longer than the best on average and 30 % at worst, where always
 // taking MID unsplit would take 66 % longer.  `outs`: products per n (2: both projections).
 inline GemmPlan gemm_plan(int64_t M, int N, int steps, int terms, int outs, int bytes, bool slim) {
-  if (forced_tile >= 0) {
+  if (forced_tile >= 0 && forced_tile < TILES) {
     GemmPlan forced = {forced_tile == TILE_SLIM && !slim ? (int)TILE_MID : forced_tile, 1, 0};
     const int per = split_steps(steps, forced_splits);
     forced.splits = (steps + per - 1) / per;

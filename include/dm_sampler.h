@@ -362,7 +362,8 @@ int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_d
                           void* stream);
 /* Test hook, for the calling thread: the tiled products of the gated block run with this tile (0: 256 x 256, 1: 128 x 128,
  * 2: 64 x 128 where a product has it, 128 x 128 elsewhere) and k ranges of `splits` parts (1 to 64; fewer where the range is shorter)
- * instead of what the sizes would choose; tile -1: as the sizes choose.  Workspace sizes follow. */
+ * instead of what the sizes would choose; tile 3: as the sizes choose, but the backward pass of up to 64 fp32 rows (widths from 4 on) by
+ * its kernel for few rows; tile -1: as the sizes choose.  Workspace sizes follow. */
 int dm_debug_ffn_plan(int tile, int splits);
 
 #ifdef __cplusplus

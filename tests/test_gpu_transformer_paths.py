@@ -10,13 +10,14 @@ from test_gpu_transformer import DEV, DTYPES, HALF, _norm_bounds, close, ffn_cas
 pytestmark = pytest.mark.gpu
 NAMES = ("y", "dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down")
 TILES = {"256x256": 0, "128x128": 1, "64x128": 2}
+COLUMNS = 3
 
 
 class plan:
     """The tiled products of the block with one tile and k ranges of `splits` parts."""
 
     def __init__(self, tile, splits):
-        self.args = TILES[tile], splits
+        self.args = TILES.get(tile, tile), splits
 
     def __enter__(self):
         _lib.check(_lib.lib().dm_debug_ffn_plan(*self.args))
@@ -322,3 +323,31 @@ def test_single_tokens_round_once(size, rows, dtype):
     e = 2.0 ** -24 * (32 + max(dd, f, n) / 8)
     close(y, res["y"], HALF[dt] * res["y"].abs() + e * exact["y"] + (2.0 ** -25 if dt == torch.float16 else 0.0), "y")
     assert torch.equal(y, d.gated_ffn(xd, *w, *b, activation="gelu", save=True)[0])
+
+
+@pytest.mark.parametrize("size", [(1, 64, 256, 64), (3, 40, 24, 56), (6, 5, 7, 3), (17, 100, 130, 100), (20, 40, 8, 5), (37, 515, 130, 129), (64, 63, 33, 1),
+                                  (2, 4, 4, 1), (33, 1030, 1100, 260), (64, 300, 2000, 1027), (48, 4, 5000, 4)], ids=lambda s: "x".join(map(str, s)))
+def test_few_fp32_rows_without_planes(size):
+    """The backward pass that reads fp32 weights as they lie, at sizes where it is not chosen too: widths off its pieces, blocks of 16 rows with a
+    rest, split sums, rows inside wider arrays."""
+    m, dd, f, n = size
+    g = torch.Generator().manual_seed(m + f)
+    x, dy, w, b = ffn_case(g, m, dd, f, n, torch.float32, True)
+    wide, pad = torch.full((m, dd + 3), float("nan"), device=DEV), torch.full((m, n + 5), float("nan"), device=DEV)
+    wide[:, 2:2 + dd], pad[:, 4:4 + n] = x.to(DEV), dy.to(DEV)
+    args = wide[:, 2:2 + dd], pad[:, 4:4 + n], [t.to(DEV) for t in w], [t.to(DEV) for t in b], "silu"
+    with plan(COLUMNS, 1):
+        got, again = step(*args), step(*args)
+    for (name, want, tol), t, t2 in zip(ffn_bounds(x, dy, w, b, "silu", torch.float32), got, again):
+        close(t, want, tol, f"{name} {size}")
+        assert torch.equal(t, t2), name
+
+
+@pytest.mark.parametrize("rows", [1, 22, 23])
+def test_few_fp32_rows_of_large_weights(rows):
+    """Both sides of the rows up to which 8 million elements of each weight are read as they lie."""
+    g = torch.Generator().manual_seed(rows)
+    x, dy, w, b = ffn_case(g, rows, 1999, 3999, 2010, torch.float32, True)
+    got = step(x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b], "silu")
+    for (name, want, tol), t in zip(ffn_bounds(x, dy, w, b, "silu", torch.float32), got):
+        close(t, want, tol, f"{name} {rows}")
