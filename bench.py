@@ -59,19 +59,25 @@ DM_X6 = int(os.environ.get("DM_X6", "487"))
 
 def split16_mfmas_per_product(k):
     return 3 if (DM_X6 & 16) or (DM_X6 & X6_CLASSES[k]) else 6
-# PMC / rocprofv3 summaries of THIS build (profiles/README.md): each file carries the key of the library it was measured on
-# (`build_key`, __graft_entry__.build_key()); a figure whose key differs from the loaded library's is reported as null
-TRAFFIC_FILE = os.path.join(ROOT, "profiles", "r3_traffic.json")
-ROCPROF_FILE = os.path.join(ROOT, "profiles", "r3_rocprof_summary.json")
+# PMC / rocprofv3 summaries of THESE kernels (profiles/README.md): each file carries the key of the sampler's sources and flags it was
+# measured on (`sampler_key`, __graft_entry__.sampler_key()); a figure whose key differs from the loaded library's is reported as null
+TRAFFIC_FILE = os.path.join(ROOT, "profiles", "sampler_traffic.json")
+ROCPROF_FILE = os.path.join(ROOT, "profiles", "sampler_rocprof_summary.json")
+
+
+def loaded_sampler_key():
+    """The key of the loaded library's sampler kernels; None when the library was not built from this tree."""
+    import __graft_entry__ as g
+    from diffusion_model_amd import _lib
+    return g.sampler_key() if _lib.lib().dm_build_key().decode() == g.build_key() else None
 
 
 def keyed_profile(path):
-    """A committed profile summary, or None when it was measured on another build of the library."""
-    from diffusion_model_amd import _lib
+    """A committed profile summary, or None when it was measured on other kernels."""
     if not os.path.exists(path):
         return None
     j = json.load(open(path))
-    return j if j.get("build_key") == _lib.lib().dm_build_key().decode() else None
+    return j if j.get("sampler_key") and j.get("sampler_key") == loaded_sampler_key() else None
 
 
 def flop_per_image_step(C_, S, cin, cout):
@@ -460,7 +466,8 @@ def main():
         "frac_fp32_mfma_peak_whole_path_algorithmic": value * n * flop_img_step / 1e12 / (PEAK_FP32_MFMA_TFLOPS * world),
     }
     from diffusion_model_amd import _lib as _l
-    res["build_key"] = _l.lib().dm_build_key().decode()  # sha256 of the library's sources + flags (profiles/ summaries are keyed by it)
+    res["build_key"] = _l.lib().dm_build_key().decode()  # sha256 of the library's sources + flags
+    res["sampler_key"] = loaded_sampler_key()            # ... of the sampler's kernels alone (profiles/ summaries are keyed by it)
     if rehearse:
         res["rehearsal"] = "CPU plumbing rehearsal (DM_BENCH_REHEARSE_CPU): stand-in sampler, `value` is not a measurement"
         args.no_roofline = args.no_cpu_baseline = args.no_configs = True

@@ -47,7 +47,8 @@ const char* dm_last_error(void);
 #define DM_ABI_VERSION 6
 int dm_version(void);
 /* sha256 over the compiler flags and sources this library was built from (__graft_entry__.build_key); "unkeyed" for a
- * hand build.  build() compares it with the tree it runs in, so a library built with other flags is not reused. */
+ * hand build.  build() compiles every time it is called; tests compare this with the tree they run in, so that no library of
+ * other sources or flags is taken for it. */
 const char* dm_build_key(void);
 
 /* ---- model container: replaces UNetMini.__init__ (diffusion/model.py:72-118) ---------- */

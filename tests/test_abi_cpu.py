@@ -45,6 +45,30 @@ def test_build_key_and_no_packed_fp32_op_sel():
     assert not g._PK.search("v_pk_mul_f32 v[78:79], v[82:83], s[4:5] op_sel_hi:[1,0]")
 
 
+def test_profiles_are_keyed_by_the_sampler_kernels(tmp_path, monkeypatch):
+    """bench.py takes a committed profile while the sampler's kernels are those it was measured on: a change of the transformer-block operators or of
+    the header's text leaves it valid, a change of a sampler kernel does not."""
+    import json
+    import shutil
+
+    import __graft_entry__ as g
+    import bench
+    key = g.sampler_key()
+    p = tmp_path / "profile.json"
+    for stored, want in ((key, True), ("0" * 64, False), (None, False)):
+        p.write_text(json.dumps({"sampler_key": stored, "classes": {}}))
+        assert (bench.keyed_profile(str(p)) is not None) == want
+    assert bench.keyed_profile(str(tmp_path / "missing.json")) is None
+    csrc = tmp_path / "csrc"
+    shutil.copytree(g.CSRC, csrc)
+    monkeypatch.setattr(g, "CSRC", str(csrc))
+    assert g.sampler_key() == key
+    for name, same in (("dm_block_gemm.hip", True), ("dm_block_common.h", True), ("dm_kernels_x6.hip", False)):
+        with open(csrc / name, "a") as f:
+            f.write("// changed\n")
+        assert (g.sampler_key() == key) == same, name
+
+
 def test_sampler_coefs_host_table_matches_torch():
     s = d.DDPMScheduler()
     o = O.make_schedule()

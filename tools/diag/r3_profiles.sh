@@ -1,8 +1,8 @@
 #!/bin/bash
 # Round-3 measurement passes on the GPU box (run through gpurun from the repo root):
-#   bash tools/diag/r3_profiles.sh stats|traffic|sq
+#   bash tools/diag/r3_profiles.sh cfg2|stats|traffic|sq
 # Every rocprofv3 pass is a run of its own (PMC passes never share a run with --stats / other counters' blocks).
-# Summaries: tools/diag/r3_summaries.py (run in the build container afterwards) -> profiles/r3_*.
+# Summaries: tools/diag/r3_summaries.py (run in the build container afterwards) -> profiles/sampler_*.
 set -u
 R=${GRAFT_REPO_ROOT:-$PWD}
 O=$R/gpurun_out/r3prof
@@ -14,6 +14,9 @@ cd /tmp && export TMPDIR=/tmp
 # traces the default once for the record.
 export DM_SPLIT=1
 case "$1" in
+cfg2)
+  timeout -k 10 300 rocprofv3 --kernel-trace --stats --output-format csv -d $O/prof_cfg2 -- python3 $R/bench.py --steps 3 --warmup 1 --no-cpu-baseline --no-configs > $O/prof_cfg2.json 2> $O/prof_cfg2.err || exit 1
+  ;;
 stats)
   timeout -k 10 300 rocprofv3 --kernel-trace --stats --output-format csv -d $O/prof_cfg2 -- python3 $R/bench.py --steps 3 --warmup 1 --no-cpu-baseline --no-configs > $O/prof_cfg2.json 2> $O/prof_cfg2.err || exit 1
   timeout -k 10 300 rocprofv3 --kernel-trace --stats --output-format csv -d $O/prof_cfg1 -- python3 $R/bench.py --steps 1 --warmup 1 --no-cpu-baseline --no-configs --sampler ancestral --ddim-steps 1000 --batch 64 > $O/prof_cfg1.json 2> $O/prof_cfg1.err || exit 1

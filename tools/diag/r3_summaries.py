@@ -1,7 +1,8 @@
-# Summaries of tools/diag/r3_profiles.sh's passes (gpurun_out/r3prof/*) -> profiles/r3_* (run in the build container):
+# Summaries of tools/diag/r3_profiles.sh's passes (gpurun_out/r3prof/*) -> profiles/sampler_* (run in the build container;
+# the passes of the other configurations and of the SQ counters are summarised where they were taken):
 #   python3 tools/diag/r3_summaries.py
-# Every JSON written here carries `build_key` = the key of the library the passes ran on (taken from the bench line each pass
-# printed); bench.py reports a figure from them only while the loaded library has the same key.
+# Every JSON written here carries `sampler_key` = the key of the sampler's sources and flags that the passes ran on (taken from the bench line
+# each pass printed); bench.py reports a figure from them only while the loaded library's sampler has the same key.
 # FETCH_SIZE / WRITE_SIZE are in KiB; on gfx950 FETCH_SIZE tallies 128-B requests as 64 B -> x2 (MI355X_MICROARCH.md, HBM).
 import collections
 import csv
@@ -67,18 +68,20 @@ keys = set()
 
 # ---- kernel-trace --stats passes: the CSV as rocprofv3 wrote it + the bench line of the same command
 for cfg in ("cfg1", "cfg2", "cfg4", "cfg5"):
-    shutil.copy(one(f"prof_{cfg}/*/*kernel_stats.csv"), os.path.join(DST, f"r3_{cfg}_kernel_stats.csv"))
+    if cfg != "cfg2" and not glob.glob(os.path.join(SRC, f"prof_{cfg}/*/*kernel_stats.csv")):
+        continue
+    shutil.copy(one(f"prof_{cfg}/*/*kernel_stats.csv"), os.path.join(DST, f"sampler_{cfg}_kernel_stats.csv"))
     j = bench_line(f"prof_{cfg}.json")
-    keys.add(j["build_key"])
-    json.dump(j, open(os.path.join(DST, f"r3_{cfg}_bench_profiled.json"), "w"), indent=1)
+    keys.add(j["sampler_key"])
+    json.dump(j, open(os.path.join(DST, f"sampler_{cfg}_bench_profiled.json"), "w"), indent=1)
 
 # ---- the DEFAULT scheduling of the cfg2 command (four sub-batch chains on parallel graph branches; r3_profiles.sh stats4), for the record:
 #      launches cover a quarter of the batch and overlap each other, so their durations are not a kernel's own time
 if glob.glob(os.path.join(SRC, "prof_cfg2_split4/*/*kernel_stats.csv")):
-    shutil.copy(one("prof_cfg2_split4/*/*kernel_stats.csv"), os.path.join(DST, "r3_cfg2_kernel_stats_split4.csv"))
+    shutil.copy(one("prof_cfg2_split4/*/*kernel_stats.csv"), os.path.join(DST, "sampler_cfg2_kernel_stats_split4.csv"))
     j = bench_line("prof_cfg2_split4.json")
-    keys.add(j["build_key"])
-    json.dump(j, open(os.path.join(DST, "r3_cfg2_bench_profiled_split4.json"), "w"), indent=1)
+    keys.add(j["sampler_key"])
+    json.dump(j, open(os.path.join(DST, "sampler_cfg2_bench_profiled_split4.json"), "w"), indent=1)
 
 # ---- class average of the dominant kernel by rocprof (cfg2 command), steady launches only
 rows = list(csv.DictReader(open(one("prof_cfg2/*/*kernel_trace.csv"))))
@@ -96,9 +99,9 @@ dom = cfg2["roofline"]["class"]
 out = {"source": "DM_SPLIT=1 (one sampling chain: a launch covers the whole batch, as in bench.py's per-class pass) rocprofv3 --kernel-trace --stats -- python3 bench.py --steps 3 --warmup 1 --no-cpu-baseline --no-configs "
                  "(tools/diag/r3_profiles.sh stats; DDIM-50, B=1024, fp32): per-kernel durations from the kernel trace, every launch of "
                  "the run (warm-up, timed passes and bench.py's per-class profiling pass)",
-       "build_key": cfg2["build_key"], "dominant_class": dom, "bench_line_avg_launch_us_same_run": cfg2["roofline"]["avg_launch_us"],
+       "sampler_key": cfg2["sampler_key"], "dominant_class": dom, "bench_line_avg_launch_us_same_run": cfg2["roofline"]["avg_launch_us"],
        "classes": classes, "per_kernel": summary}
-json.dump(out, open(os.path.join(DST, "r3_rocprof_summary.json"), "w"), indent=1)
+json.dump(out, open(os.path.join(DST, "sampler_rocprof_summary.json"), "w"), indent=1)
 print("dominant class %s: %d launches, %.1f us by rocprof (bench line of the same run: %.1f us)" % (dom, classes[dom]["launches"], classes[dom]["avg_us"], cfg2["roofline"]["avg_launch_us"]))
 
 # ---- HBM traffic (two PMC passes)
@@ -112,8 +115,8 @@ def load(path, name):
 
 f = load("pmc_fetch/*/*counter_collection.csv", "FETCH_SIZE")
 w = load("pmc_write/*/*counter_collection.csv", "WRITE_SIZE")
-keys.add(bench_line("pmc_fetch.json")["build_key"])
-keys.add(bench_line("pmc_write.json")["build_key"])
+keys.add(bench_line("pmc_fetch.json")["sampler_key"])
+keys.add(bench_line("pmc_write.json")["sampler_key"])
 tper = {}
 for k in sorted(f):
     if not k.startswith(("conv_", "final_", "sampler_", "attention", "init5", "lowres_", "gconv", "gnorm", "gstats")):
@@ -126,17 +129,17 @@ tcls = by_class(tper, "launches", ["hbm_read_bytes_per_launch", "hbm_write_bytes
 json.dump({"source": "DM_SPLIT=1 rocprofv3 --kernel-trace --pmc FETCH_SIZE / --pmc WRITE_SIZE (separate runs: tools/diag/r3_profiles.sh traffic) -- python3 "
                      "bench.py --steps 1 --warmup 0 --no-cpu-baseline --no-roofline --no-configs (DDIM-50, B=1024, fp32); FETCH_SIZE doubled "
                      "(gfx950 tallies 128-B requests as 64 B), KiB -> bytes; `classes`: launch-weighted per kernel class of bench.py",
-           "build_key": bench_line("pmc_fetch.json")["build_key"], "classes": tcls, "per_kernel": tper},
-          open(os.path.join(DST, "r3_traffic.json"), "w"), indent=1)
+           "sampler_key": bench_line("pmc_fetch.json")["sampler_key"], "classes": tcls, "per_kernel": tper},
+          open(os.path.join(DST, "sampler_traffic.json"), "w"), indent=1)
 for c, o in tcls.items():
     print(f"class {c:28s} {o['launches']:5d} launches  {o['hbm_read_bytes_per_launch']/1e6:8.1f} MB read {o['hbm_write_bytes_per_launch']/1e6:8.1f} MB written per launch")
 
 # ---- SQ counters per kernel (MFMA-busy share of SIMD cycles, vector instructions per MFMA)
 for tag in ("model", "cfg1", "cfg4"):
     d = f"pmc_sq_{tag}"
-    if tag == "cfg4" and not glob.glob(os.path.join(SRC, d + ".json")):
-        continue  # (optional pass: r3_profiles.sh sq4)
-    keys.add(bench_line(d + ".json")["build_key"])
+    if not glob.glob(os.path.join(SRC, d + ".json")):
+        continue  # (optional passes: r3_profiles.sh sq, sq4)
+    keys.add(bench_line(d + ".json")["sampler_key"])
     crow = list(csv.DictReader(open(one(d + "/*/*counter_collection.csv"))))
     trace = {r["Dispatch_Id"]: r for r in csv.DictReader(open(one(d + "/*/*kernel_trace.csv")))}
     disp = collections.defaultdict(dict)
@@ -171,9 +174,9 @@ for tag in ("model", "cfg1", "cfg4"):
     json.dump({"source": "DM_SPLIT=1 rocprofv3 --kernel-trace --pmc SQ_VALU_MFMA_BUSY_CYCLES SQ_VALU_MFMA_COEXEC_CYCLES SQ_INSTS_VALU SQ_INSTS_MFMA SQ_BUSY_CYCLES "
                          "SQ_WAVE_CYCLES GRBM_GUI_ACTIVE (tools/diag/r3_profiles.sh sq; one bench pass, " + cmd + "); all launches of a kernel summed; "
                          "busy fraction = SQ_VALU_MFMA_BUSY_CYCLES / (GRBM_GUI_ACTIVE / 8 x 1024 SIMDs)",
-               "build_key": bench_line(d + ".json")["build_key"], "per_kernel": res},
-              open(os.path.join(DST, f"r3_pmc_sq_{tag}.json"), "w"), indent=1)
+               "sampler_key": bench_line(d + ".json")["sampler_key"], "per_kernel": res},
+              open(os.path.join(DST, f"sampler_pmc_sq_{tag}.json"), "w"), indent=1)
 
 if len(keys) != 1:
     sys.exit("the passes ran on different builds: %s" % sorted(keys))
-print("build_key", keys.pop())
+print("sampler_key", keys.pop())
