@@ -73,7 +73,7 @@ _SIGS = {
                                    _sz, _vp]),
 }
 EXPORTS = tuple(_SIGS)
-ABI_VERSION = 6  # include/dm_sampler.h: DM_ABI_VERSION
+ABI_VERSION = 7  # include/dm_sampler.h: DM_ABI_VERSION
 CHUNK_FN = C.CFUNCTYPE(_vp, _vp, _i, _i)  # dm_chunk_fn
 
 

@@ -6,9 +6,10 @@
 // Three paths.  Up to TOKEN_ROWS rows, and fp32 up to SKINNY_ROWS, the weights' bandwidth bounds the block, and every wave streams weight rows
 // straight into vector (gemv_kernel) or matrix (skinny_kernel) instructions; above that the tiled products of dm_block_gemm.hip, whose
 // smallest tile and split k range serve 16-bit decode batches.
-// Rounding: h, u act'(g), act(g), dg and du are kept in the tensors' type between the products (but h of one or two rows in fp32: EXACT_ROWS).  The
-// matrix pipe takes h, dg and du in 16 bits and nothing wider; u act'(g) and act(g) are 16 bits for their bytes (32 would add 0.7 GB to a step of 8192 x 4096 x 11008, 3 % of
-// its time): a gradient has three roundings where results alone would have one, sqrt(3) of its error.  Every sum is fp32.
+// Rounding: the matrix pipe takes h, dg and du in 16 bits and nothing wider, so 16-bit tensors round them to their type between the products (but h of
+// one or two rows: EXACT_ROWS): a gradient has two roundings where results alone would have one, sqrt(2) of its error.  u act'(g) and act(g) are kept
+// in fp32, or rounded too where the caller asks for the fewer bytes (Saved; relative to 64 bits, bf16: 2.3e-3 and 2.9e-3 of a gradient).  Steps in us with
+// fp32 and 16 bits: 8192 x 4096 x 11008 bf16 5400 and 5280, 1999 x 1001 x 2731 bf16 242 and 235, 28000 x 288 x 992 bf16 472 and 421.  Every sum is fp32.
 // fp32 tensors are split into three bf16 terms and multiplied as six products (a1b1 a1b2 a2b1 a2b2 a1b3 a3b1; what is left out is below
 // 2^-25 of |a||b|): the fp32 matrix instructions have 1/16 of the bf16 ones' rate.
 #include <type_traits>
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const PackJobs jobs) {
 // elements of the weights' type (`kept`) or planes.
 template <typename T, typename X, typename O>
 struct Streamed {
-  const X* x; int64_t xs; const T *w, *w2; int64_t ldw; const T *bias, *bias2; O* out; int64_t ldo; T *ug, *ag, *kept; bf16* planes; int M, N, K, act;
+  const X* x; int64_t xs; const T *w, *w2; int64_t ldw; const T *bias, *bias2; O* out; int64_t ldo; void *ug, *ag; int kept16; T* kept; bf16* planes; int M, N, K, act;
 };
 using StreamedF32 = Streamed<float, float, float>;
 
@@ -95,7 +96,10 @@ __device__ __forceinline__ void finish_gate(const Streamed<T, X, O>& p, int n, i
   }
   p.out[at] = (O)h;
   if (p.kept) p.kept[at] = (T)h;
-  if (p.ug) { p.ug[at] = (T)u; p.ag[at] = (T)ag; }
+  if (p.ug) {
+    if (p.kept16) { ((T*)p.ug)[at] = (T)u; ((T*)p.ag)[at] = (T)ag; }
+    else { ((float*)p.ug)[at] = u; ((float*)p.ag)[at] = ag; }
+  }
   if (p.planes) {
     bf16 t[3];
     split3(h, t);
@@ -400,7 +404,7 @@ struct Carver {
 // A matrix as the products read it: rows of `ld` 16-bit elements; fp32 matrices as three planes.
 struct Operand { const void* p; int64_t ld, plane; };
 
-struct FfnSizes { int64_t M; int D, F, N, dtype; };
+struct FfnSizes { int64_t M; int D, F, N, dtype, kept16; };  // kept16: see Saved (fp32 tensors: 0)
 
 // fp32 backward passes by column_kernel: where splitting the weights into planes costs more than multiplying in vector instructions, so for
 // large weights and few rows.  Measured, backward pass in us with it and with tiles of planes, weights of ... elements each:
@@ -498,18 +502,19 @@ inline int64_t pad8(int64_t v) { return round_up(v, 8); }
 
 struct FfnIn { const void *x, *wg, *wu, *wd, *bg, *bu, *bd; int64_t xs; };
 
-// What the forward pass keeps for the backward pass: u act'(g), act(g), and h as an operand of dWd = dy^T h.
-template <typename T>
+// What the forward pass keeps for the backward pass: u act'(g) and act(g), fp32 or (kept16) of the tensors' type, and h as an operand of dWd = dy^T h.
 struct Saved {
-  T *ug = nullptr, *ag = nullptr;
+  void *ug = nullptr, *ag = nullptr;
   Operand h = {nullptr, 0, 0};
-  Saved(void* p, int64_t M, int F) {
+  int kept16;
+  Saved(void* p, int64_t M, int F, int kept16_) : kept16(kept16_) {
     if (!p) return;
-    const int64_t Fp = pad8(F);
-    ug = (T*)p;
-    ag = ug + M * Fp;
-    h = {ag + M * Fp, Fp, M * Fp};
+    const int64_t Fp = pad8(F), bytes = M * Fp * (kept16 ? 2 : 4);
+    ug = p;
+    ag = (char*)p + bytes;
+    h = {(char*)p + 2 * bytes, Fp, M * Fp};
   }
+  Out out(void* p) const { return {p, h.ld, 0, !kept16, 1}; }
 };
 
 // run: launch; otherwise only count the workspace.
@@ -517,7 +522,7 @@ template <typename T>
 int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int act, Carver& ws, bool run, hipStream_t st) {
   constexpr bool F32 = std::is_same<T, float>::value;
   const int64_t Fp = pad8(z.F);
-  const Saved<T> kept(saved, z.M, z.F);
+  const Saved kept(saved, z.M, z.F, z.kept16);
   if (z.M <= TOKEN_ROWS || (F32 && z.M <= SKINNY_ROWS && z.D >= 4 && z.F >= 4)) {
     const int M = (int)z.M;
     auto both = [&](auto type) {  // of h
@@ -525,9 +530,9 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
       H* h = (H*)ws.take((size_t)z.M * Fp * sizeof(H));
       if (!run) return 0;
       const Streamed<T, T, H> gate = {(const T*)in.x, in.xs, (const T*)in.wg, (const T*)in.wu, z.D, (const T*)in.bg, (const T*)in.bu, h, Fp,
-                                      kept.ug, kept.ag, saved && !F32 ? (T*)kept.h.p : nullptr, saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act};
+                                      kept.ug, kept.ag, kept.kept16, saved && !F32 ? (T*)kept.h.p : nullptr, saved && F32 ? (bf16*)kept.h.p : nullptr, M, z.F, z.D, act};
       if (const int rc = streamed<true>(gate, st)) return rc;
-      const Streamed<T, H, T> down = {h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, nullptr, nullptr,
+      const Streamed<T, H, T> down = {h, Fp, (const T*)in.wd, nullptr, z.F, (const T*)in.bd, nullptr, (T*)y, z.N, nullptr, nullptr, 0, nullptr, nullptr,
                                       M, z.N, z.F, act};
       return streamed<false>(down, st);
     };
@@ -550,8 +555,8 @@ int ffn_forward(const FfnSizes& z, const FfnIn& in, void* y, void* saved, int ac
   g.b2 = wu.p;
   g.M = z.M; g.N = z.F; g.K = z.D; g.iters = iters_of(g.K);
   g.out = between<T>(h);
-  g.out2 = result<T>(kept.ug, Fp);
-  g.out3 = result<T>(kept.ag, Fp);
+  g.out2 = kept.out(kept.ug);
+  g.out3 = kept.out(kept.ag);
   g.bias = in.bg; g.bias2 = in.bu; g.act = act;
   const int tile = planned(g, gate, part);
   if ((rc = gemm_launch<Mat<T>, false, false, F32 ? EPI_GATE_F32 : EPI_GATE>(g, tile, st))) return rc;
@@ -580,7 +585,7 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   }
   // dg and du side by side, so that one product gives both projections' gradients: twice the tiles of a launch, one launch less
   const Operand dg = take_operand<T>(z.M, 2 * (int)Fp, ws), du = {(char*)dg.p + 2 * Fp, dg.ld, dg.plane};
-  const Saved<T> kept(const_cast<void*>(saved), z.M, z.F);
+  const Saved kept(const_cast<void*>(saved), z.M, z.F, z.kept16);
   size_t part_bytes = gemm_plan(z.M, z.D, iters_of(z.F), terms * 2, 1, sizeof(T), true).part_bytes;
   const GemmPlan dact = gemm_plan(z.M, z.F, iters_of(z.N), terms, 1, terms > 1 ? 20 : 8, true);
   const size_t more[] = {dact.part_bytes, gemm_plan(2LL * z.F, z.D, iters_of(z.M), terms, 1, sizeof(T), false).part_bytes,
@@ -599,7 +604,7 @@ int ffn_backward(const FfnSizes& z, const FfnIn& in, const void* dy, int64_t dys
   add_terms<T>(a, y, wd);
   a.M = z.M; a.N = z.F; a.K = z.N; a.iters = iters_of(a.K);
   a.out = between<T>(dg); a.out2 = between<T>(du);
-  a.ug = kept.ug; a.ag = kept.ag; a.ldg = Fp;
+  a.ug = kept.ug; a.ag = kept.ag; a.ldg = Fp; a.kept16 = kept.kept16;
   const int tile = planned(a, dact, part);
   if constexpr (std::is_same<T, float>::value)
     if (few) {
@@ -699,13 +704,15 @@ int dm_debug_ffn_plan(int tile, int splits) {
 
 size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype) {
   using namespace dmb;
+  const bool keep = dtype & DM_FFN_KEEP_F32;
+  dtype &= ~DM_FFN_KEEP_F32;
   if (M <= 0 || F < 1 || !dtype_ok(dtype)) return 0;
-  return (size_t)M * pad8(F) * (dtype == DM_F32 ? 2 * 4 + 3 * 2 : 3 * 2);
+  return (size_t)M * pad8(F) * (dtype == DM_F32 ? 2 * 4 + 3 * 2 : keep ? 2 * 4 + 2 : 3 * 2);
 }
 
 size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype, int save) {
   using namespace dmb;
-  const FfnSizes z = {M, D, F, N, dtype};
+  const FfnSizes z = {M, D, F, N, dtype, 0};
   if (M <= 0 || ffn_check("dm_gated_ffn_workspace_bytes", z, DM_ACT_SILU)) return 0;
   Carver ws = {nullptr};
   ffn_types(dtype, [&](auto t) { return ffn_forward<decltype(t)>(z, FfnIn{}, nullptr, save ? &ws : nullptr, 0, ws, false, nullptr); });
@@ -714,7 +721,7 @@ size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype, i
 
 size_t dm_gated_ffn_backward_workspace_bytes(int64_t M, int D, int F, int N, int dtype) {
   using namespace dmb;
-  const FfnSizes z = {M, D, F, N, dtype};
+  const FfnSizes z = {M, D, F, N, dtype, 0};
   if (M <= 0 || ffn_check("dm_gated_ffn_backward_workspace_bytes", z, DM_ACT_SILU)) return 0;
   Carver ws = {nullptr};
   ffn_types(dtype, [&](auto t) {
@@ -728,7 +735,8 @@ int dm_gated_ffn(const void* x_dev, int64_t x_stride, const void* w_gate_dev, co
                  void* workspace_dev, size_t workspace_bytes, void* stream) {
   using namespace dmb;
   const char* who = "dm_gated_ffn";
-  const FfnSizes z = {M, D, F, N, dtype};
+  const FfnSizes z = {M, D, F, N, dtype, dtype != DM_F32 && !(activation & DM_FFN_KEEP_F32)};
+  activation &= ~DM_FFN_KEEP_F32;
   if (const int rc = ffn_check(who, z, activation)) return rc;
   if (M == 0) return 0;
   if (M == 1) x_stride = D;  // (rows of a product's second operand end where the stride says)
@@ -751,7 +759,8 @@ int dm_gated_ffn_backward(const void* dy_dev, int64_t dy_stride, const void* x_d
                           void* workspace_dev, size_t workspace_bytes, void* stream) {
   using namespace dmb;
   const char* who = "dm_gated_ffn_backward";
-  const FfnSizes z = {M, D, F, N, dtype};
+  const FfnSizes z = {M, D, F, N, dtype, dtype != DM_F32 && !(activation & DM_FFN_KEEP_F32)};
+  activation &= ~DM_FFN_KEEP_F32;
   if (const int rc = ffn_check(who, z, activation)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   if (M == 0) {  // no rows: the parameters' gradients are zero

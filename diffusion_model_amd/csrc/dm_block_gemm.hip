@@ -193,11 +193,12 @@ struct GemmArgs {
   int64_t M;
   int N, K;                           // N: of one projection for EPI_GATE.  K: true length; a KC row is zero from there to the end of its piece
   int tiles_m, tiles_n, splits;
-  Out out, out2, out3;                // STORE: out (out2: see `pair`).  GATE: out = h, and for the backward pass (null: not kept) out2 = u act'(g), out3 = act(g).
+  Out out, out2, out3;                // STORE: out (out2: see `pair`).  GATE: out = h, and for the backward pass (null: not kept) out2 = u act'(g), out3 = act(g), fp32 or not.
                                       // DACT: out = dg, out2 = du
   const void *bias, *bias2;           // of the result's type; GATE: of the operands'
-  const void *ug, *ag;                // DACT: u act'(g) and act(g), rows of ldg
+  const void *ug, *ag;                // DACT: u act'(g) and act(g), rows of ldg, fp32 or (kept16) of the operands' type
   int64_t ldg;
+  int kept16;
   int act;
   void* part;                         // splits > 1: fp32 partial products (GATE: of both projections in turn), rows of ldpart,
   int64_t split_stride, ldpart;       // split_stride elements from one to the next; joined by a second launch
@@ -207,6 +208,19 @@ struct GemmArgs {
   int64_t pair;                       // STORE with both operands KS: 0, or two products of one B in one launch: the second A lies `pair` bytes
   void* sums2;                        // behind the first, its result in out2.p, its sums in sums2; their partial rows follow the first's
 };
+
+// What GATE keeps for DACT, eight columns of a row
+template <typename T, bool F32>
+__device__ __forceinline__ void store_kept(const GemmArgs& p, int64_t m, int n, int np, const float (&ug)[8], const float (&ag)[8]) {
+  if (!p.out2.p) return;
+  if (F32 || p.out2.f32) {
+    store8<T, OUT_F32>(p.out2, m, n, np, ug);
+    store8<T, OUT_F32>(p.out3, m, n, np, ag);
+  } else {
+    store8<T, OUT_16>(p.out2, m, n, np, ug);
+    store8<T, OUT_16>(p.out3, m, n, np, ag);
+  }
+}
 
 // Where a stage keeps a piece of 16 bytes.  KS (one LDS row per k, R columns): piece c of row k lies at c ^ ks_key(k), so that the 32
 // lanes of two fragment reads (k .. k + 3 and k + 8 .. k + 11, two pieces each) find 16 pieces of all 64 banks.  KC (one LDS row per
@@ -303,8 +317,8 @@ gemm_kernel(const GemmArgs p) {
   constexpr int ABYTES = BM * GEMM_BK * 2, STAGE = (BM + BN) * GEMM_BK * 2;
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32,
                  DACT = EPI == EPI_DACT || EPI == EPI_DACT_F32, SUMS = AKS && BKS;
-  using Kept = typename std::conditional<F32, float, T>::type;  // what GATE keeps for DACT
-  constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
+  using Bias = typename std::conditional<F32, float, T>::type;
+  constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16;
   constexpr int XS = MI >= WN ? MI / WN : 1;  // the waves of a tile row share its sums of A: XS blocks of 16 rows each
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
@@ -551,8 +565,8 @@ gemm_kernel(const GemmArgs p) {
     const int n = n0 + threadIdx.x % PIECES * 8;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      b1[e] = EPI == EPI_STORE && p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<Kept>(p.bias, n + e, p.N);
-      b2[e] = GATE ? bias_at<Kept>(p.bias2, n + e, p.N) : 0.f;
+      b1[e] = EPI == EPI_STORE && p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<Bias>(p.bias, n + e, p.N);
+      b2[e] = GATE ? bias_at<Bias>(p.bias2, n + e, p.N) : 0.f;
     }
   }
 #pragma unroll
@@ -563,16 +577,23 @@ gemm_kernel(const GemmArgs p) {
 #pragma unroll
       for (int j = 0; j < NI; ++j)
         *(DM_LDS f32x4*)(buf + (wm * 32 + h * 16 + (lane & 15)) * PITCH + ((wn * NI + j) * 16 + (lane >> 4) * 4) * 4) = acc[i * 2 + h][j];
-    Vec<Kept, 8> ug[DACT ? TASKS : 1], ag[DACT ? TASKS : 1];  // asked for ahead of the barrier
+    f32x4 ug[DACT ? TASKS : 1][2], ag[DACT ? TASKS : 1][2];  // asked for ahead of the barrier (16 bits: the first of two, converted behind it)
     if constexpr (DACT) {
+      auto ask = [&](auto type) __attribute__((always_inline)) {
+        using S = decltype(type);
 #pragma unroll
-      for (int t = 0; t < TASKS; ++t) {
-        const int id = t * NW * 64 + threadIdx.x, row = id / PIECES, n = n0 + id % PIECES * 8;
-        const int64_t m = m0 + row / 32 * (MI * 16) + i * 32 + row % 32;
-        if (m >= p.M || n >= np || p.splits > 1) continue;
-        ug[t] = *reinterpret_cast<const Vec<Kept, 8>*>((const Kept*)p.ug + m * p.ldg + n);
-        ag[t] = *reinterpret_cast<const Vec<Kept, 8>*>((const Kept*)p.ag + m * p.ldg + n);
-      }
+        for (int t = 0; t < TASKS; ++t) {
+          const int id = t * NW * 64 + threadIdx.x, row = id / PIECES, n = n0 + id % PIECES * 8;
+          const int64_t m = m0 + row / 32 * (MI * 16) + i * 32 + row % 32;
+          if (m >= p.M || n >= np || p.splits > 1) continue;
+          const S *a = (const S*)p.ug + m * p.ldg + n, *b = (const S*)p.ag + m * p.ldg + n;
+          ug[t][0] = *(const f32x4*)a;
+          ag[t][0] = *(const f32x4*)b;
+          if (sizeof(S) == 4) { ug[t][1] = *(const f32x4*)(a + 4); ag[t][1] = *(const f32x4*)(b + 4); }
+        }
+      };
+      if (!F32 && p.kept16) ask(T());
+      else ask(float());
     }
     lds_barrier();
     if (EPI == EPI_STORE && p.splits == 1 && !p.out.vec) {  // rows off 16-byte boundaries: neighbouring lanes store neighbouring elements
@@ -609,10 +630,17 @@ gemm_kernel(const GemmArgs p) {
         gate_values<!F32>(p.act, v, u, h);
         if (ragged) zero_behind(n, p.N, h), zero_behind(n, p.N, u), zero_behind(n, p.N, v);
         store8<T, BETWEEN>(p.out, m, n, np, h);
-        if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
+        store_kept<T, F32>(p, m, n, np, u, v);
       } else if constexpr (DACT) {
+        if (!F32 && p.kept16) {
+          using T8 = typename std::conditional<std::is_same<T, bf16>::value, bf16x8, f16x8>::type;
+          const T8 a = __builtin_bit_cast(T8, ug[t][0]), b = __builtin_bit_cast(T8, ag[t][0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { u[e] = v[e] * (float)ug[t].v[e]; h[e] = v[e] * (float)ag[t].v[e]; }
+          for (int e = 0; e < 8; ++e) { u[e] = v[e] * (float)a[e]; h[e] = v[e] * (float)b[e]; }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { u[e] = v[e] * ug[t][e / 4][e % 4]; h[e] = v[e] * ag[t][e / 4][e % 4]; }
+        }
         if (ragged) zero_behind(n, p.N, u), zero_behind(n, p.N, h);
         store8<T, BETWEEN>(p.out, m, n, np, u);
         store8<T, BETWEEN>(p.out2, m, n, np, h);
@@ -671,8 +699,8 @@ __device__ __forceinline__ bool join8(const float* part, int splits, int64_t str
 template <typename T, int EPI>
 __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
   constexpr bool GATE = EPI == EPI_GATE || EPI == EPI_GATE_F32, F32 = EPI == EPI_GATE_F32 || EPI == EPI_DACT_F32;
-  using Kept = typename std::conditional<F32, float, T>::type;
-  constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16, KEPT = F32 ? OUT_F32 : OUT_16;
+  using Bias = typename std::conditional<F32, float, T>::type;
+  constexpr int BETWEEN = F32 ? OUT_PLANES : OUT_16;
   const int np = (p.N + 7) & ~7, pieces = np / 8;
   const int64_t rows = EPI == EPI_STORE && p.pair ? 2 * p.M : p.M, all = rows * pieces;
   const bool grouped = p.splits > 4;
@@ -687,11 +715,11 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
     if (!mine) continue;
     if constexpr (GATE) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { v[e] += bias_at<Kept>(p.bias, n + e, p.N); u[e] += bias_at<Kept>(p.bias2, n + e, p.N); }
+      for (int e = 0; e < 8; ++e) { v[e] += bias_at<Bias>(p.bias, n + e, p.N); u[e] += bias_at<Bias>(p.bias2, n + e, p.N); }
       gate_values<!F32>(p.act, v, u, h);
       zero_behind(n, p.N, h), zero_behind(n, p.N, u), zero_behind(n, p.N, v);
       store8<T, BETWEEN>(p.out, m, n, np, h);
-      if (p.out2.p) { store8<T, KEPT>(p.out2, m, n, np, u); store8<T, KEPT>(p.out3, m, n, np, v); }
+      store_kept<T, F32>(p, m, n, np, u, v);
     } else if constexpr (EPI == EPI_STORE) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += p.out.f32 ? bias_at<float>(p.bias, n + e, p.N) : bias_at<T>(p.bias, n + e, p.N);
@@ -701,8 +729,13 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs p) {
       else store8<T, OUT_16>(o, m >= p.M ? m - p.M : m, n, p.N, v);
     } else {
       float ag[8];
-      load8((const Kept*)p.ug + m * p.ldg + n, u);
-      load8((const Kept*)p.ag + m * p.ldg + n, ag);
+      if (!F32 && p.kept16) {
+        load8((const T*)p.ug + m * p.ldg + n, u);
+        load8((const T*)p.ag + m * p.ldg + n, ag);
+      } else {
+        load8((const float*)p.ug + m * p.ldg + n, u);
+        load8((const float*)p.ag + m * p.ldg + n, ag);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) { u[e] *= v[e]; h[e] = ag[e] * v[e]; }
       zero_behind(n, p.N, u), zero_behind(n, p.N, h);

@@ -15,6 +15,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _POSITIONS = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
+_KEEP_F32 = 256  # DM_FFN_KEEP_F32
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
 
 
@@ -286,19 +287,23 @@ def _ffn_check(x, w_gate, w_up, w_down, activation):
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation="silu", save=False):
     """(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down, with weights as nn.Linear holds them: w_gate and w_up
     [hidden, width], w_down [out, hidden].  All tensors are of one type.  ``activation``: silu, gelu (erf), gelu_tanh, relu, sigmoid.
-    ``save``: (y, saved), with ``saved`` (opaque) for ``gated_ffn_backward``.  16-bit types round the hidden values to that type
-    between the matrix products; fp32 keeps fp32 accuracy (an infinite
-    operand may give NaN where fp32 would give an infinity)."""
+    ``save``: (y, saved), with ``saved`` (opaque) for ``gated_ffn_backward``.  16-bit types round the hidden values (forward, but of one
+    or two rows) and their gradients to that type between the matrix products, in half to infinity from 65520 on; what else ``saved`` keeps of them is
+    fp32 (10 bytes per hidden value), or with ``save="compact"`` of their type too (6 bytes, gradients less exact by a quarter).  fp32 keeps fp32
+    accuracy (an infinite operand may give NaN where fp32 would give an infinity)."""
+    if save not in (False, True, "compact"):
+        raise ValueError(f"save must be False, True or 'compact' (got {save!r})")
     dt, d, f, n, w_gate, w_up, w_down = _ffn_check(x, w_gate, w_up, w_down, activation)
     b_gate, b_up, b_down = _vector(b_gate, f, x, "b_gate"), _vector(b_up, f, x, "b_up"), _vector(b_down, n, x, "b_down")
     L = _lib.lib()
     r, stride, m = _rows(x)
     y = _empty_like(x) if n == d else torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt), dtype=torch.uint8, device=x.device) if save else None
-    nbytes = L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt, save)
+    keep = _KEEP_F32 if save is True else 0
+    saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt | keep), dtype=torch.uint8, device=x.device) if save else None
+    nbytes = L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt, bool(save))
     ws = _workspace(x, nbytes)
     _call(x, L.dm_gated_ffn, r.data_ptr(), stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _ptr(b_gate), _ptr(b_up), _ptr(b_down),
-          y.data_ptr(), _ptr(saved), m, d, f, n, _ACTIVATIONS[activation], dt, ws.data_ptr(), nbytes)
+          y.data_ptr(), _ptr(saved), m, d, f, n, _ACTIVATIONS[activation] | keep, dt, ws.data_ptr(), nbytes)
     return (y, saved) if save else y
 
 
@@ -312,8 +317,11 @@ def gated_ffn_backward(grad, x, w_gate, w_up, w_down, saved, activation="silu", 
     L = _lib.lib()
     r, stride, m = _rows(x)
     g, gstride, _ = _rows(grad)
+    keep = _KEEP_F32  # by its size
+    if torch.is_tensor(saved) and saved.numel() == L.dm_gated_ffn_saved_bytes(m, f, dt):
+        keep = 0
     if not torch.is_tensor(saved) or saved.device != x.device or saved.dtype != torch.uint8 or not saved.is_contiguous() or \
-            saved.numel() != L.dm_gated_ffn_saved_bytes(m, f, dt):
+            saved.numel() != L.dm_gated_ffn_saved_bytes(m, f, dt | keep):
         raise RuntimeError("saved must be what gated_ffn(..., save=True) returned for this input")
     dx = _empty_like(x)
     dws = [torch.empty_like(w) for w in (w_gate, w_up, w_down)]
@@ -321,5 +329,5 @@ def gated_ffn_backward(grad, x, w_gate, w_up, w_down, saved, activation="silu", 
     nbytes = L.dm_gated_ffn_backward_workspace_bytes(m, d, f, n, dt)
     ws = _workspace(x, nbytes)
     _call(x, L.dm_gated_ffn_backward, g.data_ptr(), gstride, r.data_ptr(), stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-          saved.data_ptr(), dx.data_ptr(), *(_ptr(t) for t in dws + dbs), m, d, f, n, _ACTIVATIONS[activation], dt, ws.data_ptr(), nbytes)
+          saved.data_ptr(), dx.data_ptr(), *(_ptr(t) for t in dws + dbs), m, d, f, n, _ACTIVATIONS[activation] | keep, dt, ws.data_ptr(), nbytes)
     return (dx, *dws, *dbs)

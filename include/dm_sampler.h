@@ -43,8 +43,8 @@ const char* dm_last_error(void);
  * 4: dm_sample's workspace holds one carve per parallel sub-batch chain (dm_sample_workspace_bytes grew for large batches),
  *    dm_sample_branches, dm_stream_create / dm_stream_destroy;
  * 5: the transformer-block operators dm_layer_norm*, dm_rotary, dm_gated_ffn*; nothing of version 4 changed;
- * 6: dm_debug_ffn_plan; nothing of version 5 changed). */
-#define DM_ABI_VERSION 6
+ * 6: dm_debug_ffn_plan; nothing of version 5 changed; 7: DM_FFN_KEEP_F32; nothing of version 6 changed). */
+#define DM_ABI_VERSION 7
 int dm_version(void);
 /* sha256 over the compiler flags and sources this library was built from (__graft_entry__.build_key); "unkeyed" for a
  * hand build.  build() compiles every time it is called; tests compare this with the tree they run in, so that no library of
@@ -312,6 +312,7 @@ int dm_conv2d(int kind, const float* x1_dev, int c1, const float* x2_dev, int c2
  * contiguous and overlap no input unless said otherwise.  The same call gives the same bits every time. */
 enum { DM_F32 = 0, DM_BF16 = 1, DM_F16 = 2 };
 enum { DM_ACT_SILU = 0, DM_ACT_GELU = 1 /* erf */, DM_ACT_GELU_TANH = 2, DM_ACT_RELU = 3, DM_ACT_SIGMOID = 4 };
+enum { DM_FFN_KEEP_F32 = 256 }; /* with an activation or a dtype of dm_gated_ffn*: see there */
 
 /* y[m,:] = (x[m,:] - mean) rstd weight + bias over rows of C elements, rstd = 1/sqrt(var + eps), var the biased variance.
  * x rows are x_stride elements apart, at any element boundary.  weight, bias: [C] of x's type or fp32 (param_dtype), either may be NULL.
@@ -344,9 +345,11 @@ int dm_rotary(const dm_rotary_tensor* q, const dm_rotary_tensor* k, const int64_
 
 /* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down: x [M][D] rows x_stride apart, w_gate and w_up [F][D],
  * w_down [N][F], y [M][N], biases [F], [F], [N] or NULL, all of one type.  saved_dev: NULL, or dm_gated_ffn_saved_bytes for the
- * backward pass.  Between its products the block keeps the tensors' type: 16-bit types round h, and for the backward pass
- * u act'(g), act(g), dg and du, there.  fp32 operands are multiplied as three bf16 terms each, but for forward passes of few rows
- * (an infinite operand gives NaN there, where fp32 would give an infinity).
+ * backward pass.  16-bit types round h (but of one or two rows, forward), dg and du to their type between the products, and for the backward
+ * pass u act'(g) and act(g) too, unless `activation` holds DM_FFN_KEEP_F32 beside the activation's number in both calls, and `dtype` in
+ * dm_gated_ffn_saved_bytes: then these are kept in fp32, 10 bytes per hidden value instead of 6 (gradients: 1.4 times the error of one rounding
+ * instead of 1.7).  Of half tensors every value that is rounded has to stay below 65520, or it becomes infinite.  fp32 operands are
+ * multiplied as three bf16 terms each, but for passes of few rows (an infinite operand gives NaN there, where fp32 would give an infinity).
  * Rows of whole 16-byte pieces must start at multiples of 16 bytes. */
 size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype);
 size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype, int save); /* save: with saved_dev */

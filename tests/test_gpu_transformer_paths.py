@@ -199,7 +199,7 @@ def test_one_row_has_any_stride(dtype):
     g = torch.Generator().manual_seed(2)
     x, dy, w, _ = ffn_case(g, 1, 64, 136, 72, dt, False)
     xd, dyd, wd = x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w]
-    y, saved = d.gated_ffn(xd, *wd, save=True)
+    y, saved = d.gated_ffn(xd, *wd, save="compact")  # (what the entry points take without DM_FFN_KEEP_F32)
     want = d.gated_ffn_backward(dyd, xd, *wd, saved, bias=True)
     L = _lib.lib()
     nbytes = L.dm_gated_ffn_backward_workspace_bytes(1, 64, 136, 72, code)
@@ -351,3 +351,46 @@ def test_few_fp32_rows_of_large_weights(rows):
     got = step(x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b], "silu")
     for (name, want, tol), t in zip(ffn_bounds(x, dy, w, b, "silu", torch.float32), got):
         close(t, want, tol, f"{name} {rows}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,splits", [(1, 1), (4, 1), (70, 1), (70, 3), (300, 1)])
+@pytest.mark.parametrize("size", [(40, 136, 72), (33, 131, 70)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_the_hidden_values_round_once(size, rows, splits, dtype):
+    """The biases' gradients where one row alone has a gradient are its dg and du: fp32 values rounded once.  The compact form rounds
+    u act'(g) and act(g) as well: twice."""
+    dt = DTYPES[dtype]
+    dd, f, n = size
+    g = torch.Generator().manual_seed(rows + f)
+    x, dy, w, b = ffn_case(g, rows, dd, f, n, dt, True)
+    dy = dy * (torch.arange(rows)[:, None] == rows // 2)
+    res, exact, _ = ffn_oracle(x, dy, w, b, "silu")
+    e = 2.0 ** -24 * (32 + max(dd, f, n) / 8)
+    xd, dyd, w, b = x.to(DEV), dy.to(DEV), [t.to(DEV) for t in w], [t.to(DEV) for t in b]
+    for tile in TILES:
+        with plan(tile, splits):
+            for save, roundings in ((True, 1), ("compact", 2)):
+                y, saved = d.gated_ffn(xd, *w, *b, save=save)
+                got = dict(zip(NAMES[1:], d.gated_ffn_backward(dyd, xd, *w, saved, bias=True)))
+                for name in ("db_gate", "db_up"):
+                    tol = roundings * 1.004 * HALF[dt] * res[name].abs() + e * exact[name] + (2.0 ** -24 if dt == torch.float16 else 0)
+                    close(got[name], res[name], tol, f"{name} {save} {tile}")
+                assert torch.equal(y, d.gated_ffn(xd, *w, *b))
+
+
+def test_what_a_forward_pass_keeps():
+    x, w, wd = torch.ones(6, 16, dtype=torch.bfloat16, device=DEV), torch.ones(24, 16, dtype=torch.bfloat16, device=DEV), torch.ones(8, 24, dtype=torch.bfloat16, device=DEV)
+    full, compact = d.gated_ffn(x, w, w, wd, save=True)[1], d.gated_ffn(x, w, w, wd, save="compact")[1]
+    assert full.numel() == 6 * 24 * 10 and compact.numel() == 6 * 24 * 6
+    with pytest.raises(ValueError, match="save"):
+        d.gated_ffn(x, w, w, wd, save="small")
+    with pytest.raises(RuntimeError, match="saved"):
+        d.gated_ffn_backward(torch.ones_like(x[:, :8]), x, w, w, wd, full[:-1])
+    # hidden gradients of half whose slope alone is beyond the type: fp32 keeps it
+    h = lambda *s: torch.full(s, 1.0, dtype=torch.float16, device=DEV)  # noqa: E731
+    x, wg, wu, wd, dy = h(80, 8), h(8, 8) * 2.0 ** -13, h(8, 8) * 2.0 ** 14, h(8, 8) * 2.0 ** -10, h(80, 8) * 2.0 ** -3
+    y, saved = d.gated_ffn(x, wg, wu, wd, activation="relu", save=True)  # g = 2^-10, u = 2^17, h = 2^7, dh = 2^-10, dg = 2^7, du = 2^-20
+    dx, dwg, dwu, dwd = d.gated_ffn_backward(dy, x, wg, wu, wd, saved, activation="relu")[:4]
+    assert (y == 1).all() and (dwg == 80 * 2.0 ** 7).all() and (dwd == 80 * 2.0 ** 4).all() and (dwu - 80 * 2.0 ** -20).abs().max() <= 2.0 ** -25
+    want = 2.0 ** -3 + 2.0 ** -3  # 8 x dg 2^-13 + 8 x du 2^14
+    assert (dx.double() - want).abs().max() <= 2.0 ** -11 * want
