@@ -298,7 +298,7 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, acti
     L = _lib.lib()
     r, stride, m = _rows(x)
     y = _empty_like(x) if n == d else torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    keep = _KEEP_F32 if save is True else 0
+    keep = _KEEP_F32 if save and save != "compact" else 0
     saved = torch.empty(L.dm_gated_ffn_saved_bytes(m, f, dt | keep), dtype=torch.uint8, device=x.device) if save else None
     nbytes = L.dm_gated_ffn_workspace_bytes(m, d, f, n, dt, bool(save))
     ws = _workspace(x, nbytes)

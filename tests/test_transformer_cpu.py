@@ -167,3 +167,18 @@ def test_yarn_blends_every_pair_that_turns_more_than_once(dim, base, length, fac
         assert abs(yarn[i].item() - want) <= 4e-16 * want, (i, turns[i].item())
         if turns[i] > 1:
             assert yarn[i] > inv[i] / factor * (1 + 1e-12), i
+
+
+def test_gated_ffn_forms_of_what_is_kept_and_plans():
+    L = _lib.lib()
+    keep = 256  # DM_FFN_KEEP_F32
+    for dtype, plain, kept in ((0, 14, 14), (1, 6, 10), (2, 6, 10)):
+        assert L.dm_gated_ffn_saved_bytes(7, 33, dtype) == 7 * 40 * plain and L.dm_gated_ffn_saved_bytes(7, 33, dtype | keep) == 7 * 40 * kept
+    assert L.dm_gated_ffn_saved_bytes(7, 33, 3 | keep) == 0
+    need = L.dm_gated_ffn_workspace_bytes(100, 64, 128, 64, 1, 1)
+    for act in (5 | keep, -1, 512):
+        refused(L.dm_gated_ffn(P, 64, P, P, P, None, None, None, P, P, 100, 64, 128, 64, act, 1, P, need, None), "activation")
+    for tile, splits in ((4, 1), (-2, 1), (0, 0), (0, 65)):
+        refused(L.dm_debug_ffn_plan(tile, splits), "plan")
+    assert L.dm_debug_ffn_plan(0, 4) == 0 and L.dm_gated_ffn_workspace_bytes(100, 4096, 128, 64, 1, 0) > need and L.dm_debug_ffn_plan(-1, 1) == 0
+    assert L.dm_gated_ffn_workspace_bytes(100, 64, 128, 64, 1, 1) == need
