@@ -3,9 +3,10 @@
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h, biases: column sums.
 // Both projections, the activation and the product are one kernel; so are dh, dg and du: for training the forward pass keeps u act'(g),
 // act(g) and h, three values where g and u would be two, so that none is rounded twice and nothing is computed again.
-// Three paths.  Up to TOKEN_ROWS rows, and fp32 up to SKINNY_ROWS, the weights' bandwidth bounds the block, and every wave streams weight rows
+// Three paths forward.  Up to TOKEN_ROWS rows, and fp32 up to SKINNY_ROWS, the weights' bandwidth bounds the block, and every wave streams weight rows
 // straight into vector (gemv_kernel) or matrix (skinny_kernel) instructions; above that the tiled products of dm_block_gemm.hip, whose
-// smallest tile and split k range serve 16-bit decode batches.
+// smallest tile and split k range serve 16-bit decode batches.  Backward, dh and dx of few fp32 rows by large weights are sums over the weights as they
+// lie (column_kernel, columns_fit), in plain fp32; everything else the tiled products.
 // Rounding: the matrix pipe takes h, dg and du in 16 bits and nothing wider, so 16-bit tensors round them to their type between the products (but h of
 // one or two rows: EXACT_ROWS): a gradient has two roundings where results alone would have one, sqrt(2) of its error.  u act'(g) and act(g) are kept
 // in fp32, or rounded too where the caller asks for the fewer bytes (Saved; relative to 64 bits, bf16: 2.3e-3 and 2.9e-3 of a gradient).  Steps in us with
@@ -107,8 +108,9 @@ __device__ __forceinline__ void finish_gate(const Streamed<T, X, O>& p, int n, i
   }
 }
 
-// ---- up to TOKEN_ROWS rows: the weights' bandwidth (one token through 4096 x 11008 bf16: 47 us, 5.8 TB/s of 270 MB; fp32 99 us).  A wave takes R rows of w (and of w2) and multiplies them with all of x in vector
-// instructions, a row's piece of 64 V elements per load; the KSPLIT waves that share rows split the k range and meet in LDS.
+// ---- up to TOKEN_ROWS rows: the weights' bandwidth (one token through 4096 x 11008 bf16: 47 us, 5.7 TB/s of 270 MB; fp32 99 us).  A wave takes R rows
+// of w (and of w2) and multiplies them with all of x in vector instructions, a row's piece of 64 V elements per load; the KSPLIT waves that share rows split
+// the k range and meet in LDS.
 template <int NV>  // v[i] summed over the wave; lane l < NV gets the i = l-th sum
 __device__ __forceinline__ float wave_sums(float (&v)[NV], int lane) {
   int n = NV;
@@ -209,8 +211,9 @@ int gemv_launch(const Streamed<T, X, O>& a, hipStream_t st) {
   return launched("dm_gated_ffn");
 }
 
-// ---- fp32, up to SKINNY_ROWS rows (of 4 elements or more): 16 rows of 2048 x 5504 52 us (2.6 TB/s of 135 MB), 64 rows 112 us.  Tiles of
-// split operands would first write three planes of every weight.
+// ---- fp32, up to SKINNY_ROWS rows (of 4 elements or more): 16 rows of 2048 x 5504 52 us (2.6 TB/s of 135 MB), 64 rows 113 us.  Tiles of split operands,
+// which first write three planes of every weight, take 132 and 144 (256 x 1024: 16 and 30 of 16 rows, 22 and 32 of 64; 4096 x 11008: 132 and 516,
+// 288 and 542).
 // Four instructions of four k each: instruction i takes element i of every lane's piece, on both sides.
 __device__ __forceinline__ f32x4 mfma_f32(const Piece<float, 4>& a, const Piece<float, 4>& b, f32x4 c) {
 #pragma unroll
@@ -407,7 +410,7 @@ struct Operand { const void* p; int64_t ld, plane; };
 struct FfnSizes { int64_t M; int D, F, N, dtype, kept16; };  // kept16: see Saved (fp32 tensors: 0)
 
 // fp32 backward passes by column_kernel: where splitting the weights into planes costs more than multiplying in vector instructions, so for
-// large weights and few rows.  Measured, backward pass in us with it and with tiles of planes, weights of ... elements each:
+// large weights and few rows.  Measured, backward pass in us with it and with tiles of planes, by the elements of a weight:
 // 1M (512 x 2048) 62 and 55 of one row; 4.4M (1918 x 2281) 104 and 114 of one, 123 and 116 of 16; 7.6M (1456 x 5223) 112 and 154 of one, 163 and 162
 // of 32; 11M (2048 x 5504) 184 and 208 of 17, 223 and 215 of 48; 45M (4096 x 11008) 416 and 742 of one, 605 and 777 of 48, 822 and 791 of 64.
 inline bool columns_fit(const FfnSizes& z) {

@@ -13,9 +13,10 @@
 // A bias' gradient, the sum of A over k, is one more product with ones from the same fragments.
 //
 // Bound by the matrix pipe and what is issued beside it: a SIMD's time is nearly the sum of its waves' products and other instructions, so
-// everything else in a step is kept short and lies between the products.  Measured, bf16, 8192 rows of width 4096, hidden 11008: both
-// projections with their gate 1.18 ms (1.25 PFLOP/s), down 0.55 ms (1.35), dh with dg and du 0.76 ms, dx 1.12 ms (1.32), a weight's gradient
-// 0.63 ms (1.18; 688 tiles in three rounds of 256 CUs); the library's products of these shapes reach 1.03 to 1.60.
+// everything else in a step is kept short and lies between the products.  Measured, bf16, 8192 rows of width 4096, hidden 11008, a training step: both
+// projections with their gate 1.28 ms (1.15 PFLOP/s, with 0.9 GB of what is kept), down 0.55 ms (1.34), dh with dg and du 0.79 ms, dx 1.09 ms (1.36),
+// both projections' gradients in one launch 1.29 ms (1.15; 1376 tiles in six rounds of 256 CUs), the third weight's 0.64 ms (1.16; 688 in three); the
+// library's products of these shapes reach 1.03 to 1.60.
 #ifndef DM_BLOCK_GEMM_HIP
 #define DM_BLOCK_GEMM_HIP
 #include <atomic>
@@ -360,7 +361,7 @@ gemm_kernel(const GemmArgs p) {
   // A term takes a group of steps, then the next term takes the same group (the last step, if it has fewer k, is one by itself).  The
   // `early` terms, of split fp32 the small ones, go through the whole range first: an instruction's sum is as exact as the largest of what it adds,
   // so small terms that met the main one's sum would lose as much in each instruction as the main term does (step of 65536 x 256 x 1024, relative
-  // to 64 bits: 0.7 to 2.4e-6 so and 1.6 to 3.4e-7 this way; 2180 and 2215 us, as the main term's planes are fetched once more).
+  // to 64 bits: 0.4 to 2.4e-6 so and 1.6 to 3.4e-7 this way; 2180 and 2205 us, as the main term's planes are fetched once more).
   const int group = p.segments > 1 ? AKS && p.splits > 1 ? 1 : 4 : p.iters;
   auto group_end = [&](int from) __attribute__((always_inline)) { return from >= whole ? step1 : from + group < whole ? from + group : whole; };
   int seg = 0, step = step0, group0 = step0, group1 = group_end(step0);  // of the next stage to be asked for

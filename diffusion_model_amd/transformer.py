@@ -219,7 +219,7 @@ def apply_rotary(q, k, inv_freq, positions=None, layout="half", scale=1.0, inver
     """Turns the pairs of every head of ``q`` [B, T, heads, head_dim] and ``k`` (the same with its own heads, or None) by
     position * inv_freq; returns (q, k).  ``inv_freq`` (float64 [rotary_dim / 2], on the GPU) says how much of the head turns;
     the rest is copied.  ``positions``: integers [T], [B, T], or [axes, B, T] (pair i takes axis i // (pairs / axes)), None for
-    0..T-1; angles are formed in 64 bits.  ``layout``: "half" pairs element i with i + rotary_dim/2, "interleaved" 2i with 2i + 1.
+    0..T-1; angles are formed in 64 bits (off by 2^-51 of themselves).  ``layout``: "half" pairs element i with i + rotary_dim/2, "interleaved" 2i with 2i + 1.
     ``inverse`` turns back: applied to gradients it is the backward pass.  ``inplace`` writes into q and k
     themselves, which must share no elements then."""
     dt = _dtype(q, "q")

@@ -315,7 +315,7 @@ enum { DM_ACT_SILU = 0, DM_ACT_GELU = 1 /* erf */, DM_ACT_GELU_TANH = 2, DM_ACT_
 enum { DM_FFN_KEEP_F32 = 256 }; /* with an activation or a dtype of dm_gated_ffn*: see there */
 
 /* y[m,:] = (x[m,:] - mean) rstd weight + bias over rows of C elements, rstd = 1/sqrt(var + eps), var the biased variance.
- * x rows are x_stride elements apart, at any element boundary.  weight, bias: [C] of x's type or fp32 (param_dtype), either may be NULL.
+ * x rows are x_stride elements apart (of one row any, here and below), at any element boundary.  weight, bias: [C] of x's type or fp32 (param_dtype), either may be NULL.
  * mean_dev, rstd_dev: [M] fp32 for the backward pass, or NULL.  M == 0 does nothing. */
 int dm_layer_norm(const void* x_dev, int64_t x_stride, const void* weight_dev, const void* bias_dev, int param_dtype,
                   void* y_dev, float* mean_dev, float* rstd_dev, int64_t M, int C, float eps, int dtype, void* stream);
@@ -328,7 +328,7 @@ int dm_layer_norm_backward(const void* dy_dev, int64_t dy_stride, const void* x_
                            void* stream);
 
 /* Rotary positions on [B][T][heads][head_dim] tensors (query, and key or NULL) with any strides, head elements contiguous.
- * Pair i of rotary_dim / 2 turns by position * inv_freq[i] (64-bit angles; exact for positions below 2^53), its two values
+ * Pair i of rotary_dim / 2 turns by position * inv_freq[i] (64-bit angles, off by 2^-51 of themselves; positions below 2^53), its two values
  * scaled by `scale`: elements (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`.  Elements from rotary_dim on are
  * copied.  positions int64 with strides (axis, image, token) in elements, or NULL for 0 .. T-1; with `axes` > 1 pair i takes
  * the axis i / (pairs / axes).  `inverse` turns back: the gradient of the forward call.  out == in (same strides) works in
@@ -343,13 +343,14 @@ int dm_rotary(const dm_rotary_tensor* q, const dm_rotary_tensor* k, const int64_
               const int64_t* position_strides, int axes, const double* inv_freq_dev, int64_t B, int64_t T, int head_dim,
               int rotary_dim, int interleaved, float scale, int inverse, int dtype, void* stream);
 
-/* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down: x [M][D] rows x_stride apart, w_gate and w_up [F][D],
+/* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down: x [M][D] rows x_stride (of one row any) apart, w_gate and w_up [F][D],
  * w_down [N][F], y [M][N], biases [F], [F], [N] or NULL, all of one type.  saved_dev: NULL, or dm_gated_ffn_saved_bytes for the
  * backward pass.  16-bit types round h (but of one or two rows, forward), dg and du to their type between the products, and for the backward
  * pass u act'(g) and act(g) too, unless `activation` holds DM_FFN_KEEP_F32 beside the activation's number in both calls, and `dtype` in
  * dm_gated_ffn_saved_bytes: then these are kept in fp32, 10 bytes per hidden value instead of 6 (gradients: 1.4 times the error of one rounding
  * instead of 1.7).  Of half tensors every value that is rounded has to stay below 65520, or it becomes infinite.  fp32 operands are
- * multiplied as three bf16 terms each, but for passes of few rows (an infinite operand gives NaN there, where fp32 would give an infinity).
+ * multiplied as three bf16 terms each (an infinite operand gives NaN there, where fp32 would give an infinity), but in fp32 instructions in forward
+ * passes of up to 64 rows, and for dh and dx of backward passes of up to 48 rows where the weights are large.
  * Rows of whole 16-byte pieces must start at multiples of 16 bytes. */
 size_t dm_gated_ffn_saved_bytes(int64_t M, int F, int dtype);
 size_t dm_gated_ffn_workspace_bytes(int64_t M, int D, int F, int N, int dtype, int save); /* save: with saved_dev */
