@@ -101,7 +101,7 @@ def _workspace(t, nbytes):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension.  ``weight`` and ``bias`` ([C], either may be
-    missing) are of x's type or fp32.  ``return_stats``: (y, mean, rstd), fp32, for the backward pass."""
+    missing) are both of x's type or both fp32.  ``return_stats``: (y, mean, rstd), fp32, for the backward pass."""
     dt = _dtype(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"layer_norm needs a last dimension to normalise (got {tuple(x.shape)})")

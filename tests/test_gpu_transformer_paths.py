@@ -394,3 +394,16 @@ def test_what_a_forward_pass_keeps():
     assert (y == 1).all() and (dwg == 80 * 2.0 ** 7).all() and (dwd == 80 * 2.0 ** 4).all() and (dwu - 80 * 2.0 ** -20).abs().max() <= 2.0 ** -25
     want = 2.0 ** -3 + 2.0 ** -3  # 8 x dg 2^-13 + 8 x du 2^14
     assert (dx.double() - want).abs().max() <= 2.0 ** -11 * want
+
+
+def test_layer_norm_refuses_parameters_of_two_types():
+    x, w, b = torch.ones(3, 8, dtype=torch.bfloat16, device=DEV), torch.ones(8, dtype=torch.bfloat16, device=DEV), torch.ones(8, device=DEV)
+    for p, q in ((w, b), (b, w)):
+        with pytest.raises(RuntimeError, match="bias must be of type"):
+            d.layer_norm(x, p, q)
+    for p in (w.half(), b.double()):
+        with pytest.raises(RuntimeError, match="weight must be"):
+            d.layer_norm(x, p)
+    _, mu, rs = d.layer_norm(x, b, b, return_stats=True)
+    with pytest.raises(RuntimeError, match="bias must be of type"):
+        d.layer_norm_backward(x, x, b, mu, rs, bias=w)
